@@ -839,6 +839,109 @@ int pcb_keyswitch(PcbCtx* ctx, const uint64_t* d, const uint64_t* c0, int32_t c0
 /* Batched NTT over nrows rows of `x` ([nrows][N]) cycling over the Q primes (row i: prime i mod nq). */
 int pcb_ntt_batch(PcbCtx* ctx, uint64_t* x, int32_t nrows, int32_t inverse, cudaStream_t stream);
 
+/* ================================================================ 4. the clear half of the model */
+
+/* What a client computes in the clear on either side of the encrypted decode: the prompt's pass through the layers that
+ * gives the K and V rows of the caches (linear, attention), the vocabulary loss of hidden states, and the gradients that
+ * fit the head and the MLP to the polynomials of the encrypted step. Operands are 16-bit floats (PCB_BF16 or PCB_F16, one
+ * type per call), products and sums 32-bit. A matrix of r rows and c columns is given by its first element and the pitch
+ * of its rows in elements, columns adjacent. Pointers are device memory except where said. Every call is stream-ordered,
+ * makes no host copy and no sync (it can be captured in a CUDA graph), uses only the caller's workspace (`ws`, 256-byte
+ * aligned, at least the bytes that the matching _ws entry returns; that entry is negative when the arguments are refused)
+ * and returns 0, -1 (arguments refused, pcb_last_error has the reason) or a cudaError_t. Results do not depend on the
+ * order in which blocks run: no floating-point atomics. */
+enum { PCB_BF16 = 0, PCB_F16 = 1, PCB_F32 = 2 };
+enum { PCB_ACT_NONE = 0, PCB_ACT_GELU = 1, PCB_ACT_POLY = 2 };
+
+/* y = act(x w + bias) + residual: x m x k, w k x n, y m x n. w_cols = 0: w's rows (k of them) hold n adjacent elements;
+ * 1: w is given transposed, n rows of k adjacent elements. bias (n) and residual (m x n) may be null and are of the call's
+ * type or 32-bit, as is y. PCB_ACT_GELU: z Phi(z). PCB_ACT_POLY: sum_i coef[i] (z / bound)^i. */
+typedef struct PcbClearLinear {
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* residual;
+    void* y;
+    int64_t x_pitch, w_pitch, residual_pitch, y_pitch;
+    int32_t m, k, n;
+    int32_t type, w_cols, bias_type, residual_type, y_type, act;
+    float bound;
+    float coef[8];
+} PcbClearLinear;
+int64_t pcb_clear_linear_ws(const PcbClearLinear* a);
+int pcb_clear_linear(const PcbClearLinear* a, void* ws, size_t ws_bytes, cudaStream_t s);
+
+/* The gradients of y = act(x w + bias) for dy (m x n): with z = x w + bias (formed again, not kept by the forward call)
+ * and dz = dy act'(z): dx = dz w^T (m x k), dw = x^T dz (in w's own order), db = the sum of dz's rows. dx, dw and db may
+ * be null (not wanted); bias is null where the forward call had none, db then still the sum. */
+typedef struct PcbClearLinearGrad {
+    const void* dy;
+    const void* x;
+    const void* w;
+    const void* bias;
+    void* dx;
+    void* dw;
+    void* db;
+    int64_t dy_pitch, x_pitch, w_pitch, dx_pitch, dw_pitch;
+    int32_t m, k, n;
+    int32_t type, w_cols, bias_type, db_type, act;
+    float bound;
+    float coef[8];
+} PcbClearLinearGrad;
+int64_t pcb_clear_linear_grad_ws(const PcbClearLinearGrad* a);
+int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes, cudaStream_t s);
+
+/* Attention of `nseq` sequences packed along the tokens. Sequence b has q_lens[b] queries, the last of its k_lens[b]
+ * tokens (both HOST arrays, read during the call; sum q_lens = q_rows, sum k_lens = k_rows): query i sees key j iff
+ * j <= i + k_lens[b] - q_lens[b] (causal) or every key of its sequence. q, out: q_rows x heads x dim; k, v: k_rows x
+ * kv_heads x dim, query head h reads K/V head h / (heads / kv_heads). *_pitch: elements between tokens, *_head: between
+ * heads, the dim elements adjacent (dim <= 128). With s = scale <q, k>: ncoef = 0: out = sum softmax(s) v; ncoef = 1..8:
+ * out = sum_j p(s_j) v_j, p(s) = sum_i coef[i] s^i, the encrypted step's weights. A query that sees no key gets zeros. */
+typedef struct PcbClearAttention {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int32_t* q_lens;
+    const int32_t* k_lens;
+    int64_t q_pitch, q_head, k_pitch, k_head, v_pitch, v_head, out_pitch, out_head;
+    int64_t q_rows, k_rows;
+    int32_t nseq, heads, kv_heads, dim;
+    int32_t type, causal, ncoef;
+    float scale;
+    float coef[8];
+} PcbClearAttention;
+int64_t pcb_clear_attention_ws(const PcbClearAttention* a);
+int pcb_clear_attention(const PcbClearAttention* a, void* ws, size_t ws_bytes, cudaStream_t s);
+
+/* Softmax cross entropy of hidden states h (rows x dim) against a vocabulary's rows w (vocab x dim), logits l = h w^T
+ * never stored whole: lse[r] = log sum_v exp(l[r][v]), loss[r] = lse[r] - l[r][targets[r]], 0 where targets[r] = ignore.
+ * Any other target outside [0, vocab) gives a loss of NaN. */
+typedef struct PcbClearVocab {
+    const void* h;
+    const void* w;
+    const int64_t* targets;
+    float* loss;
+    float* lse;
+    int64_t h_pitch, w_pitch, ignore;
+    int32_t rows, vocab, dim, type;
+} PcbClearVocab;
+int64_t pcb_clear_vocab_loss_ws(const PcbClearVocab* a);
+int pcb_clear_vocab_loss(const PcbClearVocab* a, void* ws, size_t ws_bytes, cudaStream_t s);
+
+/* The gradients of sum_r weight[r] loss[r]: dl[r][v] = weight[r] (exp(l[r][v] - lse[r]) - [v = targets[r]]), 0 on ignored
+ * rows; dh = dl w (rows x dim), dw = dl^T h (vocab x dim), formed over pieces of the vocabulary. lse from the forward
+ * call; loss is not read. */
+typedef struct PcbClearVocabGrad {
+    PcbClearVocab v;
+    const float* weight;
+    void* dh;
+    void* dw;
+    int64_t dh_pitch, dw_pitch;
+} PcbClearVocabGrad;
+int64_t pcb_clear_vocab_grad_ws(const PcbClearVocabGrad* a);
+int pcb_clear_vocab_grad(const PcbClearVocabGrad* a, void* ws, size_t ws_bytes, cudaStream_t s);
+
 #ifdef __cplusplus
 }
 #endif
@@ -889,6 +992,11 @@ static_assert(sizeof(PcbAddConstArgs) == 48, "AddConstArgs layout");
 static_assert(sizeof(PcbMulTableArgs) == 72, "MulTableArgs layout");
 static_assert(sizeof(PcbMulAddArgs) == 104, "MulAddArgs layout");
 static_assert(sizeof(PcbMulAddNArgs) == 328, "MulAddNArgs layout");
+static_assert(sizeof(PcbClearLinear) == 144, "ClearLinear layout");
+static_assert(sizeof(PcbClearLinearGrad) == 168, "ClearLinearGrad layout");
+static_assert(sizeof(PcbClearAttention) == 192, "ClearAttention layout");
+static_assert(sizeof(PcbClearVocab) == 80, "ClearVocab layout");
+static_assert(sizeof(PcbClearVocabGrad) == 120, "ClearVocabGrad layout");
 static_assert(sizeof(PcbKernelTable) == 16 + 52 * 8, "KernelTable layout");
 static_assert(sizeof(PcbRingTable) == 16 + 9 * 8, "RingTable layout");
 #endif

@@ -276,6 +276,39 @@ class Params(C.Structure):
                 ("p", u64p), ("k_max", C.c_int32), ("key_source", C.c_int32)]
 
 
+class ClearLinear(C.Structure):
+    _fields_ = [(n, vp) for n in ("x", "w", "bias", "residual", "y")] + [
+        (n, C.c_int64) for n in ("x_pitch", "w_pitch", "residual_pitch", "y_pitch")] + [
+        (n, C.c_int32) for n in ("m", "k", "n", "type", "w_cols", "bias_type", "residual_type", "y_type", "act")] + [
+        ("bound", C.c_float), ("coef", C.c_float * 8)]
+
+
+class ClearLinearGrad(C.Structure):
+    _fields_ = [(n, vp) for n in ("dy", "x", "w", "bias", "dx", "dw", "db")] + [
+        (n, C.c_int64) for n in ("dy_pitch", "x_pitch", "w_pitch", "dx_pitch", "dw_pitch")] + [
+        (n, C.c_int32) for n in ("m", "k", "n", "type", "w_cols", "bias_type", "db_type", "act")] + [
+        ("bound", C.c_float), ("coef", C.c_float * 8)]
+
+
+class ClearAttention(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "out", "q_lens", "k_lens")] + [
+        (n, C.c_int64) for n in ("q_pitch", "q_head", "k_pitch", "k_head", "v_pitch", "v_head", "out_pitch", "out_head",
+                                 "q_rows", "k_rows")] + [
+        (n, C.c_int32) for n in ("nseq", "heads", "kv_heads", "dim", "type", "causal", "ncoef")] + [
+        ("scale", C.c_float), ("coef", C.c_float * 8)]
+
+
+class ClearVocab(C.Structure):
+    _fields_ = [(n, vp) for n in ("h", "w", "targets", "loss", "lse")] + [
+        (n, C.c_int64) for n in ("h_pitch", "w_pitch", "ignore")] + [
+        (n, C.c_int32) for n in ("rows", "vocab", "dim", "type")]
+
+
+class ClearVocabGrad(C.Structure):
+    _fields_ = [("v", ClearVocab), ("weight", vp), ("dh", vp), ("dw", vp), ("dh_pitch", C.c_int64),
+                ("dw_pitch", C.c_int64)]
+
+
 SIZES = {"PrimeConst": 64, "RowSet": 16, "PolyRef": 24, "NttArgs": 176, "BconvJob": 32, "BconvArgs": 56,
          "EwArgs": 128, "KsArgs": 176, "EpiArgs": 72, "KeyTab": 40, "KsRegenArgs": 312, "KskExpandArgs": 48,
          "TensorArgs": 192, "MdEpiArgs": 120, "RescaleArgs": 152, "RescaleCombineArgs": 80, "AutomorphArgs": 112,
@@ -283,7 +316,8 @@ SIZES = {"PrimeConst": 64, "RowSet": 16, "PolyRef": 24, "NttArgs": 176, "BconvJo
          "MulAddArgs": 104, "MulAddNArgs": 328, "ModRaiseArgs": 2136, "TensorYArgs": 240, "CtsArgs": 200, "PackSplitArgs": 64, "CoeffArgs": 80 + 16 * 32, "PackDotArgs": 120, "CtsRegenArgs": 240, "SmallInt1Args": 56, "RescaleNttArgs": 328,
          "RescaleCombineToArgs": 104, "MdEpiToArgs": 152, "WsumArgs": 256, "WsumKArgs": 264, "WsumMultiArgs": 376,
          "EwManyArgs": 4 * 48 * 8 + 16, "SubMulManyArgs": 3 * 48 * 8 + 24, "TensorSumArgs": 2 * 24 + 2 * 16 * 24 + 24,
-         "TensorMultiArgs": (2 * 4 + 2 * 4 * 32) * 24 + 32, "KernelTable": 16 + 52 * 8, "RingTable": 16 + 9 * 8}
+         "TensorMultiArgs": (2 * 4 + 2 * 4 * 32) * 24 + 32, "KernelTable": 16 + 52 * 8, "RingTable": 16 + 9 * 8,
+         "ClearLinear": 144, "ClearLinearGrad": 168, "ClearAttention": 192, "ClearVocab": 80, "ClearVocabGrad": 120}
 
 _lib = None
 
@@ -358,6 +392,10 @@ def lib():
         "pcb_mod_raise": (C.c_int, [vp, vp, i32, i32, vp]),
         "pcb_ntt_batch": (C.c_int, [vp, vp, i32, i32, vp]),
     }
+    for op, st in (("linear", ClearLinear), ("linear_grad", ClearLinearGrad), ("attention", ClearAttention),
+                   ("vocab_loss", ClearVocab), ("vocab_grad", ClearVocabGrad)):
+        sig[f"pcb_clear_{op}_ws"] = (i64, [C.POINTER(st)])
+        sig[f"pcb_clear_{op}"] = (C.c_int, [C.POINTER(st), vp, C.c_size_t, vp])
     for name, (res, args) in sig.items():
         f = getattr(L, name)
         f.restype = res

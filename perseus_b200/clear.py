@@ -1,0 +1,265 @@
+"""The clear half of the model: what a client computes on its own side of the encrypted decode, as CUDA operators.
+
+The encrypted decoder (perseus_b200.model.Decoder.load) starts from the K and V rows of the client's prompt and ends at a
+hidden state. Before it, the prompt's pass through the layers in the clear: `linear` (projections and MLP, with bias,
+activation and residual) and `prompt_attention` (whole prompts packed along the tokens, with softmax or with the
+polynomial weights that the encrypted step evaluates). After it, the score of hidden states against a vocabulary,
+`vocab_loss`. `vocab_loss_grad` and `linear_grad` give the gradients that fit the head and the MLP to the polynomials.
+perseus_b200.prefill runs them together.
+
+Operands are CUDA tensors of torch.bfloat16 or torch.float16 (one type per call), sums are 32-bit, results are rounded
+once. Every call runs on the current stream, without a host copy or sync. Results are plain tensors: nothing is recorded
+for autograd.
+"""
+import ctypes as C
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib as L
+
+_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NO_COEF = (C.c_float * 8)()
+
+
+@dataclass(frozen=True)
+class Poly:
+    """The activation sum_i coeffs[i] (z / bound)^i, at most 8 coefficients: model.gelu_poly(bound) gives the encrypted
+    MLP's."""
+
+    coeffs: tuple
+    bound: float = 1.0
+
+    def __post_init__(self):
+        object.__setattr__(self, "coeffs", tuple(float(c) for c in self.coeffs))
+        if not 1 <= len(self.coeffs) <= 8 or not all(map(math.isfinite, self.coeffs)):
+            raise ValueError(f"Poly: 1 to 8 finite coefficients, got {self.coeffs}")
+        if not (self.bound > 0 and math.isfinite(self.bound)):
+            raise ValueError(f"Poly: bound {self.bound}")
+        object.__setattr__(self, "_c", (C.c_float * 8)(*self.coeffs))
+
+
+def _act(act):
+    if act is None:
+        return 0, 1.0, _NO_COEF
+    if isinstance(act, Poly):
+        return 2, act.bound, act._c
+    if act == "gelu":
+        return 1, 1.0, _NO_COEF
+    raise ValueError(f"act {act!r}: None, 'gelu' or a Poly")
+
+
+def _is(name, t, like, dims):
+    """t: a CUDA tensor of `like`'s device, 16-bit (or of like's type) with `dims` dimensions."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise ValueError(f"{name}: a CUDA tensor, got {t.device if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if t.dim() != dims:
+        raise ValueError(f"{name}: {dims} dimensions, got shape {tuple(t.shape)}")
+    if like is None:
+        if t.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"{name}: bfloat16 or float16, got {t.dtype}")
+    elif t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name}: {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+
+
+def _aside(name, t, like, shape):
+    """An optional operand of like's type or float32."""
+    if t.shape != shape or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+        raise ValueError(f"{name}: {tuple(shape)} of {like.dtype} or float32 on {like.device}, got {tuple(t.shape)} of "
+                         f"{t.dtype} on {t.device}")
+
+
+def _rows(t):
+    """t with adjacent columns and rows that do not overlap (a copy where it is not so)."""
+    r, c = t.shape
+    if (t.stride(1) == 1 or c == 1) and (t.stride(0) >= c or r == 1):
+        return t
+    return t.contiguous()
+
+
+def _pitch(t):
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _weight(w):
+    """(w, its rows' pitch, whether its memory is the transposed matrix)."""
+    k, n = w.shape
+    if w.stride(1) == 1 and w.stride(0) >= n:
+        return w, w.stride(0), 0
+    if w.stride(0) == 1 and w.stride(1) >= k:
+        return w, w.stride(1), 1
+    return w.contiguous(), n, 0
+
+
+def _launch(op, args, device):
+    lib = L.lib()
+    with torch.cuda.device(device):
+        need = getattr(lib, f"pcb_clear_{op}_ws")(args)
+        if need < 0:
+            L.check(int(need), f"pcb_clear_{op}")
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        L.check(getattr(lib, f"pcb_clear_{op}")(args, ws.data_ptr() if need else None, need,
+                                                 torch.cuda.current_stream(device).cuda_stream), f"pcb_clear_{op}")
+
+
+def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
+    """act(x w + bias) + residual for x [..., k], w [k, n] (a transposed view of an [n, k] matrix is read as it lies).
+    act: None, "gelu" (z Phi(z)) or a Poly. bias [n] and residual [..., n] are of x's type or float32; the result is of
+    `out_dtype`: x's type (default) or float32."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("linear: x is a CUDA tensor [..., k]")
+    lead = x.shape[:-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    _is("x", x2, None, 2)
+    _is("w", w, x, 2)
+    m, k = x2.shape
+    n = w.shape[1]
+    if w.shape[0] != k or k < 1:
+        raise ValueError(f"linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"linear: out_dtype {out_dtype}: {x.dtype} or float32")
+    kind, bound, coef = _act(act)
+    if bias is not None:
+        _aside("bias", bias, x, (n,))
+        bias = bias.contiguous()
+    if residual is not None:
+        _aside("residual", residual, x, lead + (n,))
+        residual = _rows(residual if x.dim() == 2 else residual.reshape(-1, n))
+    x2 = _rows(x2)
+    wm, w_pitch, w_cols = _weight(w)
+    y = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    if m and n:
+        t = _TYPE[x.dtype]
+        _launch("linear", L.ClearLinear(
+            x2.data_ptr(), wm.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(), y.data_ptr(), _pitch(x2), w_pitch,
+            n if residual is None else _pitch(residual), n, m, k, n, t, w_cols, t if bias is None else _TYPE[bias.dtype],
+            t if residual is None else _TYPE[residual.dtype], _TYPE[out_dtype], kind, bound, coef), x.device)
+    return y if x.dim() == 2 else y.reshape(lead + (n,))
+
+
+def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
+    """The gradients (dx, dw, db) of linear(x, w, bias, act) for the gradient dy [..., n] of its result (a residual's
+    gradient is dy itself). The product x w + bias is formed again where there is an activation, so the forward call keeps
+    nothing. dx is of x's shape, dw of w's (laid out as w is), both of x's type; db [n] is of bias's type, None without a
+    bias. needs: which of the three are wanted, the others are None."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("linear_grad: x is a CUDA tensor [..., k]")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    _is("x", x2, None, 2)
+    _is("w", w, x, 2)
+    m, k = x2.shape
+    n = w.shape[1]
+    if w.shape[0] != k or k < 1 or n < 1:
+        raise ValueError(f"linear_grad: x {tuple(x.shape)} against w {tuple(w.shape)}")
+    if not isinstance(dy, torch.Tensor) or dy.shape != x.shape[:-1] + (n,):
+        raise ValueError(f"linear_grad: dy of shape {tuple(x.shape[:-1]) + (n,)}")
+    dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n)
+    _is("dy", dy2, x, 2)
+    kind, bound, coef = _act(act)
+    if bias is not None:
+        _aside("bias", bias, x, (n,))
+        bias = bias.contiguous()
+    x2, dy2 = _rows(x2), _rows(dy2)
+    wm, w_pitch, w_cols = _weight(w)
+    dev, t = x.device, _TYPE[x.dtype]
+    dx = torch.empty((m, k), dtype=x.dtype, device=dev) if needs[0] else None
+    dw = None
+    if needs[1]:
+        dw = torch.empty((n, k), dtype=x.dtype, device=dev).t() if w_cols else torch.empty((k, n), dtype=x.dtype, device=dev)
+    db = torch.empty(n, dtype=bias.dtype, device=dev) if needs[2] and bias is not None else None
+    if dx is not None or dw is not None or db is not None:
+        _launch("linear_grad", L.ClearLinearGrad(
+            dy2.data_ptr(), x2.data_ptr(), wm.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+            None if db is None else db.data_ptr(), _pitch(dy2), _pitch(x2), w_pitch, k, k if w_cols else n, m, k, n, t,
+            w_cols, t if bias is None else _TYPE[bias.dtype], t if db is None else _TYPE[db.dtype], kind, bound, coef), dev)
+    if dx is not None and x.dim() != 2:
+        dx = dx.reshape(x.shape)
+    return dx, dw, db
+
+
+def prompt_attention(q, k, v, q_lens, k_lens=None, scale=None, causal=True, weights=None):
+    """Attention of sequences packed along the tokens: q [sum q_lens, heads, dim], k and v [sum k_lens, kv_heads, dim],
+    heads a multiple of kv_heads (query head h reads K/V head h // (heads / kv_heads)), dim <= 128. q_lens, k_lens: the
+    sequences' lengths on the host; k_lens defaults to q_lens, a longer one means that the queries are the sequence's last
+    tokens (a single token against a cache has q_lens 1). Causal: query i sees key j iff j <= i + k_len - q_len; a query
+    that sees nothing gets zeros. scale defaults to 1 / sqrt(dim). weights: None for softmax, or the coefficients c_0..c_7
+    of the polynomial that stands in for it (attention.softmax_poly): sum_j p(s_j) v_j, not normalised, as the encrypted
+    step computes it."""
+    _is("q", q, None, 3)
+    _is("k", k, q, 3)
+    _is("v", v, q, 3)
+    q_rows, heads, dim = q.shape
+    k_rows, kv_heads = k.shape[:2]
+    if k.shape[2] != dim or v.shape != k.shape:
+        raise ValueError(f"prompt_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if not 1 <= dim <= 128 or kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= 128:
+        raise ValueError(f"prompt_attention: {heads} heads over {kv_heads}, dim {dim} (a multiple, at most 128 to one; 1..128)")
+    k_lens = q_lens if k_lens is None else k_lens
+    nseq = len(q_lens)
+    if len(k_lens) != nseq:
+        raise ValueError(f"prompt_attention: {nseq} q_lens, {len(k_lens)} k_lens")
+    coef = () if weights is None else tuple(weights)
+    if weights is not None and not 1 <= len(coef) <= 8:
+        raise ValueError(f"prompt_attention: 1 to 8 coefficients, got {len(coef)}")
+    out = torch.empty((q_rows, heads, dim), dtype=q.dtype, device=q.device)
+    q, k, v = (t if t.stride(2) == 1 or dim == 1 else t.contiguous() for t in (q, k, v))
+    lens = C.c_int32 * nseq
+    ql, kl = lens(*q_lens), lens(*k_lens)
+    args = L.ClearAttention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.addressof(ql), C.addressof(kl), q.stride(0),
+        q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), heads * dim, dim, q_rows, k_rows, nseq, heads,
+        kv_heads, dim, _TYPE[q.dtype], int(causal), len(coef), 1.0 / math.sqrt(dim) if scale is None else scale,
+        (C.c_float * 8)(*coef))
+    _launch("attention", args, q.device)
+    return out
+
+
+def _vocab_args(who, h, w, targets, lse, loss, ignore):
+    _is("h", h, None, 2)
+    _is("w", w, h, 2)
+    rows, dim = h.shape
+    if w.shape[1] != dim or dim < 1 or w.shape[0] < 1:
+        raise ValueError(f"{who}: h {tuple(h.shape)} against w {tuple(w.shape)}")
+    if targets.shape != (rows,) or targets.dtype != torch.int64 or targets.device != h.device:
+        raise ValueError(f"{who}: targets of shape ({rows},) in int64 on {h.device}, got {tuple(targets.shape)} of "
+                         f"{targets.dtype} on {targets.device}")
+    h, w, targets = _rows(h), _rows(w), targets.contiguous()
+    args = L.ClearVocab(h.data_ptr(), w.data_ptr(), targets.data_ptr(), None if loss is None else loss.data_ptr(),
+                        lse.data_ptr(), _pitch(h), _pitch(w), ignore, rows, w.shape[0], dim, _TYPE[h.dtype])
+    return args, (h, w, targets)
+
+
+def vocab_loss(h, w, targets, ignore=-100):
+    """Softmax cross entropy of hidden states h [rows, dim] against the vocabulary w [vocab, dim]: (loss, lse), both
+    [rows] in float32, lse = log sum_v exp(<h, w_v>), loss = lse - <h, w_target>, 0 where the target is `ignore` (any
+    other target outside the vocabulary gives NaN). The logits are never stored whole."""
+    rows = h.shape[0] if isinstance(h, torch.Tensor) and h.dim() == 2 else 0
+    loss = torch.empty(rows, dtype=torch.float32, device=h.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=h.device)
+    args, keep = _vocab_args("vocab_loss", h, w, targets, lse, loss, ignore)
+    if rows:
+        _launch("vocab_loss", args, h.device)
+    return loss, lse
+
+
+def vocab_loss_grad(h, w, targets, lse, weight, ignore=-100, needs=(True, True)):
+    """The gradients (dh, dw), of h's and w's shape and type, of sum_r weight[r] loss[r] (weight [rows] float32: 1 /
+    count for the mean); lse from vocab_loss on the same h and w. The logits are formed again, a piece of the vocabulary
+    at a time. needs: which of the two are wanted, the other is None."""
+    args, keep = _vocab_args("vocab_loss_grad", h, w, targets, lse, None, ignore)
+    rows, dim = h.shape
+    for name, t in (("lse", lse), ("weight", weight)):
+        if t.shape != (rows,) or t.dtype != torch.float32 or t.device != h.device:
+            raise ValueError(f"vocab_loss_grad: {name} of shape ({rows},) in float32 on {h.device}")
+    lse, weight = lse.contiguous(), weight.contiguous()
+    args.lse = lse.data_ptr()
+    dh = torch.empty((rows, dim), dtype=h.dtype, device=h.device) if needs[0] else None
+    dw = torch.empty((w.shape[0], dim), dtype=h.dtype, device=h.device) if needs[1] else None
+    if dh is not None or dw is not None:
+        _launch("vocab_grad", L.ClearVocabGrad(args, weight.data_ptr(), None if dh is None else dh.data_ptr(),
+                                               None if dw is None else dw.data_ptr(), dim, dim), h.device)
+    return dh, dw

@@ -1,0 +1,182 @@
+// Shared by the clear half's translation units (clear_*.cu): 16-bit element access, argument checks, the workspace.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "arith.cuh"
+#include "kernels.h"
+
+namespace pcb {
+// records the message of pcb_last_error and returns `code` (evaluator.cu)
+int report(int code, const char* fmt, ...);
+
+namespace clear {
+
+// ------------------------------------------------------------------------------------------------ elements
+// Element i of a PCB_BF16 / PCB_F16 / PCB_F32 array in 32 bits, and back with one rounding
+__device__ __forceinline__ float load(const void* p, size_t i, int type) {
+    if (type == PCB_F32) return ((const float*)p)[i];
+    return type == PCB_BF16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : __half2float(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void store(void* p, size_t i, int type, float v) {
+    if (type == PCB_F32) ((float*)p)[i] = v;
+    else if (type == PCB_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16(v);
+    else ((__half*)p)[i] = __float2half(v);
+}
+inline size_t type_bytes(int type) { return type == PCB_F32 ? 4 : 2; }
+
+// ------------------------------------------------------------------------------------------------ activations
+struct Act {
+    int kind;
+    float inv_bound;
+    float c[8];
+};
+inline Act make_act(int kind, float bound, const float* coef) {
+    Act a;
+    a.kind = kind;
+    a.inv_bound = kind == PCB_ACT_POLY ? 1.0f / bound : 1.0f;
+    for (int i = 0; i < 8; ++i) a.c[i] = kind == PCB_ACT_POLY ? coef[i] : 0.0f;
+    return a;
+}
+__device__ __forceinline__ float act(const Act& a, float z) {
+    if (a.kind == PCB_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if (a.kind == PCB_ACT_POLY) {
+        const float u = z * a.inv_bound;
+        float r = a.c[7];
+#pragma unroll
+        for (int i = 6; i >= 0; --i) r = fmaf(r, u, a.c[i]);
+        return r;
+    }
+    return z;
+}
+__device__ __forceinline__ float act_slope(const Act& a, float z) {
+    if (a.kind == PCB_ACT_GELU)  // Phi(z) + z phi(z)
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * expf(-0.5f * z * z);
+    if (a.kind == PCB_ACT_POLY) {
+        const float u = z * a.inv_bound;
+        float r = 7.0f * a.c[7];
+#pragma unroll
+        for (int i = 6; i >= 1; --i) r = fmaf(r, u, (float)i * a.c[i]);
+        return r * a.inv_bound;
+    }
+    return 1.0f;
+}
+
+// ------------------------------------------------------------------------------------------------ checks
+inline bool is16(int type) { return type == PCB_BF16 || type == PCB_F16; }
+inline bool known(int type, int call) { return type == call || type == PCB_F32; }
+inline bool poly_ok(int kind, float bound, const float* coef) {
+    if (kind != PCB_ACT_POLY) return true;
+    if (!(bound > 0.0f) || !std::isfinite(bound)) return false;
+    for (int i = 0; i < 8; ++i)
+        if (!std::isfinite(coef[i])) return false;
+    return true;
+}
+inline int bad_linear(const PcbClearLinear* a) {
+    if (!a) return report(PCB_BAD_ARGS, "clear_linear: null arguments");
+    if (a->m < 0 || a->k < 1 || a->n < 0) return report(PCB_BAD_ARGS, "clear_linear: m %d, k %d, n %d", a->m, a->k, a->n);
+    if (!is16(a->type)) return report(PCB_BAD_ARGS, "clear_linear: type %d is not PCB_BF16 or PCB_F16", a->type);
+    if (a->act < 0 || a->act > PCB_ACT_POLY || !poly_ok(a->act, a->bound, a->coef))
+        return report(PCB_BAD_ARGS, "clear_linear: act %d, bound %g", a->act, (double)a->bound);
+    if ((a->bias && !known(a->bias_type, a->type)) || (a->residual && !known(a->residual_type, a->type)) ||
+        !known(a->y_type, a->type))
+        return report(PCB_BAD_ARGS, "clear_linear: bias, residual and y are of the call's type or PCB_F32");
+    if (a->m == 0 || a->n == 0) return 0;
+    if (!a->x || !a->w || !a->y) return report(PCB_BAD_ARGS, "clear_linear: null x, w or y");
+    if (a->x_pitch < a->k || a->w_pitch < (a->w_cols ? a->k : a->n) || a->y_pitch < a->n ||
+        (a->residual && a->residual_pitch < a->n))
+        return report(PCB_BAD_ARGS, "clear_linear: a pitch is below its row's elements");
+    return 0;
+}
+inline int bad_grad(const PcbClearLinearGrad* a) {
+    if (!a) return report(PCB_BAD_ARGS, "clear_linear_grad: null arguments");
+    if (a->m < 0 || a->k < 1 || a->n < 1)
+        return report(PCB_BAD_ARGS, "clear_linear_grad: m %d, k %d, n %d", a->m, a->k, a->n);
+    if (!is16(a->type)) return report(PCB_BAD_ARGS, "clear_linear_grad: type %d is not PCB_BF16 or PCB_F16", a->type);
+    if (a->act < 0 || a->act > PCB_ACT_POLY || !poly_ok(a->act, a->bound, a->coef))
+        return report(PCB_BAD_ARGS, "clear_linear_grad: act %d, bound %g", a->act, (double)a->bound);
+    if ((a->bias && !known(a->bias_type, a->type)) || (a->db && !known(a->db_type, a->type)))
+        return report(PCB_BAD_ARGS, "clear_linear_grad: bias and db are of the call's type or PCB_F32");
+    if (a->m > 0 && (!a->dy || !a->x || !a->w)) return report(PCB_BAD_ARGS, "clear_linear_grad: null dy, x or w");
+    const int64_t wrow = a->w_cols ? a->k : a->n;
+    if ((a->m > 0 && (a->dy_pitch < a->n || a->x_pitch < a->k || a->w_pitch < wrow)) || (a->dx && a->dx_pitch < a->k) ||
+        (a->dw && a->dw_pitch < wrow))
+        return report(PCB_BAD_ARGS, "clear_linear_grad: a pitch is below its row's elements");
+    return 0;
+}
+inline int bad_attention(const PcbClearAttention* a) {
+    if (!a) return report(PCB_BAD_ARGS, "clear_attention: null arguments");
+    if (a->nseq < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->heads / a->kv_heads > 128 ||
+        a->dim < 1 || a->dim > 128)
+        return report(PCB_BAD_ARGS, "clear_attention: %d sequences, %d heads over %d (a multiple, at most 128 each), dim %d (1..128)",
+                      a->nseq, a->heads, a->kv_heads, a->dim);
+    if (!is16(a->type)) return report(PCB_BAD_ARGS, "clear_attention: type %d is not PCB_BF16 or PCB_F16", a->type);
+    if (a->ncoef < 0 || a->ncoef > 8 || !std::isfinite(a->scale))
+        return report(PCB_BAD_ARGS, "clear_attention: %d coefficients (0..8), scale %g", a->ncoef, (double)a->scale);
+    for (int i = 0; i < a->ncoef; ++i)
+        if (!std::isfinite(a->coef[i])) return report(PCB_BAD_ARGS, "clear_attention: coefficient %d is not finite", i);
+    if (a->nseq > 0 && (!a->q_lens || !a->k_lens)) return report(PCB_BAD_ARGS, "clear_attention: null lengths");
+    if (a->q_rows > INT32_MAX || a->k_rows > INT32_MAX)
+        return report(PCB_BAD_ARGS, "clear_attention: over 2^31 - 1 tokens");
+    int64_t qs = 0, ks = 0;
+    for (int b = 0; b < a->nseq; ++b) {
+        if (a->q_lens[b] < 0 || a->k_lens[b] < 0)
+            return report(PCB_BAD_ARGS, "clear_attention: sequence %d has %d queries, %d keys", b, a->q_lens[b], a->k_lens[b]);
+        qs += a->q_lens[b];
+        ks += a->k_lens[b];
+    }
+    if (qs != a->q_rows || ks != a->k_rows)
+        return report(PCB_BAD_ARGS, "clear_attention: lengths sum to %lld and %lld, q has %lld rows and k %lld", (long long)qs,
+                      (long long)ks, (long long)a->q_rows, (long long)a->k_rows);
+    if ((qs && (!a->q || !a->out)) || (qs && ks && (!a->k || !a->v)))
+        return report(PCB_BAD_ARGS, "clear_attention: null q, k, v or out");
+    const int64_t strides[] = {a->q_pitch, a->q_head, a->k_pitch, a->k_head, a->v_pitch, a->v_head, a->out_pitch, a->out_head};
+    for (int64_t st : strides)
+        if (st < 0) return report(PCB_BAD_ARGS, "clear_attention: negative stride");
+    return 0;
+}
+inline int bad_vocab(const PcbClearVocab* a, bool grad) {
+    const char* who = grad ? "clear_vocab_grad" : "clear_vocab_loss";
+    if (!a) return report(PCB_BAD_ARGS, "%s: null arguments", who);
+    if (a->rows < 0 || a->vocab < 1 || a->dim < 1)
+        return report(PCB_BAD_ARGS, "%s: %d rows, vocabulary of %d, dim %d", who, a->rows, a->vocab, a->dim);
+    if (!is16(a->type)) return report(PCB_BAD_ARGS, "%s: type %d is not PCB_BF16 or PCB_F16", who, a->type);
+    if (a->rows > 0 && (!a->h || !a->w || !a->targets || !a->lse || (!grad && !a->loss)))
+        return report(PCB_BAD_ARGS, "%s: null h, w, targets, lse or loss", who);
+    if (a->rows > 0 && (a->h_pitch < a->dim || a->w_pitch < a->dim))
+        return report(PCB_BAD_ARGS, "%s: a pitch is below its row's elements", who);
+    return 0;
+}
+inline int bad_vocab_grad(const PcbClearVocabGrad* a) {
+    if (!a) return report(PCB_BAD_ARGS, "clear_vocab_grad: null arguments");
+    if (int rc = bad_vocab(&a->v, true)) return rc;
+    if (a->v.rows > 0 && !a->weight) return report(PCB_BAD_ARGS, "clear_vocab_grad: null weight");
+    if ((a->dh && a->dh_pitch < a->v.dim) || (a->dw && a->dw_pitch < a->v.dim))
+        return report(PCB_BAD_ARGS, "clear_vocab_grad: a pitch is below its row's elements");
+    return 0;
+}
+
+// ------------------------------------------------------------------------------------------------ workspace
+// Carves 256-byte aligned pieces off the caller's workspace; with a null base it only counts.
+struct Carve {
+    char* base;
+    size_t used = 0;
+    explicit Carve(void* p) : base((char*)p) {}
+    template <class T>
+    T* take(size_t n) {
+        T* r = base ? (T*)(base + used) : nullptr;
+        used += (n * sizeof(T) + 255) / 256 * 256;
+        return r;
+    }
+};
+inline int bad_ws(const char* who, const void* ws, size_t have, size_t need) {
+    if (need && (!ws || have < need || ((uintptr_t)ws & 255)))
+        return report(PCB_BAD_ARGS, "%s: workspace of %zu bytes at %p, %zu at a 256-byte boundary needed", who, have, ws, need);
+    return 0;
+}
+
+}  // namespace clear
+}  // namespace pcb

@@ -866,6 +866,19 @@ int launch_mul_pt(PcbCtx& c, const uint64_t* x, const uint64_t* pt, const uint64
 
 }  // namespace
 
+// the message of pcb_last_error for the other translation units' entries (clear.h)
+namespace pcb {
+int report(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return code;
+}
+}  // namespace pcb
+
 // ================================================================================================ C API
 extern "C" {
 
