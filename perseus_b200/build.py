@@ -12,8 +12,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpcb200.so")
-SOURCES = ["ntt.cu", "elem.cu", "pt.cu", "ks.cu", "regen.cu", "keys.cu", "table.cu", "evaluator.cu", "probe.cu", "wire.cu", "elem_multi.cu", "cts.cu", "clear.cu"]
-HEADERS = ["arith.cuh", "chacha.cuh", "keyregen.cuh", "kernels.h", "host_math.h", "ntt_pipe.cuh", "clear.h"]
+SOURCES = ["ntt.cu", "elem.cu", "pt.cu", "ks.cu", "regen.cu", "keys.cu", "table.cu", "evaluator.cu", "probe.cu", "wire.cu", "elem_multi.cu", "cts.cu", "clear.cu", "clear_gemm.cu", "clear_attn.cu"]
+HEADERS = ["arith.cuh", "chacha.cuh", "keyregen.cuh", "kernels.h", "host_math.h", "ntt_pipe.cuh", "clear.h", "clear_gemm.h", "mma.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

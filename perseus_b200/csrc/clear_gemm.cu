@@ -1,0 +1,577 @@
+// The clear half's matrix product on the fifth-generation tensor cores.
+//
+// One persistent block per SM walks 128 x BN output tiles. Warp 0 streams the operands' 64-k blocks through a ring of
+// shared-memory stages with the TMA engine (either operand may have k or its rows adjacent in memory: the instruction
+// descriptor says which, nothing is transposed on the way); warp 1 issues the products (tcgen05.mma, 128 x BN x 16) into
+// one of two TMEM accumulators; the other warps take the finished accumulator out of TMEM, apply the epilogue in 32 bits
+// and store through shared memory, while the next tile's products run.
+//
+// Waits are bounded (mma::wait): a role that gives up tells the others, the loads and products in flight are waited for
+// (bounded as well), TMEM is freed and the block ends; pcb_device_timeouts counts it.
+#include "clear_gemm.h"
+
+#include <cstring>
+
+#include "mma.cuh"
+
+namespace pcb {
+namespace clear {
+
+using namespace mma;
+
+__device__ unsigned int g_gemm_timeouts;
+
+namespace {
+
+constexpr int SMS = 148;
+constexpr int BM = 128, BK = 64;
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int BN>
+struct Shape {
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int EWARPS = BN == 64 ? 4 : 8;         // epilogue warps: 4 cover the 128 lanes, 8 halve the columns
+    static constexpr int COLS = BN / (EWARPS / 4);          // columns of one epilogue warp
+    static constexpr int THREADS = 64 + 32 * EWARPS;
+    static constexpr int TMEM = 2 * BN;
+    static constexpr int STAGING = 4096;                    // per epilogue warp: 32 rows x 128 bytes
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EWARPS * (STAGING + 128) + 256;
+};
+
+struct alignas(64) Params {
+    CUtensorMap a, b, y;
+    int m, n, k;
+    int a_mn, b_mn, bf16;
+    int tiles_m, tiles_n, splits, kblocks, kper;  // k blocks in all and of one split
+    Act act;
+    const void* bias;
+    const void* extra;
+    void* y_ptr;
+    int64_t extra_pitch, y_pitch;
+    int bias_type, extra_type, y_type, y_tma, accumulate;
+    const float* alpha;
+    float* row_sums;
+    const VocabRow* rows;
+    int col0;
+    const int64_t* targets;
+    float2* parts;
+    float* hit;
+};
+
+// ------------------------------------------------------------------------------------------------ epilogue pieces
+// z Phi(z) and its derivative. Phi from Abramowitz and Stegun 7.1.26 (absolute error below 1.5e-7 in erf): for x = |z| /
+// sqrt 2, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x). One reciprocal and one exponential.
+__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = rcp(fmaf(0.3275911f, x, 1.0f));
+    const float e = ex2(-LOG2E * x * x);
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float half = 0.5f * p * t * e;
+    *gauss = e;
+    return z < 0.0f ? half : 1.0f - half;
+}
+__device__ __forceinline__ void apply_act(const Act& a, float* v) {
+    if (a.kind == PCB_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float g;
+            v[j] *= normal_cdf(v[j], &g);
+        }
+    } else if (a.kind == PCB_ACT_POLY) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float u = v[j] * a.inv_bound;
+            float r = a.c[7];
+#pragma unroll
+            for (int i = 6; i >= 0; --i) r = fmaf(r, u, a.c[i]);
+            v[j] = r;
+        }
+    }
+}
+__device__ __forceinline__ void apply_slope(const Act& a, float* v) {
+    if (a.kind == PCB_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float g;
+            const float c = normal_cdf(v[j], &g);
+            v[j] = fmaf(v[j] * 0.3989422804014327f, g, c);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = act_slope(a, v[j]);
+    }
+}
+
+// Sum over the warp's lanes of each of 32 values: lane l returns the sum of v[l], in a fixed order
+__device__ __forceinline__ float lane_sums(float* v) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int j = 0; j < w; ++j) {
+            const float keep = up ? v[j + w] : v[j], give = up ? v[j] : v[j + w];
+            v[j] = keep + __shfl_xor_sync(~0u, give, w);
+        }
+    }
+    return v[0];
+}
+
+// 32 x 32 values of a row-major array at (row0, col0), rows and columns past the end as zero, to the lane's row: read
+// along the rows (lane = column), turned through the warp's staging buffer
+__device__ __forceinline__ void load_block(const void* p, int64_t pitch, int type, int row0, int col0, int m, int n, float* stage,
+                                           float* out) {
+    const int lane = threadIdx.x % 32;
+    const bool in = col0 + lane < n;
+    float t[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) t[r] = in && row0 + r < m ? load(p, (int64_t)(row0 + r) * pitch + col0 + lane, type) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) stage[r * 32 + (lane ^ r)] = t[r];
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 32; ++c) out[c] = stage[lane * 32 + (c ^ lane)];
+    __syncwarp();
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel
+template <int BN, int EPI>
+__global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_constant__ Params p) {
+    using S = Shape<BN>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* base = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* staging = base + S::STAGES * S::STAGE;
+    float* bias_s = (float*)(staging + S::EWARPS * S::STAGING);
+    uint64_t* full = (uint64_t*)(bias_s + S::EWARPS * 32);
+    uint64_t* empty = full + S::STAGES;
+    uint64_t* acc_full = empty + S::STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_at = (uint32_t*)(drain + 1);
+    volatile int* dead = (volatile int*)(tmem_at + 1);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], S::EWARPS);
+        }
+        mbar_init(drain, 1);
+        mbar_init_fence();
+        *dead = 0;
+        prefetch_map(&p.a);
+        prefetch_map(&p.b);
+    }
+    if (warp == 1) tmem_alloc(tmem_at, S::TMEM);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_at;
+    pdl_wait();
+    pdl_release();
+
+    const int tiles = p.tiles_m * p.tiles_n * p.splits;
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int tile = blockIdx.x; tile < tiles && !*dead; tile += gridDim.x) {
+                const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
+                const int m0 = mn % p.tiles_m * BM, n0 = mn / p.tiles_m * BN;
+                const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int st = it % S::STAGES;
+                    if (it >= S::STAGES && !wait(&empty[st], (it / S::STAGES - 1) & 1, dead, &g_gemm_timeouts)) break;
+                    unsigned char* sa = base + st * S::STAGE;
+                    unsigned char* sb = sa + S::A_BYTES;
+                    mbar_expect(&full[st], S::STAGE);
+                    if (p.a_mn) {
+                        for (int j = 0; j < BM / 64; ++j) tma_load(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK, &full[st]);
+                    } else {
+                        tma_load(sa, &p.a, kb * BK, m0, &full[st]);
+                    }
+                    if (p.b_mn) {
+                        for (int j = 0; j < BN / 64; ++j) tma_load(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK, &full[st]);
+                    } else {
+                        tma_load(sb, &p.b, kb * BK, n0, &full[st]);
+                    }
+                }
+            }
+            if (*dead)  // the loads in flight
+                for (int i = max(0, it - S::STAGES); i < it; ++i) mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = instr_desc(p.bf16, p.a_mn, p.b_mn, BM, BN);
+            const uint32_t a_lbo = p.a_mn ? 8192 : 16, a_step = (p.a_mn ? 2048 : 32) >> 4;
+            const uint32_t b_lbo = p.b_mn ? 8192 : 16, b_step = (p.b_mn ? 2048 : 32) >> 4;
+            int it = 0, t = 0;
+            for (int tile = blockIdx.x; tile < tiles && !*dead; tile += gridDim.x, ++t) {
+                const int sp = tile / (p.tiles_m * p.tiles_n);
+                const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
+                const int buf = t & 1;
+                if (t >= 2 && !wait(&acc_empty[buf], (t / 2 - 1) & 1, dead, &g_gemm_timeouts)) break;
+                fence_after();
+                const uint32_t acc = tmem + buf * BN;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int st = it % S::STAGES;
+                    if (!wait(&full[st], (it / S::STAGES) & 1, dead, &g_gemm_timeouts)) break;
+                    fence_after();
+                    const uint32_t sa = smem_addr(base + st * S::STAGE);
+                    const uint64_t da = smem_desc(sa, a_lbo, 1024), db = smem_desc(sa + S::A_BYTES, b_lbo, 1024);
+#pragma unroll
+                    for (int q = 0; q < BK / 16; ++q) mma_ss(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
+                    mma_commit(&empty[st]);
+                }
+                mma_commit(&acc_full[buf]);
+            }
+            if (*dead) {  // the products in flight
+                mma_commit(drain);
+                mbar_wait(drain, 0);
+            }
+        }
+    } else {
+        const int ew = warp - 2, quad = warp % 4, half = ew / 4;
+        unsigned char* stage = staging + ew * S::STAGING;
+        float* bias = bias_s + ew * 32;
+        const float alpha = p.alpha ? *p.alpha : 1.0f;
+        int t = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+            const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
+            const int m0 = mn % p.tiles_m * BM, tn = mn / p.tiles_m, n0 = tn * BN;
+            const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
+            if (!wait(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
+            fence_after();
+            const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
+            const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));
+            float top = -INFINITY, sum = 0.0f;
+            VocabRow vr = {0.0f, 0.0f, -1, 0};
+            if (EPI == EPI_DL && row < p.m) vr = p.rows[row];
+            uint32_t held[16];
+            int64_t target = -1;
+            if (EPI == EPI_LSE && row < p.m) target = p.targets[row];
+            for (int c = 0; c < chunks; ++c) {
+                const int col0 = first + 32 * c;
+                float v[32];
+                tmem_ld32(acc + 32 * c, v);
+                ld_wait();
+                if (c == chunks - 1) {
+                    fence_before();
+                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                }
+                if (EPI == EPI_LSE) {
+                    float big = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (col0 + j >= p.n) v[j] = -INFINITY;
+                        else if (target == col0 + j) p.hit[row] = v[j];
+                        v[j] *= LOG2E;
+                        big = fmaxf(big, v[j]);
+                    }
+                    const float nt = fmaxf(top, big);
+                    sum *= ex2(top - nt);
+                    float s4[4] = {};
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) s4[j % 4] += ex2(v[j] - nt);
+                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    top = nt;
+                    continue;
+                }
+                if (EPI == EPI_STORE || EPI == EPI_DZ) {
+                    if (p.bias) {
+                        __syncwarp();
+                        bias[lane] = col0 + lane < p.n ? load(p.bias, col0 + lane, p.bias_type) : 0.0f;
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] += bias[j];
+                    }
+                    if (EPI == EPI_DZ) apply_slope(p.act, v);
+                    else apply_act(p.act, v);
+                    if (p.extra) {
+                        float e[32];
+                        if (lane == 0) bulk_wait_read();
+                        __syncwarp();
+                        load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, (float*)stage, e);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = EPI == EPI_DZ ? v[j] * e[j] : v[j] + e[j];
+                    }
+                    if (EPI == EPI_STORE && p.alpha) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= alpha;
+                    }
+                }
+                if (EPI == EPI_DL) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float pr = ex2(fmaf(v[j], LOG2E, -vr.lse2));
+                        v[j] = vr.weight == 0.0f ? 0.0f : vr.weight * (pr - (vr.target == p.col0 + col0 + j ? 1.0f : 0.0f));
+                    }
+                }
+                if (EPI == EPI_DZ && p.row_sums) {
+                    float t32[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) t32[j] = v[j];
+                    const float s = lane_sums(t32);
+                    if (col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
+                }
+                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
+                // 64 columns of 16 bits fill it (the first 32 wait in registers: the buffer also turns `extra`)
+                const bool narrow = p.y_type != PCB_F32;
+                if (narrow && c % 2 == 0) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) held[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
+                    if (c + 1 < chunks) continue;
+                }
+                if (lane == 0) bulk_wait_read();
+                __syncwarp();
+                uint4* srow = (uint4*)(stage + lane * 128);
+                if (narrow) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        srow[j ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
+                    if (c % 2) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) held[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            srow[(j + 4) ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        srow[j ^ (lane & 7)] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                          __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                }
+                const int box0 = narrow ? col0 - (c % 2) * 32 : col0;
+                if (p.y_tma) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && row0 < p.m) {
+                        if (p.accumulate) tma_add(&p.y, box0, row0, sp, stage);
+                        else tma_store(&p.y, box0, row0, sp, stage);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < p.m; ++r) {
+                        const unsigned char* srcrow = stage + r * 128;
+                        if (narrow) {
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int cc = lane + 32 * q;
+                                const uint16_t val = *(const uint16_t*)(srcrow + (((cc / 8) ^ (r & 7)) * 16 + (cc % 8) * 2));
+                                if (box0 + cc < p.n) ((uint16_t*)p.y_ptr)[((int64_t)sp * p.m + row0 + r) * p.y_pitch + box0 + cc] = val;
+                            }
+                        } else {
+                            const float val = *(const float*)(srcrow + (((lane / 4) ^ (r & 7)) * 16 + (lane % 4) * 4));
+                            float* at = (float*)p.y_ptr + ((int64_t)sp * p.m + row0 + r) * p.y_pitch + box0 + lane;
+                            if (box0 + lane < p.n) *at = p.accumulate ? *at + val : val;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (chunks == 0) {
+                fence_before();
+                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            }
+            if (EPI == EPI_LSE && row < p.m) p.parts[(int64_t)(tn * (S::EWARPS / 4) + half) * p.m + row] = make_float2(top, sum);
+        }
+        if (lane == 0) bulk_wait();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1) tmem_free(tmem, S::TMEM);
+}
+
+// y = alpha (act(sum of the splits + bias) + extra), the splits in order
+__global__ void __launch_bounds__(256) join(const float* part, int splits, const __grid_constant__ Params p) {
+    pdl_wait();
+    pdl_release();
+    const float alpha = p.alpha ? *p.alpha : 1.0f;
+    const int64_t total = (int64_t)p.m * p.n;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float v = 0.0f;
+        for (int s = 0; s < splits; ++s) v += part[s * total + i];
+        const int64_t r = i / p.n, c = i % p.n;
+        if (p.bias) v += load(p.bias, c, p.bias_type);
+        float g;
+        if (p.act.kind == PCB_ACT_GELU) v *= normal_cdf(v, &g);
+        else v = act(p.act, v);
+        if (p.extra) v += load(p.extra, r * p.extra_pitch + c, p.extra_type);
+        store(p.y_ptr, r * p.y_pitch + c, p.y_type, v * alpha);
+    }
+}
+
+__global__ void __launch_bounds__(256) copy_rows(const uint16_t* x, int64_t pitch, int64_t rows, int cols, uint16_t* y, int64_t to) {
+    pdl_wait();
+    pdl_release();
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * to; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / to, c = i % to;
+        y[i] = c < cols ? x[r * pitch + c] : (uint16_t)0;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                           const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                           CUtensorMapFloatOOBfill);
+Encode encoder() {
+    static Encode f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (Encode)p;
+    }();
+    return f;
+}
+
+}  // namespace
+
+int encode_map(CUtensorMap* map, int type, const void* p, int dims, const uint64_t* size, const uint64_t* stride_bytes,
+               const uint32_t* box) {
+    const Encode f = encoder();
+    if (!f) return report(PCB_BAD_ARGS, "the driver has no cuTensorMapEncodeTiled");
+    const CUtensorMapDataType t = type == PCB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : type == PCB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    const CUresult r = f(map, t, (cuuint32_t)dims, const_cast<void*>(p), size, stride_bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : report(PCB_BAD_ARGS, "cuTensorMapEncodeTiled failed with %d", (int)r);
+}
+
+namespace {
+
+// an operand's map: boxes of 64 adjacent values by `tile` rows (k adjacent), or by 64 k (rows adjacent)
+int operand_map(CUtensorMap* map, const Operand& o, int type, int rows, int k, int tile) {
+    const uint64_t size[2] = {(uint64_t)(o.k_adjacent ? k : rows), (uint64_t)(o.k_adjacent ? rows : k)};
+    const uint64_t stride[1] = {(uint64_t)o.pitch * 2};
+    const uint32_t box[2] = {64, (uint32_t)(o.k_adjacent ? tile : BK)};
+    return encode_map(map, type, o.p, 2, size, stride, box);
+}
+
+// Tile width and k splits, from estimated cycles: a 64-k block of a 128 x BN tile costs its products (BN / 256 of 512
+// cycles) or its bytes into shared memory, a tile about 1200 cycles of latency besides, a split its 32-bit traffic and
+// the joining launch.
+struct Plan {
+    int bn, splits, kper;
+};
+Plan plan(int m, int n, int k, bool may_split) {
+    const int kb = (k + BK - 1) / BK, tm = (m + BM - 1) / BM;
+    Plan best{256, 1, kb};
+    double least = 1e300;
+    for (int bn : {256, 128, 64}) {
+        const double block = bn == 256 ? 560 : bn == 128 ? 330 : 240;
+        for (int sp = 1; sp <= (may_split ? 16 : 1); sp *= 2) {
+            const int per = (kb + sp - 1) / sp;
+            if (sp > 1 && (per < 4 || (sp - 1) * per >= kb)) break;
+            const int64_t tiles = (int64_t)tm * ((n + bn - 1) / bn) * sp;
+            const double waves = (double)((tiles + SMS - 1) / SMS);
+            double cost = waves * (per * block + bn * 2.0) + 1200;
+            if (sp > 1) cost += 5000 + (double)m * n * 4 * sp * 2 / (SMS * 16.0);
+            if (cost < least) least = cost, best = Plan{bn, sp, per};
+        }
+    }
+    return best;
+}
+
+template <int BN, int EPI>
+int launch(const Params& p, cudaStream_t s) {
+    using S = Shape<BN>;
+    static_assert(S::SMEM <= 232448, "shared memory");
+    static const cudaError_t set = cudaFuncSetAttribute(product<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+    if (set != cudaSuccess) return (int)set;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    launch_pdl_smem(product<BN, EPI>, dim3((unsigned)(tiles < SMS ? tiles : SMS)), dim3(S::THREADS), S::SMEM, s, p);
+    return PCB_LAUNCH_RESULT();
+}
+template <int EPI>
+int launch(int bn, const Params& p, cudaStream_t s) {
+    return bn == 256 ? launch<256, EPI>(p, s) : bn == 128 ? launch<128, EPI>(p, s) : launch<64, EPI>(p, s);
+}
+
+}  // namespace
+
+size_t gemm_partial(int m, int n, int k) {
+    const Plan pl = plan(m, n, k, true);
+    return pl.splits > 1 ? (size_t)pl.splits * m * n : 0;
+}
+int vocab_parts(int m, int n) {
+    const int bn = plan(m, n, 1 << 20, false).bn;
+    return (n + bn - 1) / bn * (bn == 64 ? 1 : 2);
+}
+
+int gemm(const Gemm& g, cudaStream_t s) {
+    // the column blocks of an EPI_LSE product follow vocab_parts, which does not know k
+    const Plan pl = plan(g.m, g.n, g.epi == EPI_LSE ? 1 << 20 : g.k, g.epi == EPI_STORE && !g.accumulate && !g.whole);
+    const int kb = (g.k + BK - 1) / BK;
+    Params p;
+    memset(&p, 0, sizeof p);
+    if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, BM)) return rc;
+    if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn)) return rc;
+    p.m = g.m, p.n = g.n, p.k = g.k;
+    p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.bf16 = g.type == PCB_BF16;
+    p.tiles_m = (g.m + BM - 1) / BM, p.tiles_n = (g.n + pl.bn - 1) / pl.bn;
+    p.splits = pl.splits, p.kblocks = kb, p.kper = pl.splits > 1 ? pl.kper : kb;
+    p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;
+    p.extra = g.extra, p.extra_pitch = g.extra_pitch, p.extra_type = g.extra_type;
+    p.y_ptr = g.y, p.y_pitch = g.y_pitch, p.y_type = g.y_type, p.accumulate = g.accumulate;
+    p.alpha = g.alpha, p.row_sums = g.row_sums, p.rows = g.rows, p.col0 = g.col0, p.targets = g.targets, p.parts = g.parts, p.hit = g.hit;
+    Params fin = p;
+    if (pl.splits > 1) {  // 32-bit sums of each split, the epilogue in `join`
+        p.act = Act{}, p.bias = nullptr, p.extra = nullptr, p.alpha = nullptr;
+        p.y_ptr = g.partial, p.y_pitch = g.n, p.y_type = PCB_F32;
+    }
+    const size_t eb = type_bytes(p.y_type);
+    // 16-byte aligned rows go through the TMA engine; others by rows of the staging buffer
+    p.y_tma = g.epi != EPI_LSE && ((uintptr_t)p.y_ptr & 15) == 0 && p.y_pitch * eb % 16 == 0;
+    if (p.y_tma) {
+        const uint64_t size[3] = {(uint64_t)g.n, (uint64_t)g.m, (uint64_t)pl.splits};
+        const uint64_t stride[2] = {(uint64_t)p.y_pitch * eb, (uint64_t)p.y_pitch * eb * g.m};
+        const uint32_t box[3] = {(uint32_t)(128 / eb), 32, 1};
+        if (int rc = encode_map(&p.y, p.y_type, p.y_ptr, 3, size, stride, box)) return rc;
+    }
+    int rc;
+    if (g.epi == EPI_STORE) rc = launch<EPI_STORE>(pl.bn, p, s);
+    else if (g.epi == EPI_DZ) rc = launch<EPI_DZ>(pl.bn, p, s);
+    else if (g.epi == EPI_LSE) rc = launch<EPI_LSE>(pl.bn, p, s);
+    else rc = launch<EPI_DL>(pl.bn, p, s);
+    if (rc || pl.splits == 1) return rc;
+    const int64_t blocks = ((int64_t)g.m * g.n + 255) / 256;
+    launch_pdl(join, dim3((unsigned)(blocks < 8 * SMS ? blocks : 8 * SMS)), dim3(256), s, (const float*)g.partial, pl.splits, fin);
+    return PCB_LAUNCH_RESULT();
+}
+
+size_t aligned_bytes(const void* p, int64_t pitch, int64_t rows, int64_t cols) {
+    if (((uintptr_t)p & 15) == 0 && pitch % 8 == 0) return 0;
+    return (size_t)rows * ((cols + 7) / 8 * 8) * 2;
+}
+int align_rows(const void** p, int64_t* pitch, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
+    if (!aligned_bytes(*p, *pitch, rows, cols)) return 0;
+    const int64_t np = (cols + 7) / 8 * 8;
+    const int64_t blocks = (rows * np + 255) / 256;
+    launch_pdl(copy_rows, dim3((unsigned)(blocks < 16 * SMS ? blocks : 16 * SMS)), dim3(256), s, (const uint16_t*)*p, *pitch, rows,
+               (int)cols, (uint16_t*)to, np);
+    *p = to;
+    *pitch = np;
+    return PCB_LAUNCH_RESULT();
+}
+
+unsigned int gemm_timeouts() {
+    unsigned int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_gemm_timeouts, sizeof v) == cudaSuccess ? v : ~0u;
+}
+
+}  // namespace clear
+}  // namespace pcb

@@ -1,0 +1,70 @@
+// The product behind the clear half's operators: D[m][n] = sum_k A(m, k) B(n, k) with an epilogue (clear_gemm.cu).
+#pragma once
+#include "clear.h"
+
+namespace pcb {
+namespace clear {
+
+// A 16-bit operand: `rows` rows along m (or n) and `k` values. k_adjacent: row r's k-values are adjacent at p + r pitch;
+// otherwise the rows are, at p + k pitch.
+struct Operand {
+    const void* p;
+    int64_t pitch;
+    bool k_adjacent;
+};
+
+enum Epilogue {
+    EPI_STORE,  // y = alpha * (act(D + bias) + extra)
+    EPI_DZ,     // y = extra * act'(D + bias), and the sums of each 32 rows of its columns in 32 bits
+    EPI_LSE,    // the maximum and the sum of exponentials of each row of a column block, the target's logit
+    EPI_DL,     // y = weight (exp(D - lse) - [n = target])
+};
+
+// What EPI_DL needs of a row, in base 2: exp(l - lse) = 2^(l log2 e - lse2)
+struct VocabRow {
+    float lse2, weight;
+    int32_t target;  // -1: none
+    int32_t pad;
+};
+
+struct Gemm {
+    Operand a, b;
+    int m, n, k;
+    int type;  // of the operands
+    Epilogue epi;
+    void* y;
+    int64_t y_pitch;
+    int y_type;
+    bool accumulate;  // EPI_STORE in 32 bits: y += (one writer per element)
+    bool whole;       // EPI_STORE: k is not split (as under accumulate)
+    Act act;
+    const void* bias;
+    int bias_type;
+    const void* extra;
+    int64_t extra_pitch;
+    int extra_type;
+    const float* alpha;     // one value on the device, or null
+    float* row_sums;        // EPI_DZ: [ceil(m / 32)][n], or null
+    const VocabRow* rows;   // EPI_DL
+    int col0;               // EPI_DL: the vocabulary entry of this product's first column
+    const int64_t* targets; // EPI_LSE
+    float2* parts;          // EPI_LSE: [vocab_parts(n)][m] (maximum in base 2, sum)
+    float* hit;             // EPI_LSE: [m], written where the target lies in this product's columns
+    float* partial;         // workspace of gemm_partial() values (null when that is 0)
+};
+
+// 32-bit values of workspace that an EPI_STORE product wants (it splits a long k over the SMs when there are few tiles)
+size_t gemm_partial(int m, int n, int k);
+int gemm(const Gemm& g, cudaStream_t s);
+// column blocks of an EPI_LSE product over n columns
+int vocab_parts(int m, int n);
+
+// An operand as the TMA engine can read it: first element and pitch on 16 bytes, as it lies or copied to `to` (null when
+// only counting). aligned_bytes: the copy's size, 0 where none is needed.
+size_t aligned_bytes(const void* p, int64_t pitch, int64_t rows, int64_t cols);
+int align_rows(const void** p, int64_t* pitch, int64_t rows, int64_t cols, void* to, cudaStream_t s);
+
+unsigned int gemm_timeouts();
+
+}  // namespace clear
+}  // namespace pcb

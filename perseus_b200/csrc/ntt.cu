@@ -702,6 +702,11 @@ template int inv_run<16>(const PcbNttArgs*, bool, cudaStream_t);
 }  // namespace ntt
 }  // namespace pcb
 
-// Waits of the pipelined transforms that ran out on the current device since the library was loaded (0 in normal
-// operation; each stopped one CTA, whose rows were then left untransformed).
-extern "C" uint32_t pcb_device_timeouts(void) { return pcb::ntt::device_timeouts(); }
+// Waits of the pipelined transforms and of the clear half's products that ran out on the current device since the
+// library was loaded (0 in normal operation; each stopped one CTA, whose rows were then left undone).
+namespace pcb {
+namespace clear {
+unsigned int gemm_timeouts();
+}
+}  // namespace pcb
+extern "C" uint32_t pcb_device_timeouts(void) { return pcb::ntt::device_timeouts() + pcb::clear::gemm_timeouts(); }
