@@ -1,51 +1,104 @@
-// Attention over packed prompts (pcb_clear_attention). First form: one warp per query.
-#include "clear.h"
+// Attention over packed prompts on the fifth-generation tensor cores (pcb_clear_attention).
+//
+// A block takes 128 rows of one K/V head of one sequence: consecutive tokens x the query heads that share the K/V head
+// (a group is never split, so its keys and values are read once), and walks the keys in blocks of 128 up to the last one
+// its tokens see. Scores S = Q K^T land in TMEM (128 rows x 128 keys, 32 bits); four warps, one thread per row, turn them
+// into weights, which go back to TMEM in 16 bits as the left operand of O += P V. Softmax runs with a running maximum and
+// sum: O is rescaled only when a row's maximum grew by more than 2^8 (weights stay below 2^8, in range for f16), which
+// after the first blocks is rare. Under polynomial weights there is no maximum, no sum and no rescaling.
+// Two blocks share an SM: while one's warps compute weights, the other's products run. Heads of up to 64 keep P apart from
+// S, so that the next scores are formed while this block's O accumulates.
+//
+// Few rows against many keys (single tokens) split the keys over several blocks, joined in order by `join_splits`.
+//
+// A key block may reach into the next sequence, or hold keys that some rows do not see: their weights are zero, but zero
+// times a value that is not finite is not zero. So rows whose result is not finite are computed again, key by key over
+// the keys that they see (`attend_row`): exact semantics at no cost where all values are finite.
+#include <algorithm>
+#include <cstring>
+#include <numeric>
+#include <vector>
+
+#include "clear_gemm.h"
+#include "mma.cuh"
 
 namespace pcb {
 namespace clear {
 
-// ------------------------------------------------------------------------------------------------ attention
-// One warp per (query, head); lane l holds dims l, l + 32, ...; softmax with a running maximum and sum. starts: the
-// sequences' first rows come from walking the lengths, passed as blocks of up to SEQS sequences per launch.
-constexpr int SEQS = 256;
-struct Seqs {
+using namespace mma;
+
+int encode_map(CUtensorMap* map, int type, const void* p, int dims, const uint64_t* size, const uint64_t* stride_bytes,
+               const uint32_t* box);
+
+__device__ unsigned int g_attn_timeouts;
+
+namespace {
+
+constexpr int SMS = 148;
+constexpr int ROWS = 128, KEYS = 128;
+constexpr int SEQS = 512;  // sequences of one launch
+
+struct Work {
     int32_t n;
-    int32_t q0[SEQS + 1], k0[SEQS + 1];
+    int32_t tile0[SEQS + 1];  // first tile (times kv_heads blocks) of each sequence, the longest sequences first
+    int32_t q0[SEQS], nq[SEQS], k0[SEQS], nk[SEQS];
 };
-__global__ void __launch_bounds__(128) attend_rows(PcbClearAttention a, Seqs sq) {
-    const int64_t first = sq.q0[0];
-    const int64_t item = blockIdx.x * 4ll + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
-    const int64_t row = first + item / a.heads;
-    const int head = (int)(item % a.heads);
-    if (row >= sq.q0[sq.n]) return;
-    int b = 0;
-    while (row >= sq.q0[b + 1]) ++b;
-    const int nq = sq.q0[b + 1] - sq.q0[b], nk = sq.k0[b + 1] - sq.k0[b];
-    const int64_t i = row - sq.q0[b];
-    const int64_t seen = a.causal ? min((int64_t)nk, i + nk - nq + 1) : nk;
-    const int kh = head / (a.heads / a.kv_heads);
-    float q[4], o[4] = {}, top = -INFINITY, sum = 0.0f;
+struct alignas(64) Params {
+    CUtensorMap q, k, v;
+    PcbClearAttention a;  // the operands as they lie, for attend_row
+    int group, tokens;    // query heads of a K/V head, tokens of a 128-row tile
+    int splits;
+    float c;              // scores to base-2 exponents: |scale| log2 e
+    int negate;           // scale < 0: the products are negated
+    float coef[8];        // of the raw scores, the largest of the polynomial's own brought to 1
+    float out_scale;
+    float* part_o;        // splits > 1: [split][q row][head][dim] sums, and (maximum in base 2, sum of weights)
+    float2* part_ml;
+    int out_vec;          // out's rows take 16-byte stores
+    Work w;
+};
+
+template <int DP>
+struct Shape {
+    static constexpr int HALF = 128 * 128;               // 128 rows of 64 values
+    static constexpr int OPERAND = HALF * (DP / 64);     // 128 rows of DP
+    static constexpr int RING = DP == 64 ? 4 : 2;        // K and V blocks in flight
+    static constexpr uint32_t S = 0, P = DP == 64 ? 128 : 0, O = DP == 64 ? 192 : 128;  // TMEM columns
+    static constexpr uint32_t TMEM = 256;
+    static constexpr size_t SMEM = 1024 + OPERAND * (1 + RING) + 256;
+    static constexpr bool APART = P != S;
+};
+constexpr int THREADS = 192;
+
+// ------------------------------------------------------------------------------------------------ one row, key by key
+// A warp computes out = sum of weights x values over keys [j0, j1) of one query in 32 bits: lane l holds dims l + 32 t.
+// Returns the unnormalised sums, the maximum (base 2) and the sum of the weights.
+__device__ __noinline__ void attend_row(const PcbClearAttention& a, int64_t qrow, int head, int64_t k0, int j0, int j1, float c,
+                                        float* o, float* top_out, float* sum_out) {
+    const int lane = threadIdx.x % 32, kh = head / (a.heads / a.kv_heads);
+    float q[4], top = -INFINITY, sum = 0.0f;
     for (int t = 0; t < 4; ++t) {
         const int d = lane + 32 * t;
-        q[t] = d < a.dim ? load(a.q, row * a.q_pitch + head * a.q_head + d, a.type) : 0.0f;
+        q[t] = d < a.dim ? load(a.q, qrow * a.q_pitch + head * a.q_head + d, a.type) : 0.0f;
+        o[t] = 0.0f;
     }
-    for (int64_t j = 0; j < seen; ++j) {
-        const int64_t kr = sq.k0[b] + j;
+    for (int j = j0; j < j1; ++j) {
+        const int64_t kr = k0 + j;
         float s = 0.0f;
         for (int t = 0; t < 4; ++t) {
             const int d = lane + 32 * t;
             if (d < a.dim) s = fmaf(q[t], load(a.k, kr * a.k_pitch + kh * a.k_head + d, a.type), s);
         }
         for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(~0u, s, m);
-        s *= a.scale;
         float p;
         if (a.ncoef) {
+            s *= a.scale;
             p = a.coef[a.ncoef - 1];
-            for (int c = a.ncoef - 2; c >= 0; --c) p = fmaf(p, s, a.coef[c]);
+            for (int i = a.ncoef - 2; i >= 0; --i) p = fmaf(p, s, a.coef[i]);
         } else {
-            const float nt = fmaxf(top, s), f = top == -INFINITY ? 0.0f : expf(top - nt);
-            p = nt == -INFINITY ? 0.0f : expf(s - nt);
+            s = (a.scale < 0.0f ? -s : s) * c;
+            const float nt = fmaxf(top, s), f = top == -INFINITY ? 0.0f : exp2f(top - nt);
+            p = nt == -INFINITY ? (s == s ? 0.0f : s) : exp2f(s - nt);
             sum = sum * f + p;
             for (int t = 0; t < 4; ++t) o[t] *= f;
             top = nt;
@@ -55,11 +108,410 @@ __global__ void __launch_bounds__(128) attend_rows(PcbClearAttention a, Seqs sq)
             if (d < a.dim) o[t] = fmaf(p, load(a.v, kr * a.v_pitch + kh * a.v_head + d, a.type), o[t]);
         }
     }
-    const float f = a.ncoef ? 1.0f : seen > 0 ? 1.0f / sum : 0.0f;
-    for (int t = 0; t < 4; ++t) {
-        const int d = lane + 32 * t;
-        if (d < a.dim) store(a.out, row * a.out_pitch + head * a.out_head + d, a.type, o[t] * f);
+    *top_out = top;
+    *sum_out = sum;
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel
+template <int DP, bool POLY>
+__global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Params p) {
+    using S = Shape<DP>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* base = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* ring = base + S::OPERAND;
+    uint64_t* q_full = (uint64_t*)(ring + S::RING * S::OPERAND);
+    uint64_t* full = q_full + 1;
+    uint64_t* empty = full + S::RING;
+    uint64_t* s_full = empty + S::RING;
+    uint64_t* p_ready = s_full + 1;
+    uint64_t* pv_done = p_ready + 1;
+    uint64_t* drain = pv_done + 1;
+    uint32_t* tmem_at = (uint32_t*)(drain + 1);
+    volatile int* dead = (volatile int*)(tmem_at + 1);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < S::RING; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(p_ready, 4);
+        mbar_init(pv_done, 1);
+        mbar_init(drain, 1);
+        mbar_init_fence();
+        *dead = 0;
+        prefetch_map(&p.q);
+        prefetch_map(&p.k);
+        prefetch_map(&p.v);
     }
+    if (warp == 1) tmem_alloc(tmem_at, S::TMEM);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_at;
+    pdl_wait();
+    pdl_release();
+
+    // ---- this block's tile: the sequence, the K/V head, the tokens from t0 (the last ones first), the key blocks
+    const int split = blockIdx.x % p.splits, item = blockIdx.x / p.splits;
+    const int tile = item / p.a.kv_heads, kh = item % p.a.kv_heads;
+    int lo = 0, hi = p.w.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.w.tile0[mid] <= tile) lo = mid;
+        else hi = mid;
+    }
+    const int nq = p.w.nq[lo], nk = p.w.nk[lo], q0 = p.w.q0[lo], k0 = p.w.k0[lo];
+    const int t0 = (p.w.tile0[lo + 1] - 1 - tile) * p.tokens, past = nk - nq;
+    const int t1 = min(nq, t0 + p.tokens);                                           // tokens [t0, t1)
+    const int seen = p.a.causal ? min(nk, max(0, t1 + past)) : nk;                    // keys of the last token
+    const int least = p.a.causal ? min(nk, max(0, t0 + past + 1)) : nk;               // and of the first
+    const int blocks = (seen + KEYS - 1) / KEYS, per = (blocks + p.splits - 1) / p.splits;
+    const int b0 = min(blocks, split * per), n = min(blocks, b0 + per) - b0;
+
+    if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            mbar_expect(q_full, (DP / 64) * 128 * p.group * p.tokens);
+            for (int h = 0; h < DP / 64; ++h) tma_load(base + h * S::HALF, &p.q, 64 * h, kh * p.group, q0 + t0, q_full);
+            int i = 0;
+            for (; i < 2 * n; ++i) {  // K and V in turn
+                const int st = i % S::RING;
+                if (i >= S::RING && !wait(&empty[st], (i / S::RING - 1) & 1, dead, &g_attn_timeouts)) break;
+                mbar_expect(&full[st], S::OPERAND);
+                for (int h = 0; h < DP / 64; ++h)
+                    tma_load(ring + st * S::OPERAND + h * S::HALF, i % 2 ? &p.v : &p.k, 64 * h, kh, k0 + (b0 + i / 2) * KEYS, &full[st]);
+            }
+            if (*dead) {  // the loads in flight
+                mbar_wait(q_full, 0);
+                for (int f = max(0, i - S::RING); f < i; ++f) mbar_wait(&full[f % S::RING], (f / S::RING) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && n > 0) {
+            const bool bf16 = p.a.type == PCB_BF16;
+            const int ksteps = (p.a.dim + 15) / 16, nd = (p.a.dim + 15) / 16 * 16;
+            const uint32_t is = instr_desc(bf16, false, false, ROWS, KEYS) | (p.negate ? 1u << 13 : 0u);
+            const uint32_t ipv = instr_desc(bf16, false, true, ROWS, nd);
+            const uint64_t dq = smem_desc(smem_addr(base), 16, 1024);
+            bool ok = wait(q_full, 0, dead, &g_attn_timeouts);
+            auto scores = [&](int j) {  // S = Q K_j^T
+                const int i = 2 * j, st = i % S::RING;
+                if (!wait(&full[st], (i / S::RING) & 1, dead, &g_attn_timeouts)) return false;
+                fence_after();
+                const uint64_t dk = smem_desc(smem_addr(ring + st * S::OPERAND), 16, 1024);
+                for (int s = 0; s < ksteps; ++s) {
+                    const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
+                    mma_ss(tmem + S::S, dq + off, dk + off, is, s > 0);
+                }
+                mma_commit(s_full);
+                mma_commit(&empty[st]);
+                return true;
+            };
+            ok = ok && scores(0);
+            for (int j = 0; j < n && ok; ++j) {
+                ok = wait(p_ready, j & 1, dead, &g_attn_timeouts);
+                if (!ok) break;
+                fence_after();
+                if (S::APART && j + 1 < n) ok = scores(j + 1);
+                const int i = 2 * j + 1, st = i % S::RING;
+                ok = ok && wait(&full[st], (i / S::RING) & 1, dead, &g_attn_timeouts);
+                if (!ok) break;
+                fence_after();
+                const uint64_t dv = smem_desc(smem_addr(ring + st * S::OPERAND), S::HALF, 1024);
+                for (int s = 0; s < KEYS / 16; ++s)
+                    mma_ts(tmem + S::O, tmem + S::P + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, j > 0 || s > 0);
+                mma_commit(pv_done);
+                mma_commit(&empty[st]);
+                if (!S::APART && j + 1 < n) {  // the next scores take P's place
+                    ok = wait(pv_done, j & 1, dead, &g_attn_timeouts);
+                    ok = ok && scores(j + 1);
+                }
+            }
+            if (*dead) {  // the products in flight
+                mma_commit(drain);
+                mbar_wait(drain, 0);
+            }
+        }
+    } else {
+        const int quad = warp % 4, r = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const int tok = t0 + r / p.group, head = kh * p.group + r % p.group;
+        const bool mine = r < p.group * p.tokens && tok < nq;
+        const int limit = !mine ? 0 : p.a.causal ? min(nk, max(0, tok + past + 1)) : nk;  // keys that this row sees
+        const bool bf16 = p.a.type == PCB_BF16;
+        float top = -INFINITY, sum = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            ok = wait_warp(s_full, j & 1, dead, &g_attn_timeouts);
+            if (!ok) break;
+            fence_after();
+            float s[KEYS];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) tmem_ld32(tmem + S::S + lanes + 32 * h, s + 32 * h);
+            ld_wait();
+            const int at = (b0 + j) * KEYS, left = limit - at;
+            const bool masked = at + KEYS > least;
+            if (POLY) {
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    float v = p.coef[7];
+#pragma unroll
+                    for (int e = 6; e >= 0; --e) v = fmaf(v, s[i], p.coef[e]);
+                    s[i] = v;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) s[i] = i < left ? s[i] : 0.0f;
+                }
+                if (j > 0) ok = wait_warp(pv_done, (j - 1) & 1, dead, &g_attn_timeouts);
+                if (!ok) break;
+            } else {
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                }
+                float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < KEYS; ++i) m4[i % 4] = fmaxf(m4[i % 4], s[i]);
+                const float big = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.c);
+                const bool grew = big > top + 8.0f;
+                if (j > 0) ok = wait_warp(pv_done, (j - 1) & 1, dead, &g_attn_timeouts);
+                if (!ok) break;
+                if (__any_sync(~0u, grew)) {
+                    const float f = grew ? ex2(top - big) : 1.0f;
+                    if (j > 0) {
+                        fence_after();
+#pragma unroll
+                        for (int h = 0; h < DP / 32; ++h) {
+                            float o[32];
+                            tmem_ld32(tmem + S::O + lanes + 32 * h, o);
+                            ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= f;
+                            tmem_st32(tmem + S::O + lanes + 32 * h, (uint32_t*)o);
+                        }
+                    }
+                    sum *= f;
+                    if (grew) top = big;
+                }
+                const float sub = top == -INFINITY ? 0.0f : -top;
+                float s4[4] = {};
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    s[i] = ex2(fmaf(s[i], p.c, sub));
+                    s4[i % 4] += s[i];
+                }
+                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            }
+            // the weights in 16 bits (their one rounding: the products with V take 16-bit operands), two per column
+            uint32_t* w = (uint32_t*)s;
+#pragma unroll
+            for (int i = 0; i < KEYS / 2; ++i) w[i] = pack2(s[2 * i], s[2 * i + 1], bf16);
+            tmem_st32(tmem + S::P + lanes, w);
+            tmem_st32(tmem + S::P + lanes + 32, w + 32);
+            st_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
+        }
+        if (ok && n > 0) ok = wait_warp(pv_done, (n - 1) & 1, dead, &g_attn_timeouts);
+        fence_after();
+        if (ok) {
+            const int64_t qrow = q0 + tok;
+            const float scale = POLY ? p.out_scale : p.splits > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
+            const int64_t prow = ((int64_t)split * p.a.q_rows + qrow) * p.a.heads + head;
+            const int64_t orow = qrow * p.a.out_pitch + head * p.a.out_head;
+            bool odd = !(fabsf(sum) <= 3.4e38f);
+#pragma unroll 1
+            for (int h = 0; h < DP / 32; ++h) {
+                float o[32];
+                if (n > 0) {
+                    tmem_ld32(tmem + S::O + lanes + 32 * h, o);
+                    ld_wait();
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    o[i] = n > 0 ? o[i] * scale : 0.0f;
+                    odd |= !(fabsf(o[i]) <= 3.4e38f) && 32 * h + i < p.a.dim;
+                }
+                if (!mine) continue;
+                if (p.splits > 1) {
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * h + i < p.a.dim) p.part_o[prow * p.a.dim + 32 * h + i] = o[i];
+                } else if (p.out_vec) {
+                    uint4* to = (uint4*)((uint16_t*)p.a.out + orow + 32 * h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (32 * h + 8 * i < p.a.dim)
+                            to[i] = make_uint4(pack2(o[8 * i], o[8 * i + 1], bf16), pack2(o[8 * i + 2], o[8 * i + 3], bf16),
+                                               pack2(o[8 * i + 4], o[8 * i + 5], bf16), pack2(o[8 * i + 6], o[8 * i + 7], bf16));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * h + i < p.a.dim) store(p.a.out, orow + 32 * h + i, p.a.type, o[i]);
+                }
+            }
+            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(top, sum);
+            for (uint32_t again = __ballot_sync(~0u, mine && odd); again; again &= again - 1) {
+                const int src = __ffs(again) - 1;
+                const int tk = __shfl_sync(~0u, tok, src), hd = __shfl_sync(~0u, head, src), lim = __shfl_sync(~0u, limit, src);
+                const int64_t qr = q0 + tk;
+                float o[4], tp, sm;
+                attend_row(p.a, qr, hd, k0, min(lim, b0 * KEYS), min(lim, (b0 + n) * KEYS), p.c, o, &tp, &sm);
+                const int64_t pr = ((int64_t)split * p.a.q_rows + qr) * p.a.heads + hd;
+                for (int t = 0; t < 4; ++t) {
+                    const int d = lane + 32 * t;
+                    if (d >= p.a.dim) continue;
+                    if (p.splits > 1) p.part_o[pr * p.a.dim + d] = o[t];
+                    else store(p.a.out, qr * p.a.out_pitch + hd * p.a.out_head + d, p.a.type, POLY ? o[t] : o[t] / sm);
+                }
+                if (p.splits > 1 && lane == 0) p.part_ml[pr] = make_float2(tp, sm);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1) tmem_free(tmem, S::TMEM);
+}
+
+// The splits of a row joined in order: a warp per (query, head)
+__global__ void __launch_bounds__(256) join_splits(PcbClearAttention a, int splits, const float* part_o, const float2* part_ml) {
+    pdl_wait();
+    pdl_release();
+    const int64_t rows = a.q_rows * a.heads, row = blockIdx.x * 8ll + threadIdx.x / 32;
+    if (row >= rows) return;
+    const int lane = threadIdx.x % 32;
+    float top = -INFINITY, sum = 0.0f, o[4] = {};
+    if (!a.ncoef)
+        for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[s * rows + row].x);
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = part_ml[s * rows + row];
+        const float f = a.ncoef ? 1.0f : ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : exp2f(ml.x - top);
+        if (f == 0.0f) continue;
+        sum += ml.y * f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (lane + 32 * t < a.dim) o[t] = fmaf(f, part_o[(s * rows + row) * a.dim + lane + 32 * t], o[t]);
+    }
+    const float f = a.ncoef ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t at = row / a.heads * a.out_pitch + row % a.heads * a.out_head;
+    for (int t = 0; t < 4; ++t)
+        if (lane + 32 * t < a.dim) store(a.out, at + lane + 32 * t, a.type, o[t] * f);
+}
+
+// [row][head][dim] at any strides to rows of `heads` x `to` adjacent values, zeros past dim
+__global__ void __launch_bounds__(256) copy_heads(const uint16_t* x, int64_t pitch, int64_t head, int64_t rows, int heads, int dim,
+                                                  uint16_t* y, int to) {
+    pdl_wait();
+    pdl_release();
+    const int64_t total = rows * heads * to;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int d = (int)(i % to), h = (int)(i / to % heads);
+        y[i] = d < dim ? x[i / to / heads * pitch + h * head + d] : (uint16_t)0;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+// One of q, k, v as the TMA engine can read it (16-byte aligned first element and strides, none of zero between several),
+// or a copy
+struct Heads {
+    const void* p;
+    int64_t pitch, head, rows;
+    int heads;
+    bool copy;
+};
+Heads heads_of(const void* p, int64_t pitch, int64_t head, int64_t rows, int heads, int dim) {
+    Heads h{p, pitch, head, rows, heads, false};
+    if (heads == 1) h.head = (dim + 7) / 8 * 8;
+    if (rows == 1) h.pitch = heads * ((dim + 7) / 8 * 8);
+    h.copy = ((uintptr_t)p & 15) || h.pitch % 8 || h.head % 8 || h.pitch == 0 || h.head == 0 || h.pitch >= (1ll << 38) ||
+             h.head >= (1ll << 38);
+    return h;
+}
+size_t copy_bytes(const Heads& h, int dim) { return h.copy ? (size_t)h.rows * h.heads * ((dim + 7) / 8 * 8) * 2 : 0; }
+int make_copy(Heads& h, int dim, void* to, cudaStream_t s) {
+    if (!h.copy) return 0;
+    const int dp = (dim + 7) / 8 * 8;
+    const int64_t blocks = (h.rows * h.heads * dp + 255) / 256;
+    launch_pdl(copy_heads, dim3((unsigned)std::min<int64_t>(blocks, 16 * SMS)), dim3(256), s, (const uint16_t*)h.p, h.pitch, h.head,
+               h.rows, h.heads, dim, (uint16_t*)to, dp);
+    h.p = to, h.pitch = (int64_t)h.heads * dp, h.head = dp;
+    return PCB_LAUNCH_RESULT();
+}
+int heads_map(CUtensorMap* map, const Heads& h, int type, int dim, int box_heads, int box_rows) {
+    const uint64_t size[3] = {(uint64_t)dim, (uint64_t)h.heads, (uint64_t)h.rows};
+    const uint64_t stride[2] = {(uint64_t)h.head * 2, (uint64_t)h.pitch * 2};
+    const uint32_t box[3] = {64, (uint32_t)box_heads, (uint32_t)box_rows};
+    return encode_map(map, type, h.p, 3, size, stride, box);
+}
+
+// Splits of the keys: as many as fill two blocks per SM, each with at least two key blocks, when the tiles alone do not
+// (one launch's worth of sequences; more sequences have tiles enough)
+int splits_of(const PcbClearAttention* a) {
+    const int tokens = ROWS / (a->heads / a->kv_heads);
+    int64_t tiles = 0;
+    int longest = 0;
+    for (int b = 0; b < a->nseq; ++b) {
+        tiles += ((int64_t)a->q_lens[b] + tokens - 1) / tokens;
+        if (a->q_lens[b]) longest = std::max(longest, a->k_lens[b]);
+    }
+    tiles *= a->kv_heads;
+    const int blocks = (longest + KEYS - 1) / KEYS;
+    if (tiles == 0 || tiles >= 2 * SMS || a->nseq > SEQS) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * SMS + tiles - 1) / tiles, blocks / 2, 64}));
+}
+
+struct Ws {
+    size_t bytes;
+    Heads q, k, v;
+    void *qc, *kc, *vc;
+    int splits;
+    float* part_o;
+    float2* part_ml;
+};
+Ws attn_ws(const PcbClearAttention* a, void* ws) {
+    Carve c(ws);
+    Ws r;
+    r.q = heads_of(a->q, a->q_pitch, a->q_head, a->q_rows, a->heads, a->dim);
+    r.k = heads_of(a->k, a->k_pitch, a->k_head, a->k_rows, a->kv_heads, a->dim);
+    r.v = heads_of(a->v, a->v_pitch, a->v_head, a->k_rows, a->kv_heads, a->dim);
+    r.qc = c.take<char>(copy_bytes(r.q, a->dim));
+    r.kc = c.take<char>(copy_bytes(r.k, a->dim));
+    r.vc = c.take<char>(copy_bytes(r.v, a->dim));
+    r.splits = splits_of(a);
+    const size_t rows = r.splits > 1 ? (size_t)r.splits * a->q_rows * a->heads : 0;
+    r.part_o = c.take<float>(rows * a->dim);
+    r.part_ml = c.take<float2>(rows);
+    r.bytes = c.used;
+    return r;
+}
+
+template <int DP, bool POLY>
+int launch(const Params& p, int64_t blocks, cudaStream_t s) {
+    using S = Shape<DP>;
+    static_assert(2 * (S::SMEM + 1024) <= 233472, "two blocks per SM");
+    static const cudaError_t set = cudaFuncSetAttribute(attend<DP, POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+    if (set != cudaSuccess) return (int)set;
+    launch_pdl_smem(attend<DP, POLY>, dim3((unsigned)blocks), dim3(THREADS), S::SMEM, s, p);
+    return PCB_LAUNCH_RESULT();
+}
+
+__global__ void __launch_bounds__(256) zero_out(PcbClearAttention a) {
+    pdl_wait();
+    pdl_release();
+    const int64_t total = a.q_rows * a.heads * a.dim;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
+        store(a.out, i / a.dim / a.heads * a.out_pitch + i / a.dim % a.heads * a.out_head + i % a.dim, a.type, 0.0f);
+}
+
+}  // namespace
+
+unsigned int attn_timeouts() {
+    unsigned int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_attn_timeouts, sizeof v) == cudaSuccess ? v : ~0u;
 }
 
 }  // namespace clear
@@ -70,24 +522,73 @@ using namespace pcb::clear;
 
 extern "C" {
 
-int64_t pcb_clear_attention_ws(const PcbClearAttention* a) { return bad_attention(a); }
-int pcb_clear_attention(const PcbClearAttention* a, void*, size_t, cudaStream_t s) {
+int64_t pcb_clear_attention_ws(const PcbClearAttention* a) {
     if (int rc = bad_attention(a)) return rc;
-    int32_t q0 = 0, k0 = 0;
-    for (int b0 = 0; b0 < a->nseq; b0 += SEQS) {
-        Seqs sq;
-        sq.n = a->nseq - b0 < SEQS ? a->nseq - b0 : SEQS;
-        for (int i = 0; i < sq.n; ++i) {
-            sq.q0[i] = q0, sq.k0[i] = k0;
-            q0 += a->q_lens[b0 + i], k0 += a->k_lens[b0 + i];
-        }
-        sq.q0[sq.n] = q0, sq.k0[sq.n] = k0;
-        const int64_t items = (int64_t)(q0 - sq.q0[0]) * a->heads;
-        if (!items) continue;
-        attend_rows<<<(unsigned)((items + 3) / 4), 128, 0, s>>>(*a, sq);
-        if (int rc = PCB_LAUNCH_RESULT()) return rc;
+    return a->q_rows && a->k_rows ? (int64_t)attn_ws(a, nullptr).bytes : 0;
+}
+int pcb_clear_attention(const PcbClearAttention* a, void* ws, size_t ws_bytes, cudaStream_t s) {
+    if (int rc = bad_attention(a)) return rc;
+    if (!a->q_rows) return 0;
+    if (!a->k_rows) {
+        launch_pdl(zero_out, dim3(4 * SMS), dim3(256), s, *a);
+        return PCB_LAUNCH_RESULT();
     }
-    return 0;
+    Ws w = attn_ws(a, ws);
+    if (int rc = bad_ws("clear_attention", ws, ws_bytes, w.bytes)) return rc;
+    if (int rc = make_copy(w.q, a->dim, w.qc, s)) return rc;
+    if (int rc = make_copy(w.k, a->dim, w.kc, s)) return rc;
+    if (int rc = make_copy(w.v, a->dim, w.vc, s)) return rc;
+    Params p;
+    memset(&p, 0, offsetof(Params, w));
+    p.a = *a;
+    p.group = a->heads / a->kv_heads;
+    p.tokens = ROWS / p.group;
+    p.splits = w.splits;
+    // a scale of zero keeps masked scores at -inf in the exponent
+    p.c = std::max(std::fabs(a->scale) * 1.4426950408889634f, 1e-37f);
+    p.negate = a->ncoef == 0 && a->scale < 0.0f;
+    double big = 0.0, pw = 1.0;
+    for (int i = 0; i < a->ncoef; ++i) big = std::max(big, (double)std::fabs(a->coef[i]));
+    if (big == 0.0) big = 1.0;
+    for (int i = 0; i < a->ncoef; ++i, pw *= a->scale) p.coef[i] = (float)(a->coef[i] * pw / big);
+    p.out_scale = (float)big;
+    p.part_o = w.part_o, p.part_ml = w.part_ml;
+    p.out_vec = ((uintptr_t)a->out & 15) == 0 && a->out_pitch % 8 == 0 && a->out_head % 8 == 0 && a->dim % 8 == 0;
+    if (int rc = heads_map(&p.q, w.q, a->type, a->dim, p.group, p.tokens)) return rc;
+    if (int rc = heads_map(&p.k, w.k, a->type, a->dim, 1, KEYS)) return rc;
+    if (int rc = heads_map(&p.v, w.v, a->type, a->dim, 1, KEYS)) return rc;
+    int32_t q0 = 0, k0 = 0;
+    for (int first = 0; first < a->nseq; first += SEQS) {
+        const int n = std::min(a->nseq - first, SEQS);
+        int32_t order[SEQS], q[SEQS], k[SEQS];
+        for (int i = 0; i < n; ++i) {
+            order[i] = i, q[i] = q0, k[i] = k0;
+            q0 += a->q_lens[first + i], k0 += a->k_lens[first + i];
+        }
+        std::stable_sort(order, order + n, [&](int x, int y) { return a->k_lens[first + x] > a->k_lens[first + y]; });
+        Work& wk = p.w;
+        wk.n = 0;
+        int64_t tiles = 0;
+        for (int i = 0; i < n; ++i) {
+            const int b = order[i], nq = a->q_lens[first + b];
+            if (!nq) continue;
+            wk.tile0[wk.n] = (int32_t)tiles;
+            wk.q0[wk.n] = q[b], wk.nq[wk.n] = nq, wk.k0[wk.n] = k[b], wk.nk[wk.n] = a->k_lens[first + b];
+            tiles += (nq + p.tokens - 1) / p.tokens;
+            ++wk.n;
+        }
+        wk.tile0[wk.n] = (int32_t)tiles;
+        const int64_t blocks = tiles * a->kv_heads * p.splits;
+        if (!blocks) continue;
+        if (blocks > INT32_MAX) return report(PCB_BAD_ARGS, "clear_attention: %lld blocks in one launch", (long long)blocks);
+        const int rc = a->dim <= 64 ? (a->ncoef ? launch<64, true>(p, blocks, s) : launch<64, false>(p, blocks, s))
+                                    : (a->ncoef ? launch<128, true>(p, blocks, s) : launch<128, false>(p, blocks, s));
+        if (rc) return rc;
+    }
+    if (p.splits == 1) return 0;
+    const int64_t rows = a->q_rows * a->heads;
+    launch_pdl(join_splits, dim3((unsigned)((rows + 7) / 8)), dim3(256), s, *a, p.splits, (const float*)p.part_o, (const float2*)p.part_ml);
+    return PCB_LAUNCH_RESULT();
 }
 
 }  // extern "C"

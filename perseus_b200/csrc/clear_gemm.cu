@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
             const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
             const int m0 = mn % p.tiles_m * BM, tn = mn / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
-            if (!wait(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
+            if (!wait_warp(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
             const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));

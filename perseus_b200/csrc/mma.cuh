@@ -59,6 +59,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return false;
 }
 
+// the same for a whole warp: every lane takes the same way
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned int* timeouts) {
+    return __all_sync(~0u, wait(bar, parity, dead, timeouts));
+}
+
 // ------------------------------------------------------------------------------------------------ TMEM
 // One warp allocates `cols` (a power of two from 32 to 512) columns of 128 lanes x 32 bits, and frees them
 __device__ __forceinline__ void tmem_alloc(uint32_t* at, uint32_t cols) {

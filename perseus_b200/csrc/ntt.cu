@@ -702,11 +702,14 @@ template int inv_run<16>(const PcbNttArgs*, bool, cudaStream_t);
 }  // namespace ntt
 }  // namespace pcb
 
-// Waits of the pipelined transforms and of the clear half's products that ran out on the current device since the
+// Waits of the pipelined transforms and of the clear half's kernels that ran out on the current device since the
 // library was loaded (0 in normal operation; each stopped one CTA, whose rows were then left undone).
 namespace pcb {
 namespace clear {
 unsigned int gemm_timeouts();
+unsigned int attn_timeouts();
 }
 }  // namespace pcb
-extern "C" uint32_t pcb_device_timeouts(void) { return pcb::ntt::device_timeouts() + pcb::clear::gemm_timeouts(); }
+extern "C" uint32_t pcb_device_timeouts(void) { 
+    return pcb::ntt::device_timeouts() + pcb::clear::gemm_timeouts() + pcb::clear::attn_timeouts();
+}
