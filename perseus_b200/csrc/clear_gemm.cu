@@ -27,20 +27,23 @@ constexpr int SMS = 148;
 constexpr int BM = 128, BK = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <int BN>
+// A tile is 128 x BN by one block, or 256 x BN by a pair (128 rows of A and half of B's rows in each block's shared memory:
+// per product each SM reads a third less of it than alone, and half of B crosses from L2 once instead of twice)
+template <int BN, int CTAS>
 struct Shape {
-    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int B_ROWS = BN / CTAS;
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int EWARPS = BN == 64 ? 4 : 8;         // epilogue warps: 4 cover the 128 lanes, 8 halve the columns
+    static constexpr int STAGES = BN == 64 ? 8 : STAGE == 32768 ? 5 : 6;
     static constexpr int COLS = BN / (EWARPS / 4);          // columns of one epilogue warp
     static constexpr int THREADS = 64 + 32 * EWARPS;
     static constexpr int TMEM = 2 * BN;
-    static constexpr int STAGING = 4096;                    // per epilogue warp: 32 rows x 128 bytes
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EWARPS * (STAGING + 128) + 256;
+    static constexpr int STAGING = 4096;                    // per epilogue warp: 32 rows x 128 bytes, out and in
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EWARPS * (2 * STAGING + 128) + 512;
 };
 
 struct alignas(64) Params {
-    CUtensorMap a, b, y;
+    CUtensorMap a, b, y, extra_map;
     int m, n, k;
     int a_mn, b_mn, bf16;
     int tiles_m, tiles_n, splits, kblocks, kper;  // k blocks in all and of one split
@@ -49,7 +52,7 @@ struct alignas(64) Params {
     const void* extra;
     void* y_ptr;
     int64_t extra_pitch, y_pitch;
-    int bias_type, extra_type, y_type, y_tma, accumulate;
+    int bias_type, extra_type, y_type, y_tma, extra_tma, accumulate;
     const float* alpha;
     float* row_sums;
     const VocabRow* rows;
@@ -139,21 +142,23 @@ __device__ __forceinline__ void load_block(const void* p, int64_t pitch, int typ
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
-template <int BN, int EPI>
-__global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_constant__ Params p) {
-    using S = Shape<BN>;
+template <int BN, int CTAS, int EPI>
+__global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __grid_constant__ Params p) {
+    using S = Shape<BN, CTAS>;
     extern __shared__ unsigned char raw[];
     unsigned char* base = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     unsigned char* staging = base + S::STAGES * S::STAGE;
-    float* bias_s = (float*)(staging + S::EWARPS * S::STAGING);
+    float* bias_s = (float*)(staging + S::EWARPS * 2 * S::STAGING);
     uint64_t* full = (uint64_t*)(bias_s + S::EWARPS * 32);
     uint64_t* empty = full + S::STAGES;
     uint64_t* acc_full = empty + S::STAGES;
     uint64_t* acc_empty = acc_full + 2;
-    uint64_t* drain = acc_empty + 2;
+    uint64_t* extra_full = acc_empty + 2;
+    uint64_t* drain = extra_full + S::EWARPS;
     uint32_t* tmem_at = (uint32_t*)(drain + 1);
     volatile int* dead = (volatile int*)(tmem_at + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
@@ -162,58 +167,67 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], S::EWARPS);
+            mbar_init(&acc_empty[i], S::EWARPS * CTAS);
         }
+        for (int i = 0; i < S::EWARPS; ++i) mbar_init(&extra_full[i], 1);
         mbar_init(drain, 1);
         mbar_init_fence();
         *dead = 0;
         prefetch_map(&p.a);
         prefetch_map(&p.b);
     }
-    if (warp == 1) tmem_alloc(tmem_at, S::TMEM);
+    if (warp == 1) tmem_alloc<CTAS>(tmem_at, S::TMEM);
     fence_before();
     __syncthreads();
+    if (CTAS == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = *tmem_at;
     pdl_wait();
     pdl_release();
 
     const int tiles = p.tiles_m * p.tiles_n * p.splits;
+    const int first_tile = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
     if (warp == 0) {
         if (lane == 0) {
             int it = 0;
-            for (int tile = blockIdx.x; tile < tiles && !*dead; tile += gridDim.x) {
+            for (int tile = first_tile; tile < tiles && !*dead; tile += stride) {
                 const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
-                const int m0 = mn % p.tiles_m * BM, n0 = mn / p.tiles_m * BN;
+                const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, n0 = mn / p.tiles_m * BN + rank * S::B_ROWS;
                 const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int st = it % S::STAGES;
                     if (it >= S::STAGES && !wait(&empty[st], (it / S::STAGES - 1) & 1, dead, &g_gemm_timeouts)) break;
                     unsigned char* sa = base + st * S::STAGE;
                     unsigned char* sb = sa + S::A_BYTES;
-                    mbar_expect(&full[st], S::STAGE);
+                    // a pair's loads all complete on the first block's barrier, whose thread issues the products
+                    if (rank == 0) mbar_expect(&full[st], CTAS * S::STAGE);
+                    const uint32_t bar = CTAS == 2 ? cluster_addr(&full[st], 0) : 0;
+                    auto box = [&](void* dst, const CUtensorMap* map, int x, int y) {
+                        if (CTAS == 2) tma_load_pair(dst, map, x, y, bar);
+                        else tma_load(dst, map, x, y, &full[st]);
+                    };
                     if (p.a_mn) {
-                        for (int j = 0; j < BM / 64; ++j) tma_load(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK, &full[st]);
+                        for (int j = 0; j < BM / 64; ++j) box(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK);
                     } else {
-                        tma_load(sa, &p.a, kb * BK, m0, &full[st]);
+                        box(sa, &p.a, kb * BK, m0);
                     }
                     if (p.b_mn) {
-                        for (int j = 0; j < BN / 64; ++j) tma_load(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK, &full[st]);
+                        for (int j = 0; j < S::B_ROWS / 64; ++j) box(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK);
                     } else {
-                        tma_load(sb, &p.b, kb * BK, n0, &full[st]);
+                        box(sb, &p.b, kb * BK, n0);
                     }
                 }
             }
-            if (*dead)  // the loads in flight
-                for (int i = max(0, it - S::STAGES); i < it; ++i) mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+            if (*dead)  // the loads in flight: into the first block's, their barrier's; the second's are behind the cluster's end
+                for (int i = max(0, it - S::STAGES); i < it && rank == 0; ++i) mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = instr_desc(p.bf16, p.a_mn, p.b_mn, BM, BN);
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = instr_desc(p.bf16, p.a_mn, p.b_mn, BM * CTAS, BN);
             const uint32_t a_lbo = p.a_mn ? 8192 : 16, a_step = (p.a_mn ? 2048 : 32) >> 4;
             const uint32_t b_lbo = p.b_mn ? 8192 : 16, b_step = (p.b_mn ? 2048 : 32) >> 4;
             int it = 0, t = 0;
-            for (int tile = blockIdx.x; tile < tiles && !*dead; tile += gridDim.x, ++t) {
+            for (int tile = first_tile; tile < tiles && !*dead; tile += stride, ++t) {
                 const int sp = tile / (p.tiles_m * p.tiles_n);
                 const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
                 const int buf = t & 1;
@@ -227,25 +241,56 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
                     const uint32_t sa = smem_addr(base + st * S::STAGE);
                     const uint64_t da = smem_desc(sa, a_lbo, 1024), db = smem_desc(sa + S::A_BYTES, b_lbo, 1024);
 #pragma unroll
-                    for (int q = 0; q < BK / 16; ++q) mma_ss(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
-                    mma_commit(&empty[st]);
+                    for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
+                    mma_commit<CTAS>(&empty[st]);
                 }
-                mma_commit(&acc_full[buf]);
+                mma_commit<CTAS>(&acc_full[buf]);
             }
             if (*dead) {  // the products in flight
-                mma_commit(drain);
+                mma_commit<CTAS>(drain);
                 mbar_wait(drain, 0);
             }
         }
     } else {
         const int ew = warp - 2, quad = warp % 4, half = ew / 4;
-        unsigned char* stage = staging + ew * S::STAGING;
+        unsigned char* stage = staging + ew * 2 * S::STAGING;
+        unsigned char* in = stage + S::STAGING;  // `extra`'s boxes: 32 rows x 128 bytes, the next one on its way
         float* bias = bias_s + ew * 32;
         const float alpha = p.alpha ? *p.alpha : 1.0f;
+        const uint32_t leader_empty[2] = {CTAS == 2 ? cluster_addr(&acc_empty[0], 0) : 0, CTAS == 2 ? cluster_addr(&acc_empty[1], 0) : 0};
+        auto release = [&](int buf) {  // this warp has the accumulator's values
+            fence_before();
+            if (lane) return;
+            if (CTAS == 2) mbar_arrive_cluster(leader_empty[buf]);
+            else mbar_arrive(&acc_empty[buf]);
+        };
+        // the boxes of `extra` in the order that they are used: box e of a tile covers columns [e ecols, ...) of the warp's
+        constexpr bool USES_EXTRA = EPI == EPI_STORE || EPI == EPI_DZ;
+        const bool extra_tma = USES_EXTRA && p.extra_tma;
+        const int ecols = p.extra_type == PCB_F32 ? 32 : 64;
+        int fetched = 0;
+        auto fetch = [&](int tile, int e) {
+            if (!extra_tma || lane) return;
+            for (;;) {  // the next box with columns inside: of this tile, or the first of the next
+                if (tile >= tiles) return;
+                const int mn = tile % (p.tiles_m * p.tiles_n);
+                const int x = mn / p.tiles_m * BN + half * S::COLS + e * ecols;
+                if (e * ecols < S::COLS && x < p.n) {
+                    const int y = (mn % p.tiles_m * CTAS + rank) * BM + quad * 32;
+                    fence_async_smem();
+                    mbar_expect(&extra_full[ew], S::STAGING);
+                    tma_load(in, &p.extra_map, x, y, &extra_full[ew]);
+                    return;
+                }
+                tile += stride;
+                e = 0;
+            }
+        };
+        fetch(first_tile, 0);
         int t = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+        for (int tile = first_tile; tile < tiles; tile += stride, ++t) {
             const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
-            const int m0 = mn % p.tiles_m * BM, tn = mn / p.tiles_m, n0 = tn * BN;
+            const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, tn = mn / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
             if (!wait_warp(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
             fence_after();
@@ -262,10 +307,7 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
                 float v[32];
                 tmem_ld32(acc + 32 * c, v);
                 ld_wait();
-                if (c == chunks - 1) {
-                    fence_before();
-                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
-                }
+                if (c == chunks - 1) release(buf);
                 if (EPI == EPI_LSE) {
                     float big = -INFINITY;
 #pragma unroll
@@ -296,9 +338,38 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
                     else apply_act(p.act, v);
                     if (p.extra) {
                         float e[32];
-                        if (lane == 0) bulk_wait_read();
-                        __syncwarp();
-                        load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, (float*)stage, e);
+                        if (extra_tma) {
+                            const bool wide = p.extra_type == PCB_F32;
+                            if (wide || c % 2 == 0) {
+                                if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) break;
+                            }
+                            const uint4* irow = (const uint4*)(in + lane * 128);
+                            if (wide) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const uint4 q = irow[j ^ (lane & 7)];
+                                    e[4 * j] = __uint_as_float(q.x), e[4 * j + 1] = __uint_as_float(q.y);
+                                    e[4 * j + 2] = __uint_as_float(q.z), e[4 * j + 3] = __uint_as_float(q.w);
+                                }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint4 q = irow[(j + (c % 2) * 4) ^ (lane & 7)];
+                                    unpack2(q.x, p.bf16, e + 8 * j);
+                                    unpack2(q.y, p.bf16, e + 8 * j + 2);
+                                    unpack2(q.z, p.bf16, e + 8 * j + 4);
+                                    unpack2(q.w, p.bf16, e + 8 * j + 6);
+                                }
+                            }
+                            if (wide || c % 2 || c + 1 == chunks) {
+                                __syncwarp();
+                                fetch(tile, wide ? c + 1 : c / 2 + 1);
+                            }
+                        } else {
+                            if (lane == 0) bulk_wait_read();
+                            __syncwarp();
+                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, (float*)stage, e);
+                        }
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = EPI == EPI_DZ ? v[j] * e[j] : v[j] + e[j];
                     }
@@ -378,18 +449,18 @@ __global__ void __launch_bounds__(Shape<BN>::THREADS, 1) product(const __grid_co
                     __syncwarp();
                 }
             }
-            if (chunks == 0) {
-                fence_before();
-                if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            }
+            if (chunks == 0) release(buf);
             if (EPI == EPI_LSE && row < p.m) p.parts[(int64_t)(tn * (S::EWARPS / 4) + half) * p.m + row] = make_float2(top, sum);
         }
         if (lane == 0) bulk_wait();
+        if (*dead && extra_tma && lane == 0) mbar_wait(&extra_full[ew], fetched & 1);  // the box in flight
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
+    if (CTAS == 2) cluster_sync();
     fence_after();
-    if (warp == 1) tmem_free(tmem, S::TMEM);
+    if (warp == 1) tmem_free<CTAS>(tmem, S::TMEM);
 }
 
 // y = alpha (act(sum of the splits + bias) + extra), the splits in order
@@ -461,44 +532,63 @@ int operand_map(CUtensorMap* map, const Operand& o, int type, int rows, int k, i
     return encode_map(map, type, o.p, 2, size, stride, box);
 }
 
-// Tile width and k splits, from estimated cycles: a 64-k block of a 128 x BN tile costs its products (BN / 256 of 512
-// cycles) or its bytes into shared memory, a tile about 1200 cycles of latency besides, a split its 32-bit traffic and
-// the joining launch.
+// Tile and k splits, from estimated cycles: a 64-k block of a tile costs its products (512 cycles at a width of 256, the
+// tensor core's rate) or its bytes into shared memory where they take longer, a tile about 1200 cycles of latency besides, a
+// split its 32-bit traffic and the joining launch.
 struct Plan {
-    int bn, splits, kper;
+    int bn, ctas, splits, kper;
 };
 Plan plan(int m, int n, int k, bool may_split) {
-    const int kb = (k + BK - 1) / BK, tm = (m + BM - 1) / BM;
-    Plan best{256, 1, kb};
+    struct Tile {
+        int bn, ctas;
+        double block;
+    };
+    static const Tile shapes[] = {{256, 2, 530}, {128, 2, 300}, {128, 1, 330}, {64, 1, 240}};
+    const int kb = (k + BK - 1) / BK;
+    Plan best{256, 2, 1, kb};
     double least = 1e300;
-    for (int bn : {256, 128, 64}) {
-        const double block = bn == 256 ? 560 : bn == 128 ? 330 : 240;
+    for (const Tile& t : shapes) {
+        const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
         for (int sp = 1; sp <= (may_split ? 16 : 1); sp *= 2) {
             const int per = (kb + sp - 1) / sp;
             if (sp > 1 && (per < 4 || (sp - 1) * per >= kb)) break;
-            const int64_t tiles = (int64_t)tm * ((n + bn - 1) / bn) * sp;
-            const double waves = (double)((tiles + SMS - 1) / SMS);
-            double cost = waves * (per * block + bn * 2.0) + 1200;
+            const int slots = SMS / t.ctas;
+            const double waves = (double)((tm * tn * sp + slots - 1) / slots);
+            double cost = waves * (per * t.block + t.bn * 2.0) + 1200 + (t.ctas == 2 ? 300 : 0);
             if (sp > 1) cost += 5000 + (double)m * n * 4 * sp * 2 / (SMS * 16.0);
-            if (cost < least) least = cost, best = Plan{bn, sp, per};
+            if (cost < least) least = cost, best = Plan{t.bn, t.ctas, sp, per};
         }
     }
     return best;
 }
 
-template <int BN, int EPI>
+template <int BN, int CTAS, int EPI>
 int launch(const Params& p, cudaStream_t s) {
-    using S = Shape<BN>;
+    using S = Shape<BN, CTAS>;
     static_assert(S::SMEM <= 232448, "shared memory");
-    static const cudaError_t set = cudaFuncSetAttribute(product<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+    static const cudaError_t set = cudaFuncSetAttribute(product<BN, CTAS, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     if (set != cudaSuccess) return (int)set;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    launch_pdl_smem(product<BN, EPI>, dim3((unsigned)(tiles < SMS ? tiles : SMS)), dim3(S::THREADS), S::SMEM, s, p);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits, slots = SMS / CTAS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * CTAS));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CTAS;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = CTAS == 2 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, product<BN, CTAS, EPI>, p);
     return PCB_LAUNCH_RESULT();
 }
 template <int EPI>
-int launch(int bn, const Params& p, cudaStream_t s) {
-    return bn == 256 ? launch<256, EPI>(p, s) : bn == 128 ? launch<128, EPI>(p, s) : launch<64, EPI>(p, s);
+int launch(const Plan& pl, const Params& p, cudaStream_t s) {
+    if (pl.ctas == 2) return pl.bn == 256 ? launch<256, 2, EPI>(p, s) : launch<128, 2, EPI>(p, s);
+    return pl.bn == 128 ? launch<128, 1, EPI>(p, s) : launch<64, 1, EPI>(p, s);
 }
 
 }  // namespace
@@ -519,10 +609,10 @@ int gemm(const Gemm& g, cudaStream_t s) {
     Params p;
     memset(&p, 0, sizeof p);
     if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, BM)) return rc;
-    if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn)) return rc;
+    if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn / pl.ctas)) return rc;
     p.m = g.m, p.n = g.n, p.k = g.k;
     p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.bf16 = g.type == PCB_BF16;
-    p.tiles_m = (g.m + BM - 1) / BM, p.tiles_n = (g.n + pl.bn - 1) / pl.bn;
+    p.tiles_m = (int)(((int64_t)g.m + BM * pl.ctas - 1) / (BM * pl.ctas)), p.tiles_n = (g.n + pl.bn - 1) / pl.bn;
     p.splits = pl.splits, p.kblocks = kb, p.kper = pl.splits > 1 ? pl.kper : kb;
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;
     p.extra = g.extra, p.extra_pitch = g.extra_pitch, p.extra_type = g.extra_type;
@@ -542,11 +632,17 @@ int gemm(const Gemm& g, cudaStream_t s) {
         const uint32_t box[3] = {(uint32_t)(128 / eb), 32, 1};
         if (int rc = encode_map(&p.y, p.y_type, p.y_ptr, 3, size, stride, box)) return rc;
     }
+    if (p.extra && ((uintptr_t)p.extra & 15) == 0 && p.extra_pitch * type_bytes(p.extra_type) % 16 == 0) {
+        const uint64_t size[2] = {(uint64_t)g.n, (uint64_t)g.m}, stride[1] = {(uint64_t)(p.extra_pitch * type_bytes(p.extra_type))};
+        const uint32_t box[2] = {(uint32_t)(128 / type_bytes(p.extra_type)), 32};
+        if (int rc = encode_map(&p.extra_map, p.extra_type, p.extra, 2, size, stride, box)) return rc;
+        p.extra_tma = 1;
+    }
     int rc;
-    if (g.epi == EPI_STORE) rc = launch<EPI_STORE>(pl.bn, p, s);
-    else if (g.epi == EPI_DZ) rc = launch<EPI_DZ>(pl.bn, p, s);
-    else if (g.epi == EPI_LSE) rc = launch<EPI_LSE>(pl.bn, p, s);
-    else rc = launch<EPI_DL>(pl.bn, p, s);
+    if (g.epi == EPI_STORE) rc = launch<EPI_STORE>(pl, p, s);
+    else if (g.epi == EPI_DZ) rc = launch<EPI_DZ>(pl, p, s);
+    else if (g.epi == EPI_LSE) rc = launch<EPI_LSE>(pl, p, s);
+    else rc = launch<EPI_DL>(pl, p, s);
     if (rc || pl.splits == 1) return rc;
     const int64_t blocks = ((int64_t)g.m * g.n + 255) / 256;
     launch_pdl(join, dim3((unsigned)(blocks < 8 * SMS ? blocks : 8 * SMS)), dim3(256), s, (const float*)g.partial, pl.splits, fin);

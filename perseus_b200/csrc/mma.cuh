@@ -3,6 +3,7 @@
 // under the 128-byte swizzle (or the left one in TMEM), every completion on a shared-memory mbarrier. No multicast.
 #pragma once
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include "arith.cuh"
 
@@ -44,6 +45,34 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// the same by one block of a pair, completing on a barrier of either (`bar`: a cluster address)
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ pairs of blocks
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// the cluster address of block `rank`'s copy of a shared-memory object
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // ------------------------------------------------------------------------------------------------ barriers
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -65,13 +94,22 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 }
 
 // ------------------------------------------------------------------------------------------------ TMEM
-// One warp allocates `cols` (a power of two from 32 to 512) columns of 128 lanes x 32 bits, and frees them
+// One warp (of each block of a pair) allocates `cols` (a power of two from 32 to 512) columns of 128 lanes x 32 bits, and
+// frees them
+template <int CTAS = 1>
 __device__ __forceinline__ void tmem_alloc(uint32_t* at, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
 }
+template <int CTAS = 1>
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+    if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -122,12 +160,21 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, bool a_mn, bool b_m
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
            ((uint32_t)(n / 8) << 17) | ((uint32_t)(m / 16) << 24);
 }
-// acc (TMEM) = or += A B^T over 16 k-values, issued by one thread
+// acc (TMEM) = or += A B^T over 16 k-values, issued by one thread. A pair's product has 256 rows, 128 of A and of the
+// accumulator in each block, and half of B's rows in each: the first block's thread issues it, the operands lie at the same
+// offsets in both
+template <int CTAS = 1>
 __device__ __forceinline__ void mma_ss(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-        : "memory");
+    if (CTAS == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
 }
 // the same with A in TMEM (two 16-bit k-values per 32-bit column)
 __device__ __forceinline__ void mma_ts(uint32_t acc, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -136,9 +183,16 @@ __device__ __forceinline__ void mma_ts(uint32_t acc, uint32_t a, uint64_t b, uin
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
         : "memory");
 }
-// arrives on `bar` when this thread's products so far are done
+// arrives on `bar` (of a pair: on both blocks') when this thread's products so far are done
+template <int CTAS = 1>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    if (CTAS == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_addr(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------ 32-bit pieces
@@ -158,6 +212,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
     if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// and back: v[0] the lower half, v[1] the upper
+__device__ __forceinline__ void unpack2(uint32_t x, bool bf16, float* v) {
+    if (bf16) {
+        v[0] = __uint_as_float(x << 16);
+        v[1] = __uint_as_float(x & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*(const __half2*)&x);
+        v[0] = f.x, v[1] = f.y;
+    }
 }
 
 }  // namespace mma
