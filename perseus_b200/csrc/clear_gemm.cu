@@ -45,7 +45,7 @@ struct Shape {
 struct alignas(64) Params {
     CUtensorMap a, b, y, extra_map;
     int m, n, k;
-    int a_mn, b_mn, bf16;
+    int a_mn, b_mn, a_panels, b_panels, bf16;
     int tiles_m, tiles_n, splits, kblocks, kper;  // k blocks in all and of one split
     Act act;
     const void* bias;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
     uint64_t* drain = extra_full + S::EWARPS;
     uint32_t* tmem_at = (uint32_t*)(drain + 1);
     volatile int* dead = (volatile int*)(tmem_at + 1);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = warp_index(), lane = threadIdx.x % 32;
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
@@ -188,66 +188,81 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
     const int tiles = p.tiles_m * p.tiles_n * p.splits;
     const int first_tile = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            for (int tile = first_tile; tile < tiles && !*dead; tile += stride) {
-                const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
-                const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, n0 = mn / p.tiles_m * BN + rank * S::B_ROWS;
-                const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int st = it % S::STAGES;
-                    if (it >= S::STAGES && !wait(&empty[st], (it / S::STAGES - 1) & 1, dead, &g_gemm_timeouts)) break;
-                    unsigned char* sa = base + st * S::STAGE;
-                    unsigned char* sb = sa + S::A_BYTES;
-                    // a pair's loads all complete on the first block's barrier, whose thread issues the products
-                    if (rank == 0) mbar_expect(&full[st], CTAS * S::STAGE);
-                    const uint32_t bar = CTAS == 2 ? cluster_addr(&full[st], 0) : 0;
-                    auto box = [&](void* dst, const CUtensorMap* map, int x, int y) {
-                        if (CTAS == 2) tma_load_pair(dst, map, x, y, bar);
-                        else tma_load(dst, map, x, y, &full[st]);
+        Ring<S::STAGES> r;
+        int loaded = 0;
+        bool ok = true, ready = true;
+        for (int tile = first_tile; tile < tiles && ok; tile += stride) {
+            const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
+            const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, n0 = mn / p.tiles_m * BN + rank * S::B_ROWS;
+            const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
+            for (int kb = kb0; kb < kb1; ++kb, ++loaded, r.next()) {
+                // a fresh barrier's preceding phase counts as done: the first round does not wait
+                if (!__all_sync(~0u, ready)) ok = wait_warp(&empty[r.stage], r.phase ^ 1, dead, &g_gemm_timeouts);
+                if (!ok) break;
+                Ring<S::STAGES> ahead = r;
+                ahead.next();
+                ready = peek(&empty[ahead.stage], ahead.phase ^ 1);
+                unsigned char* sa = base + r.stage * S::STAGE;
+                unsigned char* sb = sa + S::A_BYTES;
+                uint64_t* bar = &full[r.stage];
+                // a pair's loads all complete on the first block's barrier, whose warp issues the products
+                const uint32_t pair_bar = CTAS == 2 ? cluster_addr(bar, 0) : 0;
+                if (elect()) {
+                    if (rank == 0) mbar_expect(bar, CTAS * S::STAGE);
+                    auto box = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
+                        if (CTAS == 2) tma_load_pair(dst, map, x, y, z, pair_bar);
+                        else tma_load(dst, map, x, y, z, bar);
                     };
-                    if (p.a_mn) {
-                        for (int j = 0; j < BM / 64; ++j) box(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK);
-                    } else {
-                        box(sa, &p.a, kb * BK, m0);
-                    }
-                    if (p.b_mn) {
-                        for (int j = 0; j < S::B_ROWS / 64; ++j) box(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK);
-                    } else {
-                        box(sb, &p.b, kb * BK, n0);
-                    }
+                    // rows adjacent: 64 x 64 panels, together in one box where the rows are whole panels (operand_map)
+                    if (!p.a_mn) box(sa, &p.a, kb * BK, m0, 0);
+                    else if (p.a_panels) box(sa, &p.a, 0, kb * BK, m0 / 64);
+                    else
+                        for (int j = 0; j < BM / 64; ++j) box(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK, 0);
+                    if (!p.b_mn) box(sb, &p.b, kb * BK, n0, 0);
+                    else if (p.b_panels) box(sb, &p.b, 0, kb * BK, n0 / 64);
+                    else
+                        for (int j = 0; j < S::B_ROWS / 64; ++j) box(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK, 0);
                 }
+                __syncwarp();
             }
-            if (*dead)  // the loads in flight: into the first block's, their barrier's; the second's are behind the cluster's end
-                for (int i = max(0, it - S::STAGES); i < it && rank == 0; ++i) mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         }
+        if (!ok && rank == 0)  // the loads in flight: a pair's complete here, before the cluster's end
+            for (int i = max(0, loaded - S::STAGES); i < loaded; ++i) mbar_wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t idesc = instr_desc(p.bf16, p.a_mn, p.b_mn, BM * CTAS, BN);
             const uint32_t a_lbo = p.a_mn ? 8192 : 16, a_step = (p.a_mn ? 2048 : 32) >> 4;
             const uint32_t b_lbo = p.b_mn ? 8192 : 16, b_step = (p.b_mn ? 2048 : 32) >> 4;
-            int it = 0, t = 0;
-            for (int tile = first_tile; tile < tiles && !*dead; tile += stride, ++t) {
+            const uint64_t a_desc = smem_desc(smem_addr(base), a_lbo, 1024), b_desc = smem_desc(smem_addr(base + S::A_BYTES), b_lbo, 1024);
+            Ring<S::STAGES> r;
+            Ring<2> out;
+            bool ok = true, ready = false;
+            for (int tile = first_tile; tile < tiles && ok; tile += stride, out.next()) {
                 const int sp = tile / (p.tiles_m * p.tiles_n);
                 const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
-                const int buf = t & 1;
-                if (t >= 2 && !wait(&acc_empty[buf], (t / 2 - 1) & 1, dead, &g_gemm_timeouts)) break;
+                ok = wait_warp(&acc_empty[out.stage], out.phase ^ 1, dead, &g_gemm_timeouts);
+                if (!ok) break;
                 fence_after();
-                const uint32_t acc = tmem + buf * BN;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int st = it % S::STAGES;
-                    if (!wait(&full[st], (it / S::STAGES) & 1, dead, &g_gemm_timeouts)) break;
+                const uint32_t acc = tmem + out.stage * BN;
+                for (int kb = kb0; kb < kb1; ++kb, r.next()) {
+                    if (!__all_sync(~0u, ready)) ok = wait_warp(&full[r.stage], r.phase, dead, &g_gemm_timeouts);
+                    if (!ok) break;
                     fence_after();
-                    const uint32_t sa = smem_addr(base + st * S::STAGE);
-                    const uint64_t da = smem_desc(sa, a_lbo, 1024), db = smem_desc(sa + S::A_BYTES, b_lbo, 1024);
+                    Ring<S::STAGES> ahead = r;
+                    ahead.next();
+                    ready = peek(&full[ahead.stage], ahead.phase);
+                    const uint64_t da = a_desc + (uint32_t)(r.stage * (S::STAGE >> 4)), db = b_desc + (uint32_t)(r.stage * (S::STAGE >> 4));
+                    if (elect()) {
 #pragma unroll
-                    for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
-                    mma_commit<CTAS>(&empty[st]);
+                        for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
+                        mma_commit<CTAS>(&empty[r.stage]);
+                        if (kb + 1 == kb1) mma_commit<CTAS>(&acc_full[out.stage]);
+                    }
+                    __syncwarp();
                 }
-                mma_commit<CTAS>(&acc_full[buf]);
             }
-            if (*dead) {  // the products in flight
-                mma_commit<CTAS>(drain);
+            if (!ok) {  // the products in flight
+                if (elect()) mma_commit<CTAS>(drain);
                 mbar_wait(drain, 0);
             }
         }
@@ -271,7 +286,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
         int fetched = 0;
         auto fetch = [&](int tile, int e) {
             if (!extra_tma || lane) return;
-            for (;;) {  // the next box with columns inside: of this tile, or the first of the next
+            while (USES_EXTRA) {  // the next box with columns inside: of this tile, or the first of the next
                 if (tile >= tiles) return;
                 const int mn = tile % (p.tiles_m * p.tiles_n);
                 const int x = mn / p.tiles_m * BN + half * S::COLS + e * ecols;
@@ -292,7 +307,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
             const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
             const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, tn = mn / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
-            if (!wait_warp(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
+            if (!wait_warp<true>(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
             const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));
@@ -524,12 +539,21 @@ int encode_map(CUtensorMap* map, int type, const void* p, int dims, const uint64
 
 namespace {
 
-// an operand's map: boxes of 64 adjacent values by `tile` rows (k adjacent), or by 64 k (rows adjacent)
+// an operand's map, three dimensions always: boxes of 64 adjacent values by `tile` rows (k adjacent), of 64 adjacent rows by
+// 64 k (rows adjacent), or of tile / 64 such panels where the rows are a multiple of 64 (each copy costs its issuing warp
+// some 80 cycles)
+bool panels(const Operand& o, int rows) { return !o.k_adjacent && rows % 64 == 0; }
 int operand_map(CUtensorMap* map, const Operand& o, int type, int rows, int k, int tile) {
-    const uint64_t size[2] = {(uint64_t)(o.k_adjacent ? k : rows), (uint64_t)(o.k_adjacent ? rows : k)};
-    const uint64_t stride[1] = {(uint64_t)o.pitch * 2};
-    const uint32_t box[2] = {64, (uint32_t)(o.k_adjacent ? tile : BK)};
-    return encode_map(map, type, o.p, 2, size, stride, box);
+    const uint64_t pitch = (uint64_t)o.pitch * 2;
+    if (panels(o, rows)) {
+        const uint64_t size[3] = {64, (uint64_t)k, (uint64_t)rows / 64}, stride[2] = {pitch, 128};
+        const uint32_t box[3] = {64, BK, (uint32_t)tile / 64};
+        return encode_map(map, type, o.p, 3, size, stride, box);
+    }
+    const uint64_t size[3] = {(uint64_t)(o.k_adjacent ? k : rows), (uint64_t)(o.k_adjacent ? rows : k), 1};
+    const uint64_t stride[2] = {pitch, pitch};
+    const uint32_t box[3] = {64, (uint32_t)(o.k_adjacent ? tile : BK), 1};
+    return encode_map(map, type, o.p, 3, size, stride, box);
 }
 
 // Tile and k splits, from estimated cycles: a 64-k block of a tile costs its products (512 cycles at a width of 256, the
@@ -611,7 +635,7 @@ int gemm(const Gemm& g, cudaStream_t s) {
     if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, BM)) return rc;
     if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn / pl.ctas)) return rc;
     p.m = g.m, p.n = g.n, p.k = g.k;
-    p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.bf16 = g.type == PCB_BF16;
+    p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.a_panels = panels(g.a, g.m), p.b_panels = panels(g.b, g.n), p.bf16 = g.type == PCB_BF16;
     p.tiles_m = (int)(((int64_t)g.m + BM * pl.ctas - 1) / (BM * pl.ctas)), p.tiles_n = (g.n + pl.bn - 1) / pl.bn;
     p.splits = pl.splits, p.kblocks = kb, p.kper = pl.splits > 1 ? pl.kper : kb;
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;

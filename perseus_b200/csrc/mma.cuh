@@ -46,11 +46,11 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 }
 
 // the same by one block of a pair, completing on a barrier of either (`bar`: a cluster address)
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 
@@ -77,21 +77,60 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// A bounded wait that also gives up when another role of the block has (`dead`, shared memory): false then, and counted
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned int* timeouts) {
-    for (uint32_t it = 0; it < MBAR_WAIT_LIMIT; ++it) {
-        if (mbar_test(bar, parity)) return true;
-        if ((it & 255) == 255 && *dead) return false;
+// whether the phase is done, without waiting: asked for the next stage before this one's instructions are issued, the
+// answer costs nothing when it is used
+__device__ __forceinline__ bool peek(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// A bounded wait of a whole warp that also gives up when another role of the block has (`dead`, shared memory): false then,
+// and counted. RELAXED waits (for a tile's worth of work, not for the next block) poll from one lane and sleep in between,
+// so that the epilogue's warps leave the barriers' unit to the warps that feed the products.
+template <bool RELAXED = false>
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned int* timeouts) {
+    bool ok = true;
+    if (!RELAXED || threadIdx.x % 32 == 0) {
+        for (uint32_t it = 1; !mbar_test(bar, parity); ++it) {
+            if (RELAXED) __nanosleep(32);
+            if ((it & 255) == 0 && *dead) {
+                ok = false;
+                break;
+            }
+            if (it >= MBAR_WAIT_LIMIT) {
+                *dead = 1;
+                atomicAdd(timeouts, 1u);
+                ok = false;
+                break;
+            }
+        }
     }
-    *dead = 1;
-    atomicAdd(timeouts, 1u);
-    return false;
+    return __all_sync(~0u, ok);
 }
 
-// the same for a whole warp: every lane takes the same way
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned int* timeouts) {
-    return __all_sync(~0u, wait(bar, parity, dead, timeouts));
+// One lane of a converged warp. The loops that feed the TMA engine and the tensor core run on whole warps, with only the
+// instructions themselves under elect(): addresses, descriptors and phases then stay in uniform registers, which those
+// instructions take. (Run on one lane, the loop's bookkeeping cost 280 cycles per 64-k block and each product was held up by
+// moves into uniform registers: 8192 x 8192 x 8192 took 829 us.)
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
+__device__ __forceinline__ int warp_index() { return __shfl_sync(~0u, (int)threadIdx.x / 32, 0); }
+// A ring of N stages: the stage, and the parity of its barriers' phase
+template <int N>
+struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++stage == N) stage = 0, phase ^= 1;
+    }
+};
 
 // ------------------------------------------------------------------------------------------------ TMEM
 // One warp (of each block of a pair) allocates `cols` (a power of two from 32 to 512) columns of 128 lanes x 32 bits, and
