@@ -29,40 +29,19 @@ __device__ __forceinline__ void store(void* p, size_t i, int type, float v) {
 inline size_t type_bytes(int type) { return type == PCB_F32 ? 4 : 2; }
 
 // ------------------------------------------------------------------------------------------------ activations
+// PCB_ACT_POLY: value sum c[i] u^i and slope sum d[i] u^i at u = z inv_bound
 struct Act {
     int kind;
     float inv_bound;
-    float c[8];
+    float c[8], d[7];
 };
 inline Act make_act(int kind, float bound, const float* coef) {
-    Act a;
-    a.kind = kind;
-    a.inv_bound = kind == PCB_ACT_POLY ? 1.0f / bound : 1.0f;
-    for (int i = 0; i < 8; ++i) a.c[i] = kind == PCB_ACT_POLY ? coef[i] : 0.0f;
+    Act a = {kind, 1.0f, {}, {}};
+    if (kind != PCB_ACT_POLY) return a;
+    a.inv_bound = 1.0f / bound;
+    for (int i = 0; i < 8; ++i) a.c[i] = coef[i];
+    for (int i = 1; i < 8; ++i) a.d[i - 1] = (float)((double)i * coef[i] / bound);
     return a;
-}
-__device__ __forceinline__ float act(const Act& a, float z) {
-    if (a.kind == PCB_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    if (a.kind == PCB_ACT_POLY) {
-        const float u = z * a.inv_bound;
-        float r = a.c[7];
-#pragma unroll
-        for (int i = 6; i >= 0; --i) r = fmaf(r, u, a.c[i]);
-        return r;
-    }
-    return z;
-}
-__device__ __forceinline__ float act_slope(const Act& a, float z) {
-    if (a.kind == PCB_ACT_GELU)  // Phi(z) + z phi(z)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * expf(-0.5f * z * z);
-    if (a.kind == PCB_ACT_POLY) {
-        const float u = z * a.inv_bound;
-        float r = 7.0f * a.c[7];
-#pragma unroll
-        for (int i = 6; i >= 1; --i) r = fmaf(r, u, (float)i * a.c[i]);
-        return r * a.inv_bound;
-    }
-    return 1.0f;
 }
 
 // ------------------------------------------------------------------------------------------------ checks

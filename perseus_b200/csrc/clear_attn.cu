@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     uint64_t* drain = pv_done + 1;
     uint32_t* tmem_at = (uint32_t*)(drain + 1);
     volatile int* dead = (volatile int*)(tmem_at + 1);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = warp_index(), lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -172,65 +172,86 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     const int b0 = min(blocks, split * per), n = min(blocks, b0 + per) - b0;
 
     if (warp == 0) {
-        if (lane == 0 && n > 0) {
-            mbar_expect(q_full, (DP / 64) * 128 * p.group * p.tokens);
-            for (int h = 0; h < DP / 64; ++h) tma_load(base + h * S::HALF, &p.q, 64 * h, kh * p.group, q0 + t0, q_full);
-            int i = 0;
-            for (; i < 2 * n; ++i) {  // K and V in turn
-                const int st = i % S::RING;
-                if (i >= S::RING && !wait(&empty[st], (i / S::RING - 1) & 1, dead, &g_attn_timeouts)) break;
-                mbar_expect(&full[st], S::OPERAND);
-                for (int h = 0; h < DP / 64; ++h)
-                    tma_load(ring + st * S::OPERAND + h * S::HALF, i % 2 ? &p.v : &p.k, 64 * h, kh, k0 + (b0 + i / 2) * KEYS, &full[st]);
+        if (n > 0) {
+            if (elect()) {
+                mbar_expect(q_full, (DP / 64) * 128 * p.group * p.tokens);
+                for (int h = 0; h < DP / 64; ++h) tma_load(base + h * S::HALF, &p.q, 64 * h, kh * p.group, q0 + t0, q_full);
             }
-            if (*dead) {  // the loads in flight
+            __syncwarp();
+            Ring<S::RING> rg;
+            int i = 0;
+            bool ok = true;
+            for (; i < 2 * n; ++i, rg.next()) {  // K and V in turn
+                ok = wait_warp(&empty[rg.stage], rg.phase ^ 1, dead, &g_attn_timeouts);
+                if (!ok) break;
+                if (elect()) {
+                    mbar_expect(&full[rg.stage], S::OPERAND);
+                    for (int h = 0; h < DP / 64; ++h)
+                        tma_load(ring + rg.stage * S::OPERAND + h * S::HALF, i % 2 ? &p.v : &p.k, 64 * h, kh, k0 + (b0 + i / 2) * KEYS,
+                                 &full[rg.stage]);
+                }
+                __syncwarp();
+            }
+            if (!ok) {  // the loads in flight
                 mbar_wait(q_full, 0);
                 for (int f = max(0, i - S::RING); f < i; ++f) mbar_wait(&full[f % S::RING], (f / S::RING) & 1);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             const bool bf16 = p.a.type == PCB_BF16;
             const int ksteps = (p.a.dim + 15) / 16, nd = (p.a.dim + 15) / 16 * 16;
             const uint32_t is = instr_desc(bf16, false, false, ROWS, KEYS) | (p.negate ? 1u << 13 : 0u);
             const uint32_t ipv = instr_desc(bf16, false, true, ROWS, nd);
             const uint64_t dq = smem_desc(smem_addr(base), 16, 1024);
-            bool ok = wait(q_full, 0, dead, &g_attn_timeouts);
-            auto scores = [&](int j) {  // S = Q K_j^T
-                const int i = 2 * j, st = i % S::RING;
-                if (!wait(&full[st], (i / S::RING) & 1, dead, &g_attn_timeouts)) return false;
+            const uint64_t dk0 = smem_desc(smem_addr(ring), 16, 1024), dv0 = smem_desc(smem_addr(ring), S::HALF, 1024);
+            Ring<S::RING> rg;
+            bool ok = wait_warp(q_full, 0, dead, &g_attn_timeouts);
+            auto scores = [&](uint64_t dk, int st) {  // S = Q K^T
                 fence_after();
-                const uint64_t dk = smem_desc(smem_addr(ring + st * S::OPERAND), 16, 1024);
-                for (int s = 0; s < ksteps; ++s) {
-                    const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
-                    mma_ss(tmem + S::S, dq + off, dk + off, is, s > 0);
+                if (elect()) {
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s) {
+                        const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
+                        if (s < ksteps) mma_ss(tmem + S::S, dq + off, dk + off, is, s > 0);
+                    }
+                    mma_commit(s_full);
+                    mma_commit(&empty[st]);
                 }
-                mma_commit(s_full);
-                mma_commit(&empty[st]);
-                return true;
+                __syncwarp();
             };
-            ok = ok && scores(0);
+            auto next_scores = [&]() {  // waits for the next K block in the ring and forms its scores
+                ok = wait_warp(&full[rg.stage], rg.phase, dead, &g_attn_timeouts);
+                if (ok) scores(dk0 + (uint32_t)(rg.stage * (S::OPERAND >> 4)), rg.stage);
+                rg.next();
+            };
+            if (ok) next_scores();
             for (int j = 0; j < n && ok; ++j) {
-                ok = wait(p_ready, j & 1, dead, &g_attn_timeouts);
+                const Ring<S::RING> rv = rg;  // this block's V; the next K after it
+                rg.next();
+                ok = wait_warp(p_ready, j & 1, dead, &g_attn_timeouts);
                 if (!ok) break;
                 fence_after();
-                if (S::APART && j + 1 < n) ok = scores(j + 1);
-                const int i = 2 * j + 1, st = i % S::RING;
-                ok = ok && wait(&full[st], (i / S::RING) & 1, dead, &g_attn_timeouts);
+                if (S::APART && j + 1 < n) next_scores();
+                ok = ok && wait_warp(&full[rv.stage], rv.phase, dead, &g_attn_timeouts);
                 if (!ok) break;
                 fence_after();
-                const uint64_t dv = smem_desc(smem_addr(ring + st * S::OPERAND), S::HALF, 1024);
-                for (int s = 0; s < KEYS / 16; ++s)
-                    mma_ts(tmem + S::O, tmem + S::P + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, j > 0 || s > 0);
-                mma_commit(pv_done);
-                mma_commit(&empty[st]);
+                const uint64_t dv = dv0 + (uint32_t)(rv.stage * (S::OPERAND >> 4));
+                if (elect()) {
+#pragma unroll
+                    for (int s = 0; s < KEYS / 16; ++s)
+                        mma_ts(tmem + S::O, tmem + S::P + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, j > 0 || s > 0);
+                    mma_commit(pv_done);
+                    mma_commit(&empty[rv.stage]);
+                }
+                __syncwarp();
                 if (!S::APART && j + 1 < n) {  // the next scores take P's place
-                    ok = wait(pv_done, j & 1, dead, &g_attn_timeouts);
-                    ok = ok && scores(j + 1);
+                    ok = wait_warp(pv_done, j & 1, dead, &g_attn_timeouts);
+                    if (ok) next_scores();
                 }
             }
-            if (*dead) {  // the products in flight
-                mma_commit(drain);
+            if (!ok) {  // the products in flight
+                if (elect()) mma_commit(drain);
                 mbar_wait(drain, 0);
             }
         }

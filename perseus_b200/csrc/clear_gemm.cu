@@ -63,50 +63,49 @@ struct alignas(64) Params {
 };
 
 // ------------------------------------------------------------------------------------------------ epilogue pieces
-// z Phi(z) and its derivative. Phi from Abramowitz and Stegun 7.1.26 (absolute error below 1.5e-7 in erf): for x = |z| /
-// sqrt 2, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x). One reciprocal and one exponential.
-__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = rcp(fmaf(0.3275911f, x, 1.0f));
-    const float e = ex2(-LOG2E * x * x);
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    const float half = 0.5f * p * t * e;
-    *gauss = e;
-    return z < 0.0f ? half : 1.0f - half;
+// GELU z Phi(z) and its slope Phi(z) + z phi(z), two values at a time. Phi from Abramowitz and Stegun 7.1.26 (absolute error
+// below 1.5e-7 in erf): for x = |z| / sqrt 2, h = erfc(x) / 2 = (a1 t + ... + a5 t^5) exp(-x^2) / 2, t = 1 / (1 + 0.3275911 x);
+// z Phi(z) = max(z, 0) - |z| h, Phi(z) = 1/2 + sign(z) (1/2 - h). A reciprocal and an exponential per value.
+__device__ __forceinline__ f32x2 half_erfc(f32x2 z, f32x2 size, f32x2& gauss) {
+    float x0, x1, e0, e1;
+    parts(fma2(size, both(0.3275911f * 0.70710678118654752f), both(1.0f)), x0, x1);
+    const f32x2 t = two(rcp(x0), rcp(x1));
+    parts(mul2(mul2(z, both(-0.5f * LOG2E)), z), e0, e1);
+    gauss = two(ex2(e0), ex2(e1));
+    f32x2 q = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    q = fma2(q, t, both(0.5f * 1.421413741f));
+    q = fma2(q, t, both(0.5f * -0.284496736f));
+    q = fma2(q, t, both(0.5f * 0.254829592f));
+    return mul2(mul2(q, t), gauss);
 }
-__device__ __forceinline__ void apply_act(const Act& a, float* v) {
-    if (a.kind == PCB_ACT_GELU) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float g;
-            v[j] *= normal_cdf(v[j], &g);
-        }
-    } else if (a.kind == PCB_ACT_POLY) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float u = v[j] * a.inv_bound;
-            float r = a.c[7];
-#pragma unroll
-            for (int i = 6; i >= 0; --i) r = fmaf(r, u, a.c[i]);
-            v[j] = r;
-        }
-    }
+__device__ __forceinline__ f32x2 gelu2(f32x2 z) {
+    float z0, z1;
+    parts(z, z0, z1);
+    const f32x2 size = two(fabsf(z0), fabsf(z1));
+    f32x2 g;
+    const f32x2 h = half_erfc(z, size, g);
+    return fma2(mul2(size, both(-1.0f)), h, two(fmaxf(z0, 0.0f), fmaxf(z1, 0.0f)));
 }
-__device__ __forceinline__ void apply_slope(const Act& a, float* v) {
-    if (a.kind == PCB_ACT_GELU) {
+__device__ __forceinline__ f32x2 gelu_slope2(f32x2 z) {
+    float z0, z1, r0, r1;
+    parts(z, z0, z1);
+    f32x2 g;
+    const f32x2 h = half_erfc(z, two(fabsf(z0), fabsf(z1)), g);
+    parts(fma2(h, both(-1.0f), both(0.5f)), r0, r1);
+    const f32x2 cdf = add2(two(copysignf(r0, z0), copysignf(r1, z1)), both(0.5f));
+    return fma2(mul2(z, both(0.3989422804014327f)), g, cdf);
+}
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ f32x2 act2(const Act& a, f32x2 z) {
+    if (ACT == PCB_ACT_GELU) return SLOPE ? gelu_slope2(z) : gelu2(z);
+    if (ACT == PCB_ACT_POLY) {
+        const f32x2 u = mul2(z, both(a.inv_bound));
+        f32x2 r = SLOPE ? both(a.d[6]) : both(a.c[7]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float g;
-            const float c = normal_cdf(v[j], &g);
-            v[j] = fmaf(v[j] * 0.3989422804014327f, g, c);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = act_slope(a, v[j]);
+        for (int i = SLOPE ? 5 : 6; i >= 0; --i) r = fma2(r, u, both(SLOPE ? a.d[i] : a.c[i]));
+        return r;
     }
+    return z;
 }
 
 // Sum over the warp's lanes of each of 32 values: lane l returns the sum of v[l], in a fixed order
@@ -124,25 +123,38 @@ __device__ __forceinline__ float lane_sums(float* v) {
     return v[0];
 }
 
-// 32 x 32 values of a row-major array at (row0, col0), rows and columns past the end as zero, to the lane's row: read
-// along the rows (lane = column), turned through the warp's staging buffer
-__device__ __forceinline__ void load_block(const void* p, int64_t pitch, int type, int row0, int col0, int m, int n, float* stage,
-                                           float* out) {
+// 32 x 32 values of a row-major array at (row0, col0), rows and columns past the end as zero, in 32 bits into the warp's
+// staging buffer as a box of the TMA engine would lie there; read along the rows (lane = column). For arrays that the engine
+// cannot read.
+__device__ __noinline__ void load_block(const void* p, int64_t pitch, int type, int row0, int col0, int m, int n, unsigned char* stage) {
     const int lane = threadIdx.x % 32;
     const bool in = col0 + lane < n;
-    float t[32];
-#pragma unroll
-    for (int r = 0; r < 32; ++r) t[r] = in && row0 + r < m ? load(p, (int64_t)(row0 + r) * pitch + col0 + lane, type) : 0.0f;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) stage[r * 32 + (lane ^ r)] = t[r];
+#pragma unroll 16
+    for (int r = 0; r < 32; ++r)
+        *(float*)(stage + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4) =
+            in && row0 + r < m ? load(p, (int64_t)(row0 + r) * pitch + col0 + lane, type) : 0.0f;
     __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 32; ++c) out[c] = stage[lane * 32 + (c ^ lane)];
+}
+// A box of the staging buffer (32 rows x 128 bytes, 16-byte pieces swizzled by the row) to rows that the engine cannot write
+__device__ __noinline__ void store_block(const unsigned char* stage, bool narrow, void* y, int64_t pitch, int rows, int cols, bool add) {
+    const int lane = threadIdx.x % 32;
+    for (int r = 0; r < rows; ++r) {
+        const unsigned char* row = stage + r * 128;
+        for (int c = lane; c < min(cols, narrow ? 64 : 32); c += 32) {
+            if (narrow) {
+                ((uint16_t*)y)[r * pitch + c] = *(const uint16_t*)(row + ((c / 8) ^ (r & 7)) * 16 + c % 8 * 2);
+            } else {
+                const float v = *(const float*)(row + ((c / 4) ^ (r & 7)) * 16 + c % 4 * 4);
+                float* at = (float*)y + r * pitch + c;
+                *at = add ? *at + v : v;
+            }
+        }
+    }
     __syncwarp();
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
-template <int BN, int CTAS, int EPI>
+template <int BN, int CTAS, int EPI, int ACT>
 __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __grid_constant__ Params p) {
     using S = Shape<BN, CTAS>;
     extern __shared__ unsigned char raw[];
@@ -307,86 +319,111 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
             const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
             const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, tn = mn / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
+            auto bias_of = [&](int col) { return col + lane < p.n ? load(p.bias, col + lane, p.bias_type) : 0.0f; };
+            float next_bias = 0.0f;
+            if (USES_EXTRA && p.bias) next_bias = bias_of(first);
             if (!wait_warp<true>(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
             const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));
-            float top = -INFINITY, sum = 0.0f;
-            VocabRow vr = {0.0f, 0.0f, -1, 0};
-            if (EPI == EPI_DL && row < p.m) vr = p.rows[row];
+            float top = -INFINITY, sum = 0.0f, lse2 = 0.0f, weight = 0.0f;
+            int target = -1;  // the row's column among this warp's, if it is there
+            if (EPI == EPI_DL && row < p.m) {
+                const VocabRow vr = p.rows[row];
+                lse2 = vr.lse2, weight = vr.weight, target = vr.target - p.col0 - first;
+            }
+            if (EPI == EPI_LSE && row < p.m) {
+                const int64_t at = p.targets[row] - first;
+                target = at >= 0 && at < S::COLS ? (int)at : -1;
+            }
             uint32_t held[16];
-            int64_t target = -1;
-            if (EPI == EPI_LSE && row < p.m) target = p.targets[row];
             for (int c = 0; c < chunks; ++c) {
                 const int col0 = first + 32 * c;
                 float v[32];
                 tmem_ld32(acc + 32 * c, v);
                 ld_wait();
                 if (c == chunks - 1) release(buf);
+                const bool has_target = (EPI == EPI_LSE || EPI == EPI_DL) && __any_sync(~0u, (unsigned)(target - 32 * c) < 32u);
                 if (EPI == EPI_LSE) {
-                    float big = -INFINITY;
+                    if (has_target) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (col0 + j >= p.n) v[j] = -INFINITY;
-                        else if (target == col0 + j) p.hit[row] = v[j];
-                        v[j] *= LOG2E;
-                        big = fmaxf(big, v[j]);
+                        for (int j = 0; j < 32; ++j)
+                            if (target == 32 * c + j && col0 + j < p.n) p.hit[row] = v[j];
                     }
-                    const float nt = fmaxf(top, big);
-                    sum *= ex2(top - nt);
-                    float s4[4] = {};
+                    if (col0 + 32 > p.n) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s4[j % 4] += ex2(v[j] - nt);
-                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                        for (int j = 0; j < 32; ++j) v[j] = col0 + j < p.n ? v[j] : -INFINITY;
+                    }
+                    float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                    for (int j = 4; j < 32; ++j) m4[j % 4] = fmaxf(m4[j % 4], v[j]);
+                    const float nt = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * LOG2E);
+                    f32x2 s2[2] = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float a, b;
+                        parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-nt)), a, b);
+                        s2[j / 2 % 2] = add2(s2[j / 2 % 2], two(ex2(a), ex2(b)));
+                    }
+                    float a, b;
+                    parts(add2(s2[0], s2[1]), a, b);
+                    sum = fmaf(sum, ex2(top - nt), a + b);
                     top = nt;
                     continue;
                 }
                 if (EPI == EPI_STORE || EPI == EPI_DZ) {
                     if (p.bias) {
                         __syncwarp();
-                        bias[lane] = col0 + lane < p.n ? load(p.bias, col0 + lane, p.bias_type) : 0.0f;
+                        bias[lane] = next_bias;
                         __syncwarp();
+                        if (c + 1 < chunks) next_bias = bias_of(col0 + 32);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += bias[j];
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 q = *(const float4*)(bias + j);
+                            parts(add2(two(v[j], v[j + 1]), two(q.x, q.y)), v[j], v[j + 1]);
+                            parts(add2(two(v[j + 2], v[j + 3]), two(q.z, q.w)), v[j + 2], v[j + 3]);
+                        }
                     }
-                    if (EPI == EPI_DZ) apply_slope(p.act, v);
-                    else apply_act(p.act, v);
+                    if (ACT != PCB_ACT_NONE) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) parts(act2<ACT, EPI == EPI_DZ>(p.act, two(v[j], v[j + 1])), v[j], v[j + 1]);
+                    }
                     if (p.extra) {
-                        float e[32];
-                        if (extra_tma) {
-                            const bool wide = p.extra_type == PCB_F32;
-                            if (wide || c % 2 == 0) {
-                                if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) break;
-                            }
-                            const uint4* irow = (const uint4*)(in + lane * 128);
-                            if (wide) {
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const uint4 q = irow[j ^ (lane & 7)];
-                                    e[4 * j] = __uint_as_float(q.x), e[4 * j + 1] = __uint_as_float(q.y);
-                                    e[4 * j + 2] = __uint_as_float(q.z), e[4 * j + 3] = __uint_as_float(q.w);
-                                }
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const uint4 q = irow[(j + (c % 2) * 4) ^ (lane & 7)];
-                                    unpack2(q.x, p.bf16, e + 8 * j);
-                                    unpack2(q.y, p.bf16, e + 8 * j + 2);
-                                    unpack2(q.z, p.bf16, e + 8 * j + 4);
-                                    unpack2(q.w, p.bf16, e + 8 * j + 6);
-                                }
-                            }
-                            if (wide || c % 2 || c + 1 == chunks) {
-                                __syncwarp();
-                                fetch(tile, wide ? c + 1 : c / 2 + 1);
-                            }
-                        } else {
+                        const bool wide = !extra_tma || p.extra_type == PCB_F32;
+                        if (!extra_tma) {
                             if (lane == 0) bulk_wait_read();
                             __syncwarp();
-                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, (float*)stage, e);
+                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, stage);
+                        } else if (wide || c % 2 == 0) {
+                            if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) break;
                         }
+                        const uint4* irow = (const uint4*)((extra_tma ? in : stage) + lane * 128);
+                        auto join = [&](int j, float e0, float e1) {
+                            const f32x2 a = two(v[j], v[j + 1]), e = two(e0, e1);
+                            parts(EPI == EPI_DZ ? mul2(a, e) : add2(a, e), v[j], v[j + 1]);
+                        };
+                        if (wide) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = EPI == EPI_DZ ? v[j] * e[j] : v[j] + e[j];
+                            for (int j = 0; j < 8; ++j) {
+                                const uint4 q = irow[j ^ (lane & 7)];
+                                join(4 * j, __uint_as_float(q.x), __uint_as_float(q.y));
+                                join(4 * j + 2, __uint_as_float(q.z), __uint_as_float(q.w));
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint4 q = irow[(j + (c % 2) * 4) ^ (lane & 7)];
+                                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    float e[2];
+                                    unpack2(w[i], p.bf16, e);
+                                    join(8 * j + 2 * i, e[0], e[1]);
+                                }
+                            }
+                        }
+                        __syncwarp();
+                        if (extra_tma && (wide || c % 2 || c + 1 == chunks)) fetch(tile, wide ? c + 1 : c / 2 + 1);
                     }
                     if (EPI == EPI_STORE && p.alpha) {
 #pragma unroll
@@ -395,40 +432,45 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                 }
                 if (EPI == EPI_DL) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float pr = ex2(fmaf(v[j], LOG2E, -vr.lse2));
-                        v[j] = vr.weight == 0.0f ? 0.0f : vr.weight * (pr - (vr.target == p.col0 + col0 + j ? 1.0f : 0.0f));
+                    for (int j = 0; j < 32; j += 2) {
+                        float a, b;
+                        parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-lse2)), a, b);
+                        parts(mul2(two(ex2(a), ex2(b)), both(weight)), v[j], v[j + 1]);
+                    }
+                    if (has_target) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = target == 32 * c + j ? v[j] - weight : v[j];
                     }
                 }
-                if (EPI == EPI_DZ && p.row_sums) {
-                    float t32[32];
+                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
+                // 64 columns of 16 bits fill it (the first 32 wait in registers: the buffer also serves `extra`)
+                const bool narrow = p.y_type != PCB_F32;
+                uint32_t now[16];
+                if (narrow) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) t32[j] = v[j];
-                    const float s = lane_sums(t32);
+                    for (int j = 0; j < 16; ++j) now[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
+                }
+                if (EPI == EPI_DZ && p.row_sums) {
+                    const float s = lane_sums(v);
                     if (col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
                 }
-                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
-                // 64 columns of 16 bits fill it (the first 32 wait in registers: the buffer also turns `extra`)
-                const bool narrow = p.y_type != PCB_F32;
-                if (narrow && c % 2 == 0) {
+                if (narrow && c % 2 == 0 && c + 1 < chunks) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) held[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
-                    if (c + 1 < chunks) continue;
+                    for (int j = 0; j < 16; ++j) held[j] = now[j];
+                    continue;
                 }
                 if (lane == 0) bulk_wait_read();
                 __syncwarp();
                 uint4* srow = (uint4*)(stage + lane * 128);
                 if (narrow) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        srow[j ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
                     if (c % 2) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) held[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
-#pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            srow[(j + 4) ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
+                            srow[j ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        srow[(j + (c % 2) * 4) ^ (lane & 7)] = make_uint4(now[4 * j], now[4 * j + 1], now[4 * j + 2], now[4 * j + 3]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -446,22 +488,8 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                     }
                 } else {
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < p.m; ++r) {
-                        const unsigned char* srcrow = stage + r * 128;
-                        if (narrow) {
-#pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                const int cc = lane + 32 * q;
-                                const uint16_t val = *(const uint16_t*)(srcrow + (((cc / 8) ^ (r & 7)) * 16 + (cc % 8) * 2));
-                                if (box0 + cc < p.n) ((uint16_t*)p.y_ptr)[((int64_t)sp * p.m + row0 + r) * p.y_pitch + box0 + cc] = val;
-                            }
-                        } else {
-                            const float val = *(const float*)(srcrow + (((lane / 4) ^ (r & 7)) * 16 + (lane % 4) * 4));
-                            float* at = (float*)p.y_ptr + ((int64_t)sp * p.m + row0 + r) * p.y_pitch + box0 + lane;
-                            if (box0 + lane < p.n) *at = p.accumulate ? *at + val : val;
-                        }
-                    }
-                    __syncwarp();
+                    const int64_t at = ((int64_t)sp * p.m + row0) * p.y_pitch + box0;
+                    store_block(stage, narrow, (char*)p.y_ptr + at * (narrow ? 2 : 4), p.y_pitch, min(32, p.m - row0), p.n - box0, p.accumulate);
                 }
             }
             if (chunks == 0) release(buf);
@@ -489,9 +517,9 @@ __global__ void __launch_bounds__(256) join(const float* part, int splits, const
         for (int s = 0; s < splits; ++s) v += part[s * total + i];
         const int64_t r = i / p.n, c = i % p.n;
         if (p.bias) v += load(p.bias, c, p.bias_type);
-        float g;
-        if (p.act.kind == PCB_ACT_GELU) v *= normal_cdf(v, &g);
-        else v = act(p.act, v);
+        float skip;
+        if (p.act.kind == PCB_ACT_GELU) parts(act2<PCB_ACT_GELU, false>(p.act, both(v)), v, skip);
+        else if (p.act.kind == PCB_ACT_POLY) parts(act2<PCB_ACT_POLY, false>(p.act, both(v)), v, skip);
         if (p.extra) v += load(p.extra, r * p.extra_pitch + c, p.extra_type);
         store(p.y_ptr, r * p.y_pitch + c, p.y_type, v * alpha);
     }
@@ -586,11 +614,11 @@ Plan plan(int m, int n, int k, bool may_split) {
     return best;
 }
 
-template <int BN, int CTAS, int EPI>
+template <int BN, int CTAS, int EPI, int ACT>
 int launch(const Params& p, cudaStream_t s) {
     using S = Shape<BN, CTAS>;
     static_assert(S::SMEM <= 232448, "shared memory");
-    static const cudaError_t set = cudaFuncSetAttribute(product<BN, CTAS, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+    static const cudaError_t set = cudaFuncSetAttribute(product<BN, CTAS, EPI, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     if (set != cudaSuccess) return (int)set;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits, slots = SMS / CTAS;
     cudaLaunchConfig_t cfg = {};
@@ -606,13 +634,13 @@ int launch(const Params& p, cudaStream_t s) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, product<BN, CTAS, EPI>, p);
+    cudaLaunchKernelEx(&cfg, product<BN, CTAS, EPI, ACT>, p);
     return PCB_LAUNCH_RESULT();
 }
-template <int EPI>
+template <int EPI, int ACT>
 int launch(const Plan& pl, const Params& p, cudaStream_t s) {
-    if (pl.ctas == 2) return pl.bn == 256 ? launch<256, 2, EPI>(p, s) : launch<128, 2, EPI>(p, s);
-    return pl.bn == 128 ? launch<128, 1, EPI>(p, s) : launch<64, 1, EPI>(p, s);
+    if (pl.ctas == 2) return pl.bn == 256 ? launch<256, 2, EPI, ACT>(p, s) : launch<128, 2, EPI, ACT>(p, s);
+    return pl.bn == 128 ? launch<128, 1, EPI, ACT>(p, s) : launch<64, 1, EPI, ACT>(p, s);
 }
 
 }  // namespace
@@ -663,10 +691,12 @@ int gemm(const Gemm& g, cudaStream_t s) {
         p.extra_tma = 1;
     }
     int rc;
-    if (g.epi == EPI_STORE) rc = launch<EPI_STORE>(pl, p, s);
-    else if (g.epi == EPI_DZ) rc = launch<EPI_DZ>(pl, p, s);
-    else if (g.epi == EPI_LSE) rc = launch<EPI_LSE>(pl, p, s);
-    else rc = launch<EPI_DL>(pl, p, s);
+    if (g.epi == EPI_LSE) rc = launch<EPI_LSE, 0>(pl, p, s);
+    else if (g.epi == EPI_DL) rc = launch<EPI_DL, 0>(pl, p, s);
+    else if (g.epi == EPI_DZ) rc = p.act.kind == PCB_ACT_GELU ? launch<EPI_DZ, PCB_ACT_GELU>(pl, p, s) : launch<EPI_DZ, PCB_ACT_POLY>(pl, p, s);
+    else if (p.act.kind == PCB_ACT_GELU) rc = launch<EPI_STORE, PCB_ACT_GELU>(pl, p, s);
+    else if (p.act.kind == PCB_ACT_POLY) rc = launch<EPI_STORE, PCB_ACT_POLY>(pl, p, s);
+    else rc = launch<EPI_STORE, PCB_ACT_NONE>(pl, p, s);
     if (rc || pl.splits == 1) return rc;
     const int64_t blocks = ((int64_t)g.m * g.n + 255) / 256;
     launch_pdl(join, dim3((unsigned)(blocks < 8 * SMS ? blocks : 8 * SMS)), dim3(256), s, (const float*)g.partial, pl.splits, fin);
