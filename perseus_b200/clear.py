@@ -51,56 +51,65 @@ def _act(act):
 
 
 def _is(name, t, like, dims):
-    """t: a CUDA tensor of `like`'s device, 16-bit (or of like's type) with `dims` dimensions."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    """t: a CUDA tensor with `dims` dimensions, 16-bit, or of like's type and device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor, got {t.device if isinstance(t, torch.Tensor) else type(t).__name__}")
     if t.dim() != dims:
         raise ValueError(f"{name}: {dims} dimensions, got shape {tuple(t.shape)}")
     if like is None:
-        if t.dtype not in (torch.bfloat16, torch.float16):
+        if t.dtype is not torch.bfloat16 and t.dtype is not torch.float16:
             raise ValueError(f"{name}: bfloat16 or float16, got {t.dtype}")
-    elif t.dtype != like.dtype or t.device != like.device:
+    elif t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name}: {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
 
 
 def _aside(name, t, like, shape):
     """An optional operand of like's type or float32."""
-    if t.shape != shape or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+    if t.shape != shape or not t.is_cuda or t.get_device() != like.get_device() or \
+            (t.dtype is not like.dtype and t.dtype is not torch.float32):
         raise ValueError(f"{name}: {tuple(shape)} of {like.dtype} or float32 on {like.device}, got {tuple(t.shape)} of "
                          f"{t.dtype} on {t.device}")
 
 
 def _rows(t):
-    """t with adjacent columns and rows that do not overlap (a copy where it is not so)."""
+    """(t, the pitch of its rows) with adjacent columns and rows that do not overlap (a copy where it is not so)."""
     r, c = t.shape
-    if (t.stride(1) == 1 or c == 1) and (t.stride(0) >= c or r == 1):
-        return t
-    return t.contiguous()
-
-
-def _pitch(t):
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    sr, sc = t.stride()
+    if sc != 1 and c != 1 or sr < c and r != 1:
+        return t.contiguous(), c
+    return t, sr if r > 1 else c
 
 
 def _weight(w):
     """(w, its rows' pitch, whether its memory is the transposed matrix)."""
     k, n = w.shape
-    if w.stride(1) == 1 and w.stride(0) >= n:
-        return w, w.stride(0), 0
-    if w.stride(0) == 1 and w.stride(1) >= k:
-        return w, w.stride(1), 1
+    sk, sn = w.stride()
+    if sn == 1 and sk >= n:
+        return w, sk, 0
+    if sk == 1 and sn >= k:
+        return w, sn, 1
     return w.contiguous(), n, 0
 
 
-def _launch(op, args, device):
-    lib = L.lib()
-    with torch.cuda.device(device):
-        need = getattr(lib, f"pcb_clear_{op}_ws")(args)
-        if need < 0:
-            L.check(int(need), f"pcb_clear_{op}")
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        L.check(getattr(lib, f"pcb_clear_{op}")(args, ws.data_ptr() if need else None, need,
-                                                 torch.cuda.current_stream(device).cuda_stream), f"pcb_clear_{op}")
+def _launch(op, args, like):
+    dev = like.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(op, args, like)
+    entry = _ENTRY.get(op)
+    if entry is None:
+        lib = L.lib()
+        entry = _ENTRY[op] = getattr(lib, f"pcb_clear_{op}_ws"), getattr(lib, f"pcb_clear_{op}")
+    need = entry[0](args)
+    if need < 0:
+        L.check(int(need), f"pcb_clear_{op}")
+    ws = like.new_empty(need, dtype=torch.uint8) if need else None  # lives until the launches are queued
+    rc = entry[1](args, None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        L.check(rc, f"pcb_clear_{op}")
+
+
+_ENTRY = {}
 
 
 def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
@@ -109,35 +118,38 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
     `out_dtype`: x's type (default) or float32."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError("linear: x is a CUDA tensor [..., k]")
-    lead = x.shape[:-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
     _is("x", x2, None, 2)
-    _is("w", w, x, 2)
+    _is("w", w, x2, 2)
     m, k = x2.shape
-    n = w.shape[1]
-    if w.shape[0] != k or k < 1:
+    kw, n = w.shape
+    if kw != k or k < 1:
         raise ValueError(f"linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
-    out_dtype = out_dtype or x.dtype
-    if out_dtype not in (x.dtype, torch.float32):
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype is not x.dtype and out_dtype is not torch.float32:
         raise ValueError(f"linear: out_dtype {out_dtype}: {x.dtype} or float32")
     kind, bound, coef = _act(act)
+    t = _TYPE[x.dtype]
+    bias_ptr = res_ptr = None
+    bias_type, res_type, res_pitch = t, t, n
     if bias is not None:
-        _aside("bias", bias, x, (n,))
+        _aside("bias", bias, x2, (n,))
         bias = bias.contiguous()
+        bias_ptr, bias_type = bias.data_ptr(), _TYPE[bias.dtype]
     if residual is not None:
-        _aside("residual", residual, x, lead + (n,))
-        residual = _rows(residual if x.dim() == 2 else residual.reshape(-1, n))
-    x2 = _rows(x2)
-    wm, w_pitch, w_cols = _weight(w)
-    y = torch.empty((m, n), dtype=out_dtype, device=x.device)
+        _aside("residual", residual, x2, (m, n) if flat else x.shape[:-1] + (n,))
+        residual, res_pitch = _rows(residual if flat else residual.reshape(-1, n))
+        res_ptr, res_type = residual.data_ptr(), _TYPE[residual.dtype]
+    x2, x_pitch = _rows(x2)
+    w, w_pitch, w_cols = _weight(w)
+    y = x2.new_empty((m, n)) if out_dtype is x.dtype else x2.new_empty((m, n), dtype=out_dtype)
     if m and n:
-        t = _TYPE[x.dtype]
-        _launch("linear", L.ClearLinear(
-            x2.data_ptr(), wm.data_ptr(), None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), y.data_ptr(), _pitch(x2), w_pitch,
-            n if residual is None else _pitch(residual), n, m, k, n, t, w_cols, t if bias is None else _TYPE[bias.dtype],
-            t if residual is None else _TYPE[residual.dtype], _TYPE[out_dtype], kind, bound, coef), x.device)
-    return y if x.dim() == 2 else y.reshape(lead + (n,))
+        _launch("linear", L.ClearLinear(x2.data_ptr(), w.data_ptr(), bias_ptr, res_ptr, y.data_ptr(), x_pitch, w_pitch,
+                                        res_pitch, n, m, k, n, t, w_cols, bias_type, res_type, _TYPE[out_dtype], kind,
+                                        bound, coef), x2)
+    return y if flat else y.reshape(x.shape[:-1] + (n,))
 
 
 def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
@@ -162,20 +174,21 @@ def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
     if bias is not None:
         _aside("bias", bias, x, (n,))
         bias = bias.contiguous()
-    x2, dy2 = _rows(x2), _rows(dy2)
-    wm, w_pitch, w_cols = _weight(w)
-    dev, t = x.device, _TYPE[x.dtype]
-    dx = torch.empty((m, k), dtype=x.dtype, device=dev) if needs[0] else None
+    x2, x_pitch = _rows(x2)
+    dy2, dy_pitch = _rows(dy2)
+    w, w_pitch, w_cols = _weight(w)
+    t = _TYPE[x.dtype]
+    dx = x2.new_empty((m, k)) if needs[0] else None
     dw = None
     if needs[1]:
-        dw = torch.empty((n, k), dtype=x.dtype, device=dev).t() if w_cols else torch.empty((k, n), dtype=x.dtype, device=dev)
-    db = torch.empty(n, dtype=bias.dtype, device=dev) if needs[2] and bias is not None else None
+        dw = x2.new_empty((n, k)).t() if w_cols else x2.new_empty((k, n))
+    db = bias.new_empty(n) if needs[2] and bias is not None else None
     if dx is not None or dw is not None or db is not None:
         _launch("linear_grad", L.ClearLinearGrad(
-            dy2.data_ptr(), x2.data_ptr(), wm.data_ptr(), None if bias is None else bias.data_ptr(),
+            dy2.data_ptr(), x2.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(),
             None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-            None if db is None else db.data_ptr(), _pitch(dy2), _pitch(x2), w_pitch, k, k if w_cols else n, m, k, n, t,
-            w_cols, t if bias is None else _TYPE[bias.dtype], t if db is None else _TYPE[db.dtype], kind, bound, coef), dev)
+            None if db is None else db.data_ptr(), dy_pitch, x_pitch, w_pitch, k, k if w_cols else n, m, k, n, t, w_cols,
+            t if bias is None else _TYPE[bias.dtype], t if db is None else _TYPE[db.dtype], kind, bound, coef), x2)
     if dx is not None and x.dim() != 2:
         dx = dx.reshape(x.shape)
     return dx, dw, db
@@ -205,16 +218,18 @@ def prompt_attention(q, k, v, q_lens, k_lens=None, scale=None, causal=True, weig
     coef = () if weights is None else tuple(weights)
     if weights is not None and not 1 <= len(coef) <= 8:
         raise ValueError(f"prompt_attention: 1 to 8 coefficients, got {len(coef)}")
-    out = torch.empty((q_rows, heads, dim), dtype=q.dtype, device=q.device)
-    q, k, v = (t if t.stride(2) == 1 or dim == 1 else t.contiguous() for t in (q, k, v))
+    out = q.new_empty((q_rows, heads, dim))
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if dim != 1 and (sq[2] != 1 or sk[2] != 1 or sv[2] != 1):
+        q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
     lens = C.c_int32 * nseq
-    ql, kl = lens(*q_lens), lens(*k_lens)
-    args = L.ClearAttention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.addressof(ql), C.addressof(kl), q.stride(0),
-        q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), heads * dim, dim, q_rows, k_rows, nseq, heads,
-        kv_heads, dim, _TYPE[q.dtype], int(causal), len(coef), 1.0 / math.sqrt(dim) if scale is None else scale,
-        (C.c_float * 8)(*coef))
-    _launch("attention", args, q.device)
+    ql = lens(*q_lens)
+    kl = ql if k_lens is q_lens else lens(*k_lens)
+    _launch("attention", L.ClearAttention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.addressof(ql), C.addressof(kl), sq[0], sq[1], sk[0],
+        sk[1], sv[0], sv[1], heads * dim, dim, q_rows, k_rows, nseq, heads, kv_heads, dim, _TYPE[q.dtype], int(causal),
+        len(coef), 1.0 / math.sqrt(dim) if scale is None else scale, (C.c_float * 8)(*coef) if coef else _NO_COEF), q)
     return out
 
 
@@ -227,22 +242,25 @@ def _vocab_args(who, h, w, targets, lse, loss, ignore):
     if targets.shape != (rows,) or targets.dtype != torch.int64 or targets.device != h.device:
         raise ValueError(f"{who}: targets of shape ({rows},) in int64 on {h.device}, got {tuple(targets.shape)} of "
                          f"{targets.dtype} on {targets.device}")
-    h, w, targets = _rows(h), _rows(w), targets.contiguous()
+    h, h_pitch = _rows(h)
+    w, w_pitch = _rows(w)
+    targets = targets.contiguous()
     args = L.ClearVocab(h.data_ptr(), w.data_ptr(), targets.data_ptr(), None if loss is None else loss.data_ptr(),
-                        lse.data_ptr(), _pitch(h), _pitch(w), ignore, rows, w.shape[0], dim, _TYPE[h.dtype])
-    return args, (h, w, targets)
+                        lse.data_ptr(), h_pitch, w_pitch, ignore, rows, w.shape[0], dim, _TYPE[h.dtype])
+    return args, (h, w, targets)  # the tensors that args points into
 
 
 def vocab_loss(h, w, targets, ignore=-100):
     """Softmax cross entropy of hidden states h [rows, dim] against the vocabulary w [vocab, dim]: (loss, lse), both
     [rows] in float32, lse = log sum_v exp(<h, w_v>), loss = lse - <h, w_target>, 0 where the target is `ignore` (any
     other target outside the vocabulary gives NaN). The logits are never stored whole."""
-    rows = h.shape[0] if isinstance(h, torch.Tensor) and h.dim() == 2 else 0
-    loss = torch.empty(rows, dtype=torch.float32, device=h.device)
-    lse = torch.empty(rows, dtype=torch.float32, device=h.device)
+    _is("h", h, None, 2)
+    rows = h.shape[0]
+    loss = h.new_empty(rows, dtype=torch.float32)
+    lse = h.new_empty(rows, dtype=torch.float32)
     args, keep = _vocab_args("vocab_loss", h, w, targets, lse, loss, ignore)
     if rows:
-        _launch("vocab_loss", args, h.device)
+        _launch("vocab_loss", args, h)
     return loss, lse
 
 
@@ -257,9 +275,9 @@ def vocab_loss_grad(h, w, targets, lse, weight, ignore=-100, needs=(True, True))
             raise ValueError(f"vocab_loss_grad: {name} of shape ({rows},) in float32 on {h.device}")
     lse, weight = lse.contiguous(), weight.contiguous()
     args.lse = lse.data_ptr()
-    dh = torch.empty((rows, dim), dtype=h.dtype, device=h.device) if needs[0] else None
-    dw = torch.empty((w.shape[0], dim), dtype=h.dtype, device=h.device) if needs[1] else None
+    dh = h.new_empty((rows, dim)) if needs[0] else None
+    dw = h.new_empty((w.shape[0], dim)) if needs[1] else None
     if dh is not None or dw is not None:
         _launch("vocab_grad", L.ClearVocabGrad(args, weight.data_ptr(), None if dh is None else dh.data_ptr(),
-                                               None if dw is None else dw.data_ptr(), dim, dim), h.device)
+                                               None if dw is None else dw.data_ptr(), dim, dim), h)
     return dh, dw

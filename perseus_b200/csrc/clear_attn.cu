@@ -36,7 +36,7 @@ namespace {
 
 constexpr int SMS = 148;
 constexpr int ROWS = 128, KEYS = 128;
-constexpr int SEQS = 512;  // sequences of one launch
+constexpr int SEQS = 128;  // sequences of one launch
 
 struct Work {
     int32_t n;
