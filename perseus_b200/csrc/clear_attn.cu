@@ -6,8 +6,8 @@
 // into weights, which go back to TMEM in 16 bits as the left operand of O += P V. Softmax runs with a running maximum and
 // sum: O is rescaled only when a row's maximum grew by more than 2^8 (weights stay below 2^8, in range for f16), which
 // after the first blocks is rare. Under polynomial weights there is no maximum, no sum and no rescaling.
-// Two blocks share an SM: while one's warps compute weights, the other's products run. Heads of up to 64 keep P apart from
-// S, so that the next scores are formed while this block's O accumulates.
+// Two blocks share an SM: while one's warps compute weights, the other's products run. The keys of a block go in two steps
+// of 64 through two score buffers, so that a step's scores are there when the step before it is done.
 //
 // Few rows against many keys (single tokens) split the keys over several blocks, joined in order by `join_splits`.
 //
@@ -35,7 +35,7 @@ __device__ unsigned int g_attn_timeouts;
 namespace {
 
 constexpr int SMS = 148;
-constexpr int ROWS = 128, KEYS = 128;
+constexpr int ROWS = 128, KEYS = 128, STEP = 64;  // rows of a tile, keys of a copy, keys of a product
 constexpr int SEQS = 128;  // sequences of one launch
 
 struct Work {
@@ -58,15 +58,15 @@ struct alignas(64) Params {
     Work w;
 };
 
+// TMEM columns of a block: two buffers of 64 keys' scores, each turned into weights in place (16 bits: its first 32
+// columns), and the sums O
 template <int DP>
 struct Shape {
     static constexpr int HALF = 128 * 128;               // 128 rows of 64 values
     static constexpr int OPERAND = HALF * (DP / 64);     // 128 rows of DP
     static constexpr int RING = DP == 64 ? 4 : 2;        // K and V blocks in flight
-    static constexpr uint32_t S = 0, P = DP == 64 ? 128 : 0, O = DP == 64 ? 192 : 128;  // TMEM columns
-    static constexpr uint32_t TMEM = 256;
+    static constexpr uint32_t S = 0, O = 2 * STEP, TMEM = 256;
     static constexpr size_t SMEM = 1024 + OPERAND * (1 + RING) + 256;
-    static constexpr bool APART = P != S;
 };
 constexpr int THREADS = 192;
 
@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     uint64_t* full = q_full + 1;
     uint64_t* empty = full + S::RING;
     uint64_t* s_full = empty + S::RING;
-    uint64_t* p_ready = s_full + 1;
-    uint64_t* pv_done = p_ready + 1;
-    uint64_t* drain = pv_done + 1;
+    uint64_t* p_ready = s_full + 2;
+    uint64_t* pv_done = p_ready + 2;
+    uint64_t* drain = pv_done + 2;
     uint32_t* tmem_at = (uint32_t*)(drain + 1);
     volatile int* dead = (volatile int*)(tmem_at + 1);
     const int warp = warp_index(), lane = threadIdx.x % 32;
@@ -136,9 +136,11 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        mbar_init(s_full, 1);
-        mbar_init(p_ready, 4);
-        mbar_init(pv_done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_ready[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
         mbar_init(drain, 1);
         mbar_init_fence();
         *dead = 0;
@@ -170,6 +172,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     const int least = p.a.causal ? min(nk, max(0, t0 + past + 1)) : nk;               // and of the first
     const int blocks = (seen + KEYS - 1) / KEYS, per = (blocks + p.splits - 1) / p.splits;
     const int b0 = min(blocks, split * per), n = min(blocks, b0 + per) - b0;
+    const int steps = n > 0 ? (min(seen, (b0 + n) * KEYS) - b0 * KEYS + STEP - 1) / STEP : 0;  // products of 64 keys
 
     if (warp == 0) {
         if (n > 0) {
@@ -201,53 +204,51 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         if (n > 0) {
             const bool bf16 = p.a.type == PCB_BF16;
             const int ksteps = (p.a.dim + 15) / 16, nd = (p.a.dim + 15) / 16 * 16;
-            const uint32_t is = instr_desc(bf16, false, false, ROWS, KEYS) | (p.negate ? 1u << 13 : 0u);
+            const uint32_t is = instr_desc(bf16, false, false, ROWS, STEP) | (p.negate ? 1u << 13 : 0u);
             const uint32_t ipv = instr_desc(bf16, false, true, ROWS, nd);
             const uint64_t dq = smem_desc(smem_addr(base), 16, 1024);
             const uint64_t dk0 = smem_desc(smem_addr(ring), 16, 1024), dv0 = smem_desc(smem_addr(ring), S::HALF, 1024);
-            Ring<S::RING> rg;
+            constexpr uint32_t NEXT = S::OPERAND >> 4;
+            Ring<S::RING> rk, rv;  // the K and the V block in use
+            rv.next();
             bool ok = wait_warp(q_full, 0, dead, &g_attn_timeouts);
-            auto scores = [&](uint64_t dk, int st) {  // S = Q K^T
+            auto scores = [&](int i) {  // S[i % 2] = Q K^T over the 64 keys of step i
+                if (i % 2 == 0) ok = ok && wait_warp(&full[rk.stage], rk.phase, dead, &g_attn_timeouts);
+                if (!ok) return;
                 fence_after();
+                const uint64_t dk = dk0 + rk.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
                 if (elect()) {
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s) {
                         const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
-                        if (s < ksteps) mma_ss(tmem + S::S, dq + off, dk + off, is, s > 0);
+                        if (s < ksteps) mma_ss(tmem + S::S + i % 2 * STEP, dq + off, dk + off, is, s > 0);
                     }
-                    mma_commit(s_full);
-                    mma_commit(&empty[st]);
+                    mma_commit(&s_full[i % 2]);
+                    if (i % 2 || i + 1 == steps) mma_commit(&empty[rk.stage]);
                 }
                 __syncwarp();
+                if (i % 2) rk.next(), rk.next();
             };
-            auto next_scores = [&]() {  // waits for the next K block in the ring and forms its scores
-                ok = wait_warp(&full[rg.stage], rg.phase, dead, &g_attn_timeouts);
-                if (ok) scores(dk0 + (uint32_t)(rg.stage * (S::OPERAND >> 4)), rg.stage);
-                rg.next();
-            };
-            if (ok) next_scores();
-            for (int j = 0; j < n && ok; ++j) {
-                const Ring<S::RING> rv = rg;  // this block's V; the next K after it
-                rg.next();
-                ok = wait_warp(p_ready, j & 1, dead, &g_attn_timeouts);
+            scores(0);
+            if (steps > 1) scores(1);
+            for (int i = 0; i < steps && ok; ++i) {
+                ok = wait_warp(&p_ready[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
+                if (i % 2 == 0) ok = ok && wait_warp(&full[rv.stage], rv.phase, dead, &g_attn_timeouts);
                 if (!ok) break;
                 fence_after();
-                if (S::APART && j + 1 < n) next_scores();
-                ok = ok && wait_warp(&full[rv.stage], rv.phase, dead, &g_attn_timeouts);
-                if (!ok) break;
-                fence_after();
-                const uint64_t dv = dv0 + (uint32_t)(rv.stage * (S::OPERAND >> 4));
+                const uint64_t dv = dv0 + rv.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
                 if (elect()) {
 #pragma unroll
-                    for (int s = 0; s < KEYS / 16; ++s)
-                        mma_ts(tmem + S::O, tmem + S::P + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, j > 0 || s > 0);
-                    mma_commit(pv_done);
-                    mma_commit(&empty[rv.stage]);
+                    for (int s = 0; s < STEP / 16; ++s)
+                        mma_ts(tmem + S::O, tmem + S::S + i % 2 * STEP + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, i > 0 || s > 0);
+                    mma_commit(&pv_done[i % 2]);
+                    if (i % 2 || i + 1 == steps) mma_commit(&empty[rv.stage]);
                 }
                 __syncwarp();
-                if (!S::APART && j + 1 < n) {  // the next scores take P's place
-                    ok = wait_warp(pv_done, j & 1, dead, &g_attn_timeouts);
-                    if (ok) next_scores();
+                if (i % 2) rv.next(), rv.next();
+                if (i + 2 < steps) {  // scores in place of the weights just used
+                    ok = wait_warp(&pv_done[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
+                    scores(i + 2);
                 }
             }
             if (!ok) {  // the products in flight
@@ -264,80 +265,83 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         const bool bf16 = p.a.type == PCB_BF16;
         float top = -INFINITY, sum = 0.0f;
         bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            ok = wait_warp(s_full, j & 1, dead, &g_attn_timeouts);
+        for (int i = 0; i < steps; ++i) {
+            ok = wait_warp(&s_full[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
             if (!ok) break;
             fence_after();
-            float s[KEYS];
-#pragma unroll
-            for (int h = 0; h < 4; ++h) tmem_ld32(tmem + S::S + lanes + 32 * h, s + 32 * h);
+            const uint32_t at_s = tmem + S::S + i % 2 * STEP + lanes;
+            float s[STEP];
+            tmem_ld32(at_s, s);
+            tmem_ld32(at_s + 32, s + 32);
             ld_wait();
-            const int at = (b0 + j) * KEYS, left = limit - at;
-            const bool masked = at + KEYS > least;
+            const int at = b0 * KEYS + i * STEP, left = limit - at;
+            const bool masked = at + STEP > least;
+            uint32_t w[STEP / 2];
             if (POLY) {
 #pragma unroll
-                for (int i = 0; i < KEYS; ++i) {
-                    float v = p.coef[7];
+                for (int j = 0; j < STEP; j += 2) {
+                    const f32x2 x = two(s[j], s[j + 1]);
+                    f32x2 r = both(p.coef[7]);
 #pragma unroll
-                    for (int e = 6; e >= 0; --e) v = fmaf(v, s[i], p.coef[e]);
-                    s[i] = v;
+                    for (int e = 6; e >= 0; --e) r = fma2(r, x, both(p.coef[e]));
+                    parts(r, s[j], s[j + 1]);
                 }
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) s[i] = i < left ? s[i] : 0.0f;
+                    for (int j = 0; j < STEP; ++j) s[j] = j < left ? s[j] : 0.0f;
                 }
-                if (j > 0) ok = wait_warp(pv_done, (j - 1) & 1, dead, &g_attn_timeouts);
-                if (!ok) break;
             } else {
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                    for (int j = 0; j < STEP; ++j) s[j] = j < left ? s[j] : -INFINITY;
                 }
                 float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < KEYS; ++i) m4[i % 4] = fmaxf(m4[i % 4], s[i]);
+                for (int j = 4; j < STEP; ++j) m4[j % 4] = fmaxf(m4[j % 4], s[j]);
                 const float big = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.c);
                 const bool grew = big > top + 8.0f;
-                if (j > 0) ok = wait_warp(pv_done, (j - 1) & 1, dead, &g_attn_timeouts);
-                if (!ok) break;
                 if (__any_sync(~0u, grew)) {
                     const float f = grew ? ex2(top - big) : 1.0f;
-                    if (j > 0) {
+                    if (i > 0) {
+                        ok = wait_warp(&pv_done[(i - 1) % 2], (i - 1) / 2 & 1, dead, &g_attn_timeouts);
+                        if (!ok) break;
                         fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int h = 0; h < DP / 32; ++h) {
                             float o[32];
                             tmem_ld32(tmem + S::O + lanes + 32 * h, o);
                             ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= f;
+                            for (int j = 0; j < 32; ++j) o[j] *= f;
                             tmem_st32(tmem + S::O + lanes + 32 * h, (uint32_t*)o);
                         }
                     }
                     sum *= f;
                     if (grew) top = big;
                 }
-                const float sub = top == -INFINITY ? 0.0f : -top;
-                float s4[4] = {};
+                const f32x2 c = both(p.c), sub = both(top == -INFINITY ? 0.0f : -top);
+                f32x2 s2[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < KEYS; ++i) {
-                    s[i] = ex2(fmaf(s[i], p.c, sub));
-                    s4[i % 4] += s[i];
+                for (int j = 0; j < STEP; j += 2) {
+                    float x0, x1;
+                    parts(fma2(two(s[j], s[j + 1]), c, sub), x0, x1);
+                    s[j] = ex2(x0), s[j + 1] = ex2(x1);
+                    s2[j / 2 % 2] = add2(s2[j / 2 % 2], two(s[j], s[j + 1]));
                 }
-                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                float x0, x1;
+                parts(add2(s2[0], s2[1]), x0, x1);
+                sum += x0 + x1;
             }
             // the weights in 16 bits (their one rounding: the products with V take 16-bit operands), two per column
-            uint32_t* w = (uint32_t*)s;
 #pragma unroll
-            for (int i = 0; i < KEYS / 2; ++i) w[i] = pack2(s[2 * i], s[2 * i + 1], bf16);
-            tmem_st32(tmem + S::P + lanes, w);
-            tmem_st32(tmem + S::P + lanes + 32, w + 32);
+            for (int j = 0; j < STEP / 2; ++j) w[j] = pack2(s[2 * j], s[2 * j + 1], bf16);
+            tmem_st32(at_s, w);
             st_wait();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready);
+            if (lane == 0) mbar_arrive(&p_ready[i % 2]);
         }
-        if (ok && n > 0) ok = wait_warp(pv_done, (n - 1) & 1, dead, &g_attn_timeouts);
+        if (ok && steps > 0) ok = wait_warp(&pv_done[(steps - 1) % 2], (steps - 1) / 2 & 1, dead, &g_attn_timeouts);
         fence_after();
         if (ok) {
             const int64_t qrow = q0 + tok;
