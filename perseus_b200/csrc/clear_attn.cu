@@ -16,8 +16,6 @@
 // the keys that they see (`attend_row`): exact semantics at no cost where all values are finite.
 #include <algorithm>
 #include <cstring>
-#include <numeric>
-#include <vector>
 
 #include "clear_gemm.h"
 #include "mma.cuh"
@@ -68,7 +66,7 @@ struct Shape {
     static constexpr uint32_t S = 0, O = 2 * STEP, TMEM = 256;
     static constexpr size_t SMEM = 1024 + OPERAND * (1 + RING) + 256;
 };
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;  // loads, scores, sums, and four warps with a row per thread
 
 // ------------------------------------------------------------------------------------------------ one row, key by key
 // A warp computes out = sum of weights x values over keys [j0, j1) of one query in 32 bits: lane l holds dims l + 32 t.
@@ -112,6 +110,30 @@ __device__ __noinline__ void attend_row(const PcbClearAttention& a, int64_t qrow
     *sum_out = sum;
 }
 
+// 2^x for two values on the multiply-add pipe: the special-function pipe gives 16 exponentials per cycle and SM, half of what
+// the products need at 64 dims, so a quarter of them is computed here (8192 tokens, 12 heads over 4: 164 us without, 156 with
+// a quarter, 166 with half; at 128 dims the products take as long as the exponentials, and it costs 1 %). x = n + f with n the nearest integer (in the low bits of
+// x + 1.5 2^23), |f| <= 1/2; 2^f by the polynomial of least relative error of degree 4 (2.6e-6, a thousandth of the weights'
+// rounding), 2^n added to its exponent. Below -126 it stays at 2^-126, which a masked key then weighs
+// against at least 2^-8 (a row that sees nothing is told by its limit); NaN gives a value that is not finite in 16 bits.
+__device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
+    float x0, x1, t0, t1, p0, p1;
+    parts(x, x0, x1);
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x0) : "f"(x0));  // -126
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x1) : "f"(x1));
+    x = two(x0, x1);
+    const f32x2 t = add2(x, both(12582912.0f));
+    const f32x2 f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), x);
+    f32x2 p = fma2(f, both(0.009570102207362652f), both(0.05591785907745361f));
+    p = fma2(p, f, both(0.240247443318367f));
+    p = fma2(p, f, both(0.6931217908859253f));
+    p = fma2(p, f, both(0.9999992847442627f));
+    parts(t, t0, t1);
+    parts(p, p0, p1);
+    return two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
+               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+}
+
 // ------------------------------------------------------------------------------------------------ the kernel
 template <int DP, bool POLY>
 __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Params p) {
@@ -126,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     uint64_t* p_ready = s_full + 2;
     uint64_t* pv_done = p_ready + 2;
     uint64_t* drain = pv_done + 2;
-    uint32_t* tmem_at = (uint32_t*)(drain + 1);
+    uint32_t* tmem_at = (uint32_t*)(drain + 2);
     volatile int* dead = (volatile int*)(tmem_at + 1);
     const int warp = warp_index(), lane = threadIdx.x % 32;
 
@@ -141,7 +163,8 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
             mbar_init(&p_ready[i], 4);
             mbar_init(&pv_done[i], 1);
         }
-        mbar_init(drain, 1);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
         mbar_init_fence();
         *dead = 0;
         prefetch_map(&p.q);
@@ -200,60 +223,67 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                 for (int f = max(0, i - S::RING); f < i; ++f) mbar_wait(&full[f % S::RING], (f / S::RING) & 1);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp <= 2) {
+        // Two warps issue the products, one the scores and one the sums: each of these loops costs its warp some 500 cycles
+        // a step in waits and issue, and both in one warp (1530 cycles) kept everything else waiting.
         if (n > 0) {
             const bool bf16 = p.a.type == PCB_BF16;
             const int ksteps = (p.a.dim + 15) / 16, nd = (p.a.dim + 15) / 16 * 16;
-            const uint32_t is = instr_desc(bf16, false, false, ROWS, STEP) | (p.negate ? 1u << 13 : 0u);
-            const uint32_t ipv = instr_desc(bf16, false, true, ROWS, nd);
-            const uint64_t dq = smem_desc(smem_addr(base), 16, 1024);
-            const uint64_t dk0 = smem_desc(smem_addr(ring), 16, 1024), dv0 = smem_desc(smem_addr(ring), S::HALF, 1024);
             constexpr uint32_t NEXT = S::OPERAND >> 4;
-            Ring<S::RING> rk, rv;  // the K and the V block in use
-            rv.next();
-            bool ok = wait_warp(q_full, 0, dead, &g_attn_timeouts);
-            auto scores = [&](int i) {  // S[i % 2] = Q K^T over the 64 keys of step i
-                if (i % 2 == 0) ok = ok && wait_warp(&full[rk.stage], rk.phase, dead, &g_attn_timeouts);
-                if (!ok) return;
-                fence_after();
-                const uint64_t dk = dk0 + rk.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
-                if (elect()) {
+            Ring<S::RING> rg;  // the K (or V) block in use: every other one of the ring
+            bool ok = true, ready = false;
+            if (warp == 1) {  // S[i % 2] = Q K^T over the 64 keys of step i, in place of weights already used
+                const uint32_t is = instr_desc(bf16, false, false, ROWS, STEP) | (p.negate ? 1u << 13 : 0u);
+                const uint64_t dq = smem_desc(smem_addr(base), 16, 1024), dk0 = smem_desc(smem_addr(ring), 16, 1024);
+                ok = wait_warp(q_full, 0, dead, &g_attn_timeouts);
+                for (int i = 0; i < steps && ok; ++i) {
+                    if (i % 2 == 0 && !__all_sync(~0u, ready)) ok = wait_warp(&full[rg.stage], rg.phase, dead, &g_attn_timeouts);
+                    if (i >= 2) ok = ok && wait_warp(&pv_done[i % 2], (i - 2) / 2 & 1, dead, &g_attn_timeouts);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t dk = dk0 + rg.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
+                    if (elect()) {
 #pragma unroll
-                    for (int s = 0; s < DP / 16; ++s) {
-                        const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
-                        if (s < ksteps) mma_ss(tmem + S::S + i % 2 * STEP, dq + off, dk + off, is, s > 0);
+                        for (int s = 0; s < DP / 16; ++s) {
+                            const uint32_t off = ((s / 4) * S::HALF + (s % 4) * 32) >> 4;
+                            if (s < ksteps) mma_ss(tmem + S::S + i % 2 * STEP, dq + off, dk + off, is, s > 0);
+                        }
+                        mma_commit(&s_full[i % 2]);
+                        if (i % 2 || i + 1 == steps) mma_commit(&empty[rg.stage]);
                     }
-                    mma_commit(&s_full[i % 2]);
-                    if (i % 2 || i + 1 == steps) mma_commit(&empty[rk.stage]);
+                    __syncwarp();
+                    if (i % 2) {
+                        rg.next(), rg.next();
+                        ready = peek(&full[rg.stage], rg.phase);
+                    }
                 }
-                __syncwarp();
-                if (i % 2) rk.next(), rk.next();
-            };
-            scores(0);
-            if (steps > 1) scores(1);
-            for (int i = 0; i < steps && ok; ++i) {
-                ok = wait_warp(&p_ready[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
-                if (i % 2 == 0) ok = ok && wait_warp(&full[rv.stage], rv.phase, dead, &g_attn_timeouts);
-                if (!ok) break;
-                fence_after();
-                const uint64_t dv = dv0 + rv.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
-                if (elect()) {
+            } else {  // O += P[i % 2] V
+                const uint32_t ipv = instr_desc(bf16, false, true, ROWS, nd);
+                const uint64_t dv0 = smem_desc(smem_addr(ring), S::HALF, 1024);
+                rg.next();
+                for (int i = 0; i < steps && ok; ++i) {
+                    if (i % 2 == 0 && !__all_sync(~0u, ready)) ok = wait_warp(&full[rg.stage], rg.phase, dead, &g_attn_timeouts);
+                    ok = ok && wait_warp(&p_ready[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t dv = dv0 + rg.stage * NEXT + (uint32_t)(i % 2 * (STEP * 128) >> 4);
+                    if (elect()) {
 #pragma unroll
-                    for (int s = 0; s < STEP / 16; ++s)
-                        mma_ts(tmem + S::O, tmem + S::S + i % 2 * STEP + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, i > 0 || s > 0);
-                    mma_commit(&pv_done[i % 2]);
-                    if (i % 2 || i + 1 == steps) mma_commit(&empty[rv.stage]);
-                }
-                __syncwarp();
-                if (i % 2) rv.next(), rv.next();
-                if (i + 2 < steps) {  // scores in place of the weights just used
-                    ok = wait_warp(&pv_done[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
-                    scores(i + 2);
+                        for (int s = 0; s < STEP / 16; ++s)
+                            mma_ts(tmem + S::O, tmem + S::S + i % 2 * STEP + 8 * s, dv + (uint32_t)(s * 2048 >> 4), ipv, i > 0 || s > 0);
+                        mma_commit(&pv_done[i % 2]);
+                        if (i % 2 || i + 1 == steps) mma_commit(&empty[rg.stage]);
+                    }
+                    __syncwarp();
+                    if (i % 2) {
+                        rg.next(), rg.next();
+                        ready = peek(&full[rg.stage], rg.phase);
+                    }
                 }
             }
             if (!ok) {  // the products in flight
-                if (elect()) mma_commit(drain);
-                mbar_wait(drain, 0);
+                if (elect()) mma_commit(&drain[warp - 1]);
+                mbar_wait(&drain[warp - 1], 0);
             }
         }
     } else {
@@ -265,8 +295,9 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         const bool bf16 = p.a.type == PCB_BF16;
         float top = -INFINITY, sum = 0.0f;
         bool ok = true;
+        bool ready = false;
         for (int i = 0; i < steps; ++i) {
-            ok = wait_warp(&s_full[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
+            if (!__all_sync(~0u, ready)) ok = wait_warp(&s_full[i % 2], i / 2 & 1, dead, &g_attn_timeouts);
             if (!ok) break;
             fence_after();
             const uint32_t at_s = tmem + S::S + i % 2 * STEP + lanes;
@@ -276,7 +307,13 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
             ld_wait();
             const int at = b0 * KEYS + i * STEP, left = limit - at;
             const bool masked = at + STEP > least;
-            uint32_t w[STEP / 2];
+            // 32 weights in 16 bits (their one rounding: the products with V take 16-bit operands), two per column
+            auto put = [&](int h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = pack2(s[32 * h + 2 * j], s[32 * h + 2 * j + 1], bf16);
+                tmem_st16(at_s + 16 * h, w);
+            };
             if (POLY) {
 #pragma unroll
                 for (int j = 0; j < STEP; j += 2) {
@@ -297,7 +334,11 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                 }
                 float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 4; j < STEP; ++j) m4[j % 4] = fmaxf(m4[j % 4], s[j]);
+                for (int j = 4; j + 7 < STEP; j += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m4[e] = fmaxf(fmaxf(m4[e], s[j + e]), s[j + 4 + e]);
+#pragma unroll
+                for (int j = STEP - 4; j < STEP; ++j) m4[j % 4] = fmaxf(m4[j % 4], s[j]);
                 const float big = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.c);
                 const bool grew = big > top + 8.0f;
                 if (__any_sync(~0u, grew)) {
@@ -307,13 +348,13 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                         if (!ok) break;
                         fence_after();
 #pragma unroll 1
-                        for (int h = 0; h < DP / 32; ++h) {
-                            float o[32];
-                            tmem_ld32(tmem + S::O + lanes + 32 * h, o);
+                        for (int h = 0; h < DP / 16; ++h) {
+                            float o[16];
+                            tmem_ld16(tmem + S::O + lanes + 16 * h, o);
                             ld_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= f;
-                            tmem_st32(tmem + S::O + lanes + 32 * h, (uint32_t*)o);
+                            for (int j = 0; j < 16; ++j) o[j] *= f;
+                            tmem_st16(tmem + S::O + lanes + 16 * h, (uint32_t*)o);
                         }
                     }
                     sum *= f;
@@ -322,20 +363,29 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                 const f32x2 c = both(p.c), sub = both(top == -INFINITY ? 0.0f : -top);
                 f32x2 s2[2] = {0, 0};
 #pragma unroll
-                for (int j = 0; j < STEP; j += 2) {
-                    float x0, x1;
-                    parts(fma2(two(s[j], s[j + 1]), c, sub), x0, x1);
-                    s[j] = ex2(x0), s[j + 1] = ex2(x1);
-                    s2[j / 2 % 2] = add2(s2[j / 2 % 2], two(s[j], s[j + 1]));
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 32 * h; j < 32 * h + 32; j += 2) {
+                        const f32x2 x = fma2(two(s[j], s[j + 1]), c, sub);
+                        f32x2 e;
+                        if (DP == 64 && j / 2 % 4 == 3) {
+                            e = exp2_fma(x);
+                        } else {
+                            float x0, x1;
+                            parts(x, x0, x1);
+                            e = two(ex2(x0), ex2(x1));
+                        }
+                        parts(e, s[j], s[j + 1]);
+                        s2[j / 2 % 2] = add2(s2[j / 2 % 2], e);
+                    }
+                    put(h);
                 }
                 float x0, x1;
                 parts(add2(s2[0], s2[1]), x0, x1);
                 sum += x0 + x1;
             }
-            // the weights in 16 bits (their one rounding: the products with V take 16-bit operands), two per column
-#pragma unroll
-            for (int j = 0; j < STEP / 2; ++j) w[j] = pack2(s[2 * j], s[2 * j + 1], bf16);
-            tmem_st32(at_s, w);
+            if (POLY) put(0), put(1);
+            ready = i + 1 < steps && peek(&s_full[(i + 1) % 2], (i + 1) / 2 & 1);
             st_wait();
             fence_before();
             __syncwarp();
@@ -345,7 +395,8 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         fence_after();
         if (ok) {
             const int64_t qrow = q0 + tok;
-            const float scale = POLY ? p.out_scale : p.splits > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
+            const bool blind = limit <= b0 * KEYS;  // sees none of these keys
+            const float scale = POLY ? p.out_scale : blind ? 0.0f : p.splits > 1 ? 1.0f : 1.0f / sum;
             const int64_t prow = ((int64_t)split * p.a.q_rows + qrow) * p.a.heads + head;
             const int64_t orow = qrow * p.a.out_pitch + head * p.a.out_head;
             bool odd = !(fabsf(sum) <= 3.4e38f);
@@ -378,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                         if (32 * h + i < p.a.dim) store(p.a.out, orow + 32 * h + i, p.a.type, o[i]);
                 }
             }
-            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(top, sum);
+            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(blind ? -INFINITY : top, blind ? 0.0f : sum);
             for (uint32_t again = __ballot_sync(~0u, mine && odd); again; again &= again - 1) {
                 const int src = __ffs(again) - 1;
                 const int tk = __shfl_sync(~0u, tok, src), hd = __shfl_sync(~0u, head, src), lim = __shfl_sync(~0u, limit, src);
