@@ -1,6 +1,8 @@
 // The clear half's operators on the product of clear_gemm.cu (include/pcb200.h section 4): linear, its gradients, and the
 // vocabulary loss with its gradients.
+#include <algorithm>
 #include <cstring>
+#include <utility>
 
 #include "clear_gemm.h"
 
@@ -105,23 +107,42 @@ __global__ void __launch_bounds__(1024) prepare_rows(PcbClearVocab a, const floa
     rows[i] = VocabRow{a.lse[i] * 1.4426950408889634f, t == a.ignore ? 0.0f : ldexpf(weight[i], e),
                        t >= 0 && t < a.vocab ? (int32_t)t : -1, 0};
 }
-// y = x * factor, rounded
-__global__ void __launch_bounds__(256) finish(const float* x, int64_t rows, int64_t cols, const float* factor, void* y, int64_t pitch,
-                                              int type) {
+// y = factor * (the sum of `slices` matrices x of pitch `from`, in order), rounded
+__global__ void __launch_bounds__(256) finish(const float* x, int slices, int64_t rows, int cols, int64_t from, const float* factor, void* y,
+                                              int64_t pitch, int type) {
     pdl_wait();
     pdl_release();
     const float f = *factor;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256)
-        store(y, i / cols * pitch + i % cols, type, x[i] * f);
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < cols; c += 256) {
+            float s = x[r * from + c];
+            for (int i = 1; i < slices; ++i) s += x[(i * rows + r) * from + c];
+            store(y, r * pitch + c, type, s * f);
+        }
 }
 
-// Columns of one piece of the vocabulary: the piece's slopes (16 bits) take at most 96 MiB, so that the two products that
-// read them find them in L2; pieces alike, in multiples of 256
-int piece(int rows, int vocab) {
-    const int64_t fit = (96ll << 20) / 2 / (rows > 0 ? rows : 1);
-    const int64_t most = fit < 256 ? 256 : fit / 256 * 256;
-    const int64_t pieces = (vocab + most - 1) / most;
-    return (int)(((vocab + pieces - 1) / pieces + 255) / 256 * 256);
+// The pieces of the vocabulary: at most 96 MiB of slopes (16 bits) each, so that the two products that read them find them in
+// L2, and of the widths that fit, alike but for the last and multiples of 256, the one whose three products fill the SMs best
+// (rows x columns, columns x dim, and rows x dim with k in `slices` parts).
+struct Pieces {
+    int cols, slices;
+};
+Pieces pieces_of(int rows, int vocab, int dim, bool dh, bool dw) {
+    const int64_t fit = (96ll << 20) / 2 / rows;
+    const int64_t most = fit < 256 ? 256 : fit / 256 * 256, least = (vocab + most - 1) / most;
+    Pieces best{(int)most, 1};
+    double ns = 1e300;
+    for (int64_t n = least; n <= least + 6; ++n) {
+        const int cols = (int)(((vocab + n - 1) / n + 255) / 256 * 256);
+        const int full = vocab / cols, rest = vocab % cols, slices = gemm_slices(rows, dim, cols);
+        double t = 0.0;
+        for (const auto& [count, width] : {std::pair<int, int>{full, cols}, {1, rest}})
+            if (count && width)
+                t += count * (gemm_cost(rows, width, dim, false) + (dw ? gemm_cost(width, dim, rows, true) : 0.0) +
+                              (dh ? gemm_cost(rows, dim, (width + slices - 1) / slices, false) * 1.0 : 0.0) + 6000.0);
+        if (t < ns) ns = t, best = Pieces{cols, slices};
+    }
+    return best;
 }
 
 }  // namespace clear
@@ -177,8 +198,8 @@ struct VocabWs {
     float2* parts;
     float *hit, *unscale, *dh, *partial;
     VocabRow* rows;
-    int piece;
-    int64_t slope_pitch;
+    int piece, slices;
+    int64_t slope_pitch, dh_pitch;
 };
 VocabWs loss_ws(const PcbClearVocab* a, void* ws) {
     Carve c(ws);
@@ -196,12 +217,15 @@ VocabWs vgrad_ws(const PcbClearVocabGrad* a, void* ws) {
     VocabWs r{};
     r.h = c.take<char>(aligned_bytes(v.h, v.h_pitch, v.rows, v.dim));
     r.w = c.take<char>(aligned_bytes(v.w, v.w_pitch, v.vocab, v.dim));
-    r.piece = piece(v.rows, v.vocab);
+    const Pieces pc = pieces_of(v.rows, v.vocab, v.dim, a->dh, a->dw);
+    r.piece = pc.cols;
+    r.slices = pc.slices;
     r.slope_pitch = r.piece;
+    r.dh_pitch = (v.dim + 3) / 4 * 4;
     r.slopes = c.take<uint16_t>((size_t)v.rows * r.slope_pitch);
     r.rows = c.take<VocabRow>(v.rows);
     r.unscale = c.take<float>(1);
-    r.dh = c.take<float>(a->dh && r.piece < v.vocab ? (size_t)v.rows * v.dim : 0);
+    r.dh = c.take<float>(a->dh && r.piece < v.vocab ? (size_t)r.slices * v.rows * r.dh_pitch : 0);
     size_t part = 0;
     for (int v0 = 0; v0 < v.vocab; v0 += r.piece) {
         const int cols = v.vocab - v0 < r.piece ? v.vocab - v0 : r.piece;
@@ -235,8 +259,8 @@ int pcb_clear_linear(const PcbClearLinear* a, void* ws, size_t ws_bytes, cudaStr
     const LinearWs w = linear_ws(a, ws);
     if (int rc = bad_ws("clear_linear", ws, ws_bytes, w.bytes)) return rc;
     Operand x{a->x, a->x_pitch, true}, wt{a->w, a->w_pitch, a->w_cols != 0};
-    if (int rc = align_rows(&x.p, &x.pitch, a->m, a->k, w.x, s)) return rc;
-    if (int rc = align_rows(&wt.p, &wt.pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n, w.w, s)) return rc;
+    const Rows rows[] = {{&x.p, &x.pitch, a->m, a->k, w.x}, {&wt.p, &wt.pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n, w.w}};
+    if (int rc = align_rows(rows, 2, s)) return rc;
     Gemm g = product_of(x, wt, a->m, a->n, a->k, a->type);
     g.y = a->y, g.y_pitch = a->y_pitch, g.y_type = a->y_type;
     g.act = make_act(a->act, a->bound, a->coef);
@@ -260,10 +284,12 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
     const GradWs w = grad_ws(a, ws);
     if (int rc = bad_ws("clear_linear_grad", ws, ws_bytes, w.bytes)) return rc;
     Operand x{a->x, a->x_pitch, true}, wt{a->w, a->w_pitch, a->w_cols != 0}, dz{a->dy, a->dy_pitch, true};
-    if (a->dw || a->act)
-        if (int rc = align_rows(&x.p, &x.pitch, a->m, a->k, w.x, s)) return rc;
-    if (a->dx || a->act)
-        if (int rc = align_rows(&wt.p, &wt.pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n, w.w, s)) return rc;
+    Rows rows[3];
+    int nrows = 0;
+    if (a->dw || a->act) rows[nrows++] = Rows{&x.p, &x.pitch, a->m, a->k, w.x};
+    if (a->dx || a->act) rows[nrows++] = Rows{&wt.p, &wt.pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n, w.w};
+    if (!a->act && (a->dx || a->dw)) rows[nrows++] = Rows{&dz.p, &dz.pitch, a->m, a->n, w.dy};
+    if (int rc = align_rows(rows, nrows, s)) return rc;
     if (a->act) {  // dz, and the sums of its rows from the same 32-bit values
         Gemm g = product_of(x, wt, a->m, a->n, a->k, a->type);
         g.epi = EPI_DZ;
@@ -281,8 +307,6 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
             if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, w.sums, nullptr, 0, s)) return rc;
             if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, s)) return rc;
         }
-        if (a->dx || a->dw)
-            if (int rc = align_rows(&dz.p, &dz.pitch, a->m, a->n, w.dy, s)) return rc;
     }
     if (a->dx) {
         Gemm g = product_of(dz, Operand{wt.p, wt.pitch, a->w_cols == 0}, a->m, a->k, a->n, a->type);
@@ -307,8 +331,8 @@ int pcb_clear_vocab_loss(const PcbClearVocab* a, void* ws, size_t ws_bytes, cuda
     const VocabWs w = loss_ws(a, ws);
     if (int rc = bad_ws("clear_vocab_loss", ws, ws_bytes, w.bytes)) return rc;
     Operand h{a->h, a->h_pitch, true}, wt{a->w, a->w_pitch, true};
-    if (int rc = align_rows(&h.p, &h.pitch, a->rows, a->dim, w.h, s)) return rc;
-    if (int rc = align_rows(&wt.p, &wt.pitch, a->vocab, a->dim, w.w, s)) return rc;
+    const Rows rows[] = {{&h.p, &h.pitch, a->rows, a->dim, w.h}, {&wt.p, &wt.pitch, a->vocab, a->dim, w.w}};
+    if (int rc = align_rows(rows, 2, s)) return rc;
     Gemm g = product_of(h, wt, a->rows, a->vocab, a->dim, a->type);
     g.epi = EPI_LSE;
     g.targets = a->targets, g.parts = w.parts, g.hit = w.hit;
@@ -329,8 +353,8 @@ int pcb_clear_vocab_grad(const PcbClearVocabGrad* a, void* ws, size_t ws_bytes, 
     const VocabWs w = vgrad_ws(a, ws);
     if (int rc = bad_ws("clear_vocab_grad", ws, ws_bytes, w.bytes)) return rc;
     Operand h{v.h, v.h_pitch, true}, wt{v.w, v.w_pitch, true};
-    if (int rc = align_rows(&h.p, &h.pitch, v.rows, v.dim, w.h, s)) return rc;
-    if (int rc = align_rows(&wt.p, &wt.pitch, v.vocab, v.dim, w.w, s)) return rc;
+    const Rows rows[] = {{&h.p, &h.pitch, v.rows, v.dim, w.h}, {&wt.p, &wt.pitch, v.vocab, v.dim, w.w}};
+    if (int rc = align_rows(rows, 2, s)) return rc;
     launch_pdl(prepare_rows, dim3((v.rows + 1023) / 1024), dim3(1024), s, v, a->weight, w.rows, w.unscale);
     if (int rc = PCB_LAUNCH_RESULT()) return rc;
     const bool whole = w.piece >= v.vocab;
@@ -344,7 +368,7 @@ int pcb_clear_vocab_grad(const PcbClearVocabGrad* a, void* ws, size_t ws_bytes, 
         if (a->dh) {
             g = product_of(Operand{w.slopes, w.slope_pitch, true}, Operand{wp, wt.pitch, false}, v.rows, v.dim, cols, v.type);
             if (whole) g.y = a->dh, g.y_pitch = a->dh_pitch, g.alpha = w.unscale, g.partial = w.partial;
-            else g.y = w.dh, g.y_pitch = v.dim, g.y_type = PCB_F32, g.accumulate = v0 > 0, g.whole = true;
+            else g.y = w.dh, g.y_pitch = w.dh_pitch, g.y_type = PCB_F32, g.slices = w.slices, g.accumulate = v0 > 0;
             if (int rc = gemm(g, s)) return rc;
         }
         if (a->dw) {
@@ -354,8 +378,8 @@ int pcb_clear_vocab_grad(const PcbClearVocabGrad* a, void* ws, size_t ws_bytes, 
         }
     }
     if (!a->dh || whole) return 0;
-    launch_pdl(finish, dim3(1184), dim3(256), s, (const float*)w.dh, (int64_t)v.rows, (int64_t)v.dim, (const float*)w.unscale, a->dh,
-               a->dh_pitch, v.type);
+    launch_pdl(finish, dim3((unsigned)std::min(v.rows, 4096)), dim3(256), s, (const float*)w.dh, w.slices, (int64_t)v.rows, v.dim, w.dh_pitch,
+               (const float*)w.unscale, a->dh, a->dh_pitch, v.type);
     return PCB_LAUNCH_RESULT();
 }
 

@@ -10,6 +10,7 @@
 // (bounded as well), TMEM is freed and the block ends; pcb_device_timeouts counts it.
 #include "clear_gemm.h"
 
+#include <algorithm>
 #include <cstring>
 
 #include "mma.cuh"
@@ -26,33 +27,40 @@ namespace {
 constexpr int SMS = 148;
 constexpr int BM = 128, BK = 64;
 constexpr float LOG2E = 1.4426950408889634f;
+// the kernels' epilogues: EPI_STORE without and with `extra`, and the others
+enum { KERNEL_STORE, KERNEL_ADD, KERNEL_DZ, KERNEL_LSE, KERNEL_DL };
+enum { EXTRA_TMA = 1, EXTRA_COPY = 2, EXTRA_LOAD = 3 };  // how `extra` is read: boxes, 4-byte asynchronous copies, loads
 
 // A tile is 128 x BN by one block, or 256 x BN by a pair (128 rows of A and half of B's rows in each block's shared memory:
 // per product each SM reads a third less of it than alone, and half of B crosses from L2 once instead of twice)
-template <int BN, int CTAS>
+template <int BN, int CTAS, int EPI>
 struct Shape {
     static constexpr int B_ROWS = BN / CTAS;
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int EWARPS = BN == 64 ? 4 : 8;         // epilogue warps: 4 cover the 128 lanes, 8 halve the columns
-    static constexpr int STAGES = BN == 64 ? 8 : STAGE == 32768 ? 5 : 6;
     static constexpr int COLS = BN / (EWARPS / 4);          // columns of one epilogue warp
     static constexpr int THREADS = 64 + 32 * EWARPS;
     static constexpr int TMEM = 2 * BN;
-    static constexpr int STAGING = 4096;                    // per epilogue warp: 32 rows x 128 bytes, out and in
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EWARPS * (2 * STAGING + 128) + 512;
+    static constexpr int STAGING = 4096;                    // per epilogue warp and direction: 32 rows x 128 bytes
+    static constexpr int BUFFERS = EPI == KERNEL_ADD || EPI == KERNEL_DZ ? 2 : 1;
+    static constexpr int STAGES = BN == 64 ? 8 : STAGE == 32768 ? (BUFFERS == 2 ? 5 : 6) : (BUFFERS == 2 ? 6 : 8);
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EWARPS * (BUFFERS * STAGING + 128) + 512;
 };
 
 struct alignas(64) Params {
-    CUtensorMap a, b, y, extra_map;
+    CUtensorMap a, b, y, extra_map, part;
     int m, n, k;
     int a_mn, b_mn, a_panels, b_panels, bf16;
-    int tiles_m, tiles_n, splits, kblocks, kper;  // k blocks in all and of one split
+    int tiles_m, tiles_n, kblocks;
+    // Units of work: tiles [0, whole) entire, then the other `tail` tiles in `splits` parts of `kper` k blocks: to 32-bit
+    // sums that `join` finishes, or (slices) each part to its own y
+    int whole, tail, splits, kper, slices;
     Act act;
     const void* bias;
     const void* extra;
     void* y_ptr;
     int64_t extra_pitch, y_pitch;
-    int bias_type, extra_type, y_type, y_tma, extra_tma, accumulate;
+    int bias_type, extra_type, y_type, y_tma, extra_mode, accumulate;
     const float* alpha;
     float* row_sums;
     const VocabRow* rows;
@@ -61,6 +69,22 @@ struct alignas(64) Params {
     float2* parts;
     float* hit;
 };
+
+struct Unit {
+    int tile, split, kb0, kb1;
+    bool partial;
+};
+__device__ __forceinline__ Unit unit_of(const Params& p, int u) {
+    Unit w = {u, 0, 0, p.kblocks, false};
+    if (u >= p.whole) {
+        w.split = (u - p.whole) / p.tail;
+        w.tile = u - w.split * p.tail;
+        w.kb0 = w.split * p.kper;
+        w.kb1 = min(p.kblocks, w.kb0 + p.kper);
+        w.partial = !p.slices;
+    }
+    return w;
+}
 
 // ------------------------------------------------------------------------------------------------ epilogue pieces
 // GELU z Phi(z) and its slope Phi(z) + z phi(z), two values at a time. Phi from Abramowitz and Stegun 7.1.26 (absolute error
@@ -123,21 +147,37 @@ __device__ __forceinline__ float lane_sums(float* v) {
     return v[0];
 }
 
-// 32 x 32 values of a row-major array at (row0, col0), rows and columns past the end as zero, in 32 bits into the warp's
-// staging buffer as a box of the TMA engine would lie there; read along the rows (lane = column). For arrays that the engine
-// cannot read.
-__device__ __noinline__ void load_block(const void* p, int64_t pitch, int type, int row0, int col0, int m, int n, unsigned char* stage) {
+// 32 x 32 values of a row-major array at (row0, col0), rows and columns past the end as zero, in 32 bits to where a box of
+// the TMA engine would put them; along the rows (lane = column). For arrays that the engine cannot read: 32-bit values by
+// asynchronous copies of 4 bytes (copy_wait, then __syncwarp), 16-bit ones by loads.
+__device__ __forceinline__ uint32_t block_at(int r, int c) { return r * 128 + ((c / 4) ^ (r & 7)) * 16 + c % 4 * 4; }
+__device__ __noinline__ void copy_block(const void* p, int64_t pitch, int row0, int col0, int m, int n, unsigned char* to) {
     const int lane = threadIdx.x % 32;
     const bool in = col0 + lane < n;
-#pragma unroll 16
-    for (int r = 0; r < 32; ++r)
-        *(float*)(stage + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4) =
-            in && row0 + r < m ? load(p, (int64_t)(row0 + r) * pitch + col0 + lane, type) : 0.0f;
+    const float* x = (const float*)p + (int64_t)row0 * pitch + col0 + lane;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r, x += pitch) {
+        const bool here = in && row0 + r < m;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(to + block_at(r, lane))), "l"(here ? (const void*)x : p),
+                     "r"(here ? 4 : 0)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __noinline__ void load_block(const void* p, int64_t pitch, int type, int row0, int col0, int m, int n, unsigned char* to) {
+    const int lane = threadIdx.x % 32;
+    const bool in = col0 + lane < n;
+    float v[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) v[r] = in && row0 + r < m ? load(p, (int64_t)(row0 + r) * pitch + col0 + lane, type) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) *(float*)(to + block_at(r, lane)) = v[r];
     __syncwarp();
 }
 // A box of the staging buffer (32 rows x 128 bytes, 16-byte pieces swizzled by the row) to rows that the engine cannot write
 __device__ __noinline__ void store_block(const unsigned char* stage, bool narrow, void* y, int64_t pitch, int rows, int cols, bool add) {
     const int lane = threadIdx.x % 32;
+#pragma unroll 4
     for (int r = 0; r < rows; ++r) {
         const unsigned char* row = stage + r * 128;
         for (int c = lane; c < min(cols, narrow ? 64 : 32); c += 32) {
@@ -155,12 +195,12 @@ __device__ __noinline__ void store_block(const unsigned char* stage, bool narrow
 
 // ------------------------------------------------------------------------------------------------ the kernel
 template <int BN, int CTAS, int EPI, int ACT>
-__global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __grid_constant__ Params p) {
-    using S = Shape<BN, CTAS>;
+__global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(const __grid_constant__ Params p) {
+    using S = Shape<BN, CTAS, EPI>;
     extern __shared__ unsigned char raw[];
     unsigned char* base = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     unsigned char* staging = base + S::STAGES * S::STAGE;
-    float* bias_s = (float*)(staging + S::EWARPS * 2 * S::STAGING);
+    float* bias_s = (float*)(staging + S::EWARPS * S::BUFFERS * S::STAGING);
     uint64_t* full = (uint64_t*)(bias_s + S::EWARPS * 32);
     uint64_t* empty = full + S::STAGES;
     uint64_t* acc_full = empty + S::STAGES;
@@ -197,17 +237,16 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
     pdl_wait();
     pdl_release();
 
-    const int tiles = p.tiles_m * p.tiles_n * p.splits;
-    const int first_tile = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
+    const int units = p.whole + p.tail * p.splits;
+    const int first_unit = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
     if (warp == 0) {
         Ring<S::STAGES> r;
         int loaded = 0;
         bool ok = true, ready = true;
-        for (int tile = first_tile; tile < tiles && ok; tile += stride) {
-            const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
-            const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, n0 = mn / p.tiles_m * BN + rank * S::B_ROWS;
-            const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
-            for (int kb = kb0; kb < kb1; ++kb, ++loaded, r.next()) {
+        for (int u = first_unit; u < units && ok; u += stride) {
+            const Unit w = unit_of(p, u);
+            const int m0 = (w.tile % p.tiles_m * CTAS + rank) * BM, n0 = w.tile / p.tiles_m * BN + rank * S::B_ROWS;
+            for (int kb = w.kb0; kb < w.kb1; ++kb, ++loaded, r.next()) {
                 // a fresh barrier's preceding phase counts as done: the first round does not wait
                 if (!__all_sync(~0u, ready)) ok = wait_warp(&empty[r.stage], r.phase ^ 1, dead, &g_gemm_timeouts);
                 if (!ok) break;
@@ -249,14 +288,14 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
             Ring<S::STAGES> r;
             Ring<2> out;
             bool ok = true, ready = false;
-            for (int tile = first_tile; tile < tiles && ok; tile += stride, out.next()) {
-                const int sp = tile / (p.tiles_m * p.tiles_n);
-                const int kb0 = sp * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
+            for (int u = first_unit; u < units && ok; u += stride) {
+                const Unit w = unit_of(p, u);
+                if (w.kb0 >= w.kb1) continue;
                 ok = wait_warp(&acc_empty[out.stage], out.phase ^ 1, dead, &g_gemm_timeouts);
                 if (!ok) break;
                 fence_after();
                 const uint32_t acc = tmem + out.stage * BN;
-                for (int kb = kb0; kb < kb1; ++kb, r.next()) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb, r.next()) {
                     if (!__all_sync(~0u, ready)) ok = wait_warp(&full[r.stage], r.phase, dead, &g_gemm_timeouts);
                     if (!ok) break;
                     fence_after();
@@ -266,12 +305,13 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                     const uint64_t da = a_desc + (uint32_t)(r.stage * (S::STAGE >> 4)), db = b_desc + (uint32_t)(r.stage * (S::STAGE >> 4));
                     if (elect()) {
 #pragma unroll
-                        for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > kb0 || q > 0);
+                        for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > w.kb0 || q > 0);
                         mma_commit<CTAS>(&empty[r.stage]);
-                        if (kb + 1 == kb1) mma_commit<CTAS>(&acc_full[out.stage]);
+                        if (kb + 1 == w.kb1) mma_commit<CTAS>(&acc_full[out.stage]);
                     }
                     __syncwarp();
                 }
+                out.next();
             }
             if (!ok) {  // the products in flight
                 if (elect()) mma_commit<CTAS>(drain);
@@ -280,8 +320,8 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
         }
     } else {
         const int ew = warp - 2, quad = warp % 4, half = ew / 4;
-        unsigned char* stage = staging + ew * 2 * S::STAGING;
-        unsigned char* in = stage + S::STAGING;  // `extra`'s boxes: 32 rows x 128 bytes, the next one on its way
+        unsigned char* stage = staging + ew * S::BUFFERS * S::STAGING;
+        unsigned char* in = stage + (S::BUFFERS - 1) * S::STAGING;  // `extra`'s boxes: 32 rows x 128 bytes, the next one on its way
         float* bias = bias_s + ew * 32;
         const float alpha = p.alpha ? *p.alpha : 1.0f;
         const uint32_t leader_empty[2] = {CTAS == 2 ? cluster_addr(&acc_empty[0], 0) : 0, CTAS == 2 ? cluster_addr(&acc_empty[1], 0) : 0};
@@ -292,59 +332,74 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
             else mbar_arrive(&acc_empty[buf]);
         };
         // the boxes of `extra` in the order that they are used: box e of a tile covers columns [e ecols, ...) of the warp's
-        constexpr bool USES_EXTRA = EPI == EPI_STORE || EPI == EPI_DZ;
-        const bool extra_tma = USES_EXTRA && p.extra_tma;
-        const int ecols = p.extra_type == PCB_F32 ? 32 : 64;
+        constexpr bool HAS_EXTRA = S::BUFFERS == 2, AFFINE = HAS_EXTRA || EPI == KERNEL_STORE;
+        const bool extra_wide = p.extra_mode != EXTRA_TMA || p.extra_type == PCB_F32;
+        const int ecols = extra_wide ? 32 : 64;
         int fetched = 0;
-        auto fetch = [&](int tile, int e) {
-            if (!extra_tma || lane) return;
-            while (USES_EXTRA) {  // the next box with columns inside: of this tile, or the first of the next
-                if (tile >= tiles) return;
-                const int mn = tile % (p.tiles_m * p.tiles_n);
-                const int x = mn / p.tiles_m * BN + half * S::COLS + e * ecols;
-                if (e * ecols < S::COLS && x < p.n) {
-                    const int y = (mn % p.tiles_m * CTAS + rank) * BM + quad * 32;
-                    fence_async_smem();
-                    mbar_expect(&extra_full[ew], S::STAGING);
-                    tma_load(in, &p.extra_map, x, y, &extra_full[ew]);
-                    return;
+        auto fetch = [&](int u, int e) {
+            if (p.extra_mode == EXTRA_LOAD) return;
+            for (; HAS_EXTRA && u < units; u += stride, e = 0) {  // the next box with columns inside: of this unit, or the first of a later one
+                const Unit w = unit_of(p, u);
+                const int x = w.tile / p.tiles_m * BN + half * S::COLS + e * ecols;
+                if (w.partial || e * ecols >= S::COLS || x >= p.n) continue;
+                const int y = (w.tile % p.tiles_m * CTAS + rank) * BM + quad * 32;
+                if (p.extra_mode == EXTRA_TMA) {
+                    if (lane == 0) {
+                        fence_async_smem();
+                        mbar_expect(&extra_full[ew], S::STAGING);
+                        tma_load(in, &p.extra_map, x, y, &extra_full[ew]);
+                    }
+                } else {
+                    copy_block(p.extra, p.extra_pitch, y, x, p.m, p.n, in);
                 }
-                tile += stride;
-                e = 0;
+                return;
             }
         };
-        fetch(first_tile, 0);
+        if constexpr (HAS_EXTRA) fetch(first_unit, 0);
         int t = 0;
-        for (int tile = first_tile; tile < tiles; tile += stride, ++t) {
-            const int sp = tile / (p.tiles_m * p.tiles_n), mn = tile % (p.tiles_m * p.tiles_n);
-            const int m0 = (mn % p.tiles_m * CTAS + rank) * BM, tn = mn / p.tiles_m, n0 = tn * BN;
+        for (int u = first_unit; u < units; u += stride) {
+            const Unit w = unit_of(p, u);
+            if (w.kb0 >= w.kb1) continue;
+            const int m0 = (w.tile % p.tiles_m * CTAS + rank) * BM, tn = w.tile / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
             auto bias_of = [&](int col) { return col + lane < p.n ? load(p.bias, col + lane, p.bias_type) : 0.0f; };
             float next_bias = 0.0f;
-            if (USES_EXTRA && p.bias) next_bias = bias_of(first);
+            if (AFFINE && p.bias && !w.partial) next_bias = bias_of(first);
             if (!wait_warp<true>(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
+            ++t;
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
             const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));
             float top = -INFINITY, sum = 0.0f, lse2 = 0.0f, weight = 0.0f;
             int target = -1;  // the row's column among this warp's, if it is there
-            if (EPI == EPI_DL && row < p.m) {
+            if (EPI == KERNEL_DL && row < p.m) {
                 const VocabRow vr = p.rows[row];
                 lse2 = vr.lse2, weight = vr.weight, target = vr.target - p.col0 - first;
             }
-            if (EPI == EPI_LSE && row < p.m) {
+            if (EPI == KERNEL_LSE && row < p.m) {
                 const int64_t at = p.targets[row] - first;
                 target = at >= 0 && at < S::COLS ? (int)at : -1;
             }
             uint32_t held[16];
+            auto put_wide = [&](const float* v) {  // the lane's 32 values into the staging buffer
+                if (lane == 0) bulk_wait_read();
+                __syncwarp();
+                uint4* srow = (uint4*)(stage + lane * 128);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    srow[j ^ (lane & 7)] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                      __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                fence_async_smem();
+                __syncwarp();
+            };
             for (int c = 0; c < chunks; ++c) {
                 const int col0 = first + 32 * c;
                 float v[32];
                 tmem_ld32(acc + 32 * c, v);
                 ld_wait();
                 if (c == chunks - 1) release(buf);
-                const bool has_target = (EPI == EPI_LSE || EPI == EPI_DL) && __any_sync(~0u, (unsigned)(target - 32 * c) < 32u);
-                if (EPI == EPI_LSE) {
+                const bool has_target = (EPI == KERNEL_LSE || EPI == KERNEL_DL) && __any_sync(~0u, (unsigned)(target - 32 * c) < 32u);
+                if (EPI == KERNEL_LSE) {
                     if (has_target) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
@@ -371,7 +426,16 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                     top = nt;
                     continue;
                 }
-                if (EPI == EPI_STORE || EPI == EPI_DZ) {
+                if (AFFINE && w.partial) {  // 32-bit sums for `join`, in tiles of their own
+                    put_wide(v);
+                    if (lane == 0 && row0 < p.m) {
+                        const int at = ((w.split * p.tail + w.tile - p.whole) * CTAS + (int)rank) * BM + quad * 32;
+                        tma_store(&p.part, half * S::COLS + 32 * c, at, 0, stage);
+                        bulk_commit();
+                    }
+                    continue;
+                }
+                if (AFFINE) {
                     if (p.bias) {
                         __syncwarp();
                         bias[lane] = next_bias;
@@ -386,23 +450,25 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                     }
                     if (ACT != PCB_ACT_NONE) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) parts(act2<ACT, EPI == EPI_DZ>(p.act, two(v[j], v[j + 1])), v[j], v[j + 1]);
+                        for (int j = 0; j < 32; j += 2) parts(act2<ACT, EPI == KERNEL_DZ>(p.act, two(v[j], v[j + 1])), v[j], v[j + 1]);
                     }
-                    if (p.extra) {
-                        const bool wide = !extra_tma || p.extra_type == PCB_F32;
-                        if (!extra_tma) {
-                            if (lane == 0) bulk_wait_read();
-                            __syncwarp();
-                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, stage);
-                        } else if (wide || c % 2 == 0) {
-                            if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) break;
+                    if constexpr (HAS_EXTRA) {
+                        if (p.extra_mode == EXTRA_LOAD) {
+                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, in);
+                        } else if (extra_wide || c % 2 == 0) {
+                            if (p.extra_mode == EXTRA_COPY) {
+                                copy_wait();
+                                __syncwarp();
+                            } else if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) {
+                                break;
+                            }
                         }
-                        const uint4* irow = (const uint4*)((extra_tma ? in : stage) + lane * 128);
+                        const uint4* irow = (const uint4*)(in + lane * 128);
                         auto join = [&](int j, float e0, float e1) {
                             const f32x2 a = two(v[j], v[j + 1]), e = two(e0, e1);
-                            parts(EPI == EPI_DZ ? mul2(a, e) : add2(a, e), v[j], v[j + 1]);
+                            parts(EPI == KERNEL_DZ ? mul2(a, e) : add2(a, e), v[j], v[j + 1]);
                         };
-                        if (wide) {
+                        if (extra_wide) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
                                 const uint4 q = irow[j ^ (lane & 7)];
@@ -413,24 +479,24 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const uint4 q = irow[(j + (c % 2) * 4) ^ (lane & 7)];
-                                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                                const uint32_t x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     float e[2];
-                                    unpack2(w[i], p.bf16, e);
+                                    unpack2(x[i], p.bf16, e);
                                     join(8 * j + 2 * i, e[0], e[1]);
                                 }
                             }
                         }
                         __syncwarp();
-                        if (extra_tma && (wide || c % 2 || c + 1 == chunks)) fetch(tile, wide ? c + 1 : c / 2 + 1);
+                        if (extra_wide || c % 2 || c + 1 == chunks) fetch(u, extra_wide ? c + 1 : c / 2 + 1);
                     }
-                    if (EPI == EPI_STORE && p.alpha) {
+                    if (EPI != KERNEL_DZ && p.alpha) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] *= alpha;
                     }
                 }
-                if (EPI == EPI_DL) {
+                if (EPI == KERNEL_DL) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         float a, b;
@@ -450,7 +516,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
 #pragma unroll
                     for (int j = 0; j < 16; ++j) now[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
                 }
-                if (EPI == EPI_DZ && p.row_sums) {
+                if (EPI == KERNEL_DZ && p.row_sums) {
                     const float s = lane_sums(v);
                     if (col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
                 }
@@ -459,10 +525,10 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
                     for (int j = 0; j < 16; ++j) held[j] = now[j];
                     continue;
                 }
-                if (lane == 0) bulk_wait_read();
-                __syncwarp();
-                uint4* srow = (uint4*)(stage + lane * 128);
                 if (narrow) {
+                    if (lane == 0) bulk_wait_read();
+                    __syncwarp();
+                    uint4* srow = (uint4*)(stage + lane * 128);
                     if (c % 2) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
@@ -471,32 +537,31 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         srow[(j + (c % 2) * 4) ^ (lane & 7)] = make_uint4(now[4 * j], now[4 * j + 1], now[4 * j + 2], now[4 * j + 3]);
+                    fence_async_smem();
+                    __syncwarp();
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        srow[j ^ (lane & 7)] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                          __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                    put_wide(v);
                 }
                 const int box0 = narrow ? col0 - (c % 2) * 32 : col0;
                 if (p.y_tma) {
-                    fence_async_smem();
-                    __syncwarp();
                     if (lane == 0 && row0 < p.m) {
-                        if (p.accumulate) tma_add(&p.y, box0, row0, sp, stage);
-                        else tma_store(&p.y, box0, row0, sp, stage);
+                        if (p.accumulate) tma_add(&p.y, box0, row0, w.split, stage);
+                        else tma_store(&p.y, box0, row0, w.split, stage);
                         bulk_commit();
                     }
                 } else {
-                    __syncwarp();
-                    const int64_t at = ((int64_t)sp * p.m + row0) * p.y_pitch + box0;
+                    const int64_t at = ((int64_t)w.split * p.m + row0) * p.y_pitch + box0;
                     store_block(stage, narrow, (char*)p.y_ptr + at * (narrow ? 2 : 4), p.y_pitch, min(32, p.m - row0), p.n - box0, p.accumulate);
                 }
             }
             if (chunks == 0) release(buf);
-            if (EPI == EPI_LSE && row < p.m) p.parts[(int64_t)(tn * (S::EWARPS / 4) + half) * p.m + row] = make_float2(top, sum);
+            if (EPI == KERNEL_LSE && row < p.m) p.parts[(int64_t)(tn * (S::EWARPS / 4) + half) * p.m + row] = make_float2(top, sum);
         }
         if (lane == 0) bulk_wait();
-        if (*dead && extra_tma && lane == 0) mbar_wait(&extra_full[ew], fetched & 1);  // the box in flight
+        if (HAS_EXTRA) {  // the box in flight, where the warp gave up
+            copy_wait();
+            if (*dead && p.extra_mode == EXTRA_TMA && lane == 0) mbar_wait(&extra_full[ew], fetched & 1);
+        }
     }
     __syncwarp();
     fence_before();
@@ -506,31 +571,58 @@ __global__ void __launch_bounds__(Shape<BN, CTAS>::THREADS, 1) product(const __g
     if (warp == 1) tmem_free<CTAS>(tmem, S::TMEM);
 }
 
-// y = alpha (act(sum of the splits + bias) + extra), the splits in order
-__global__ void __launch_bounds__(256) join(const float* part, int splits, const __grid_constant__ Params p) {
+// The split tiles: y = alpha (act(sum of the parts in order + bias) + extra). Sixteen rows of a tile per block.
+constexpr int JOIN_ROWS = 16;
+__global__ void __launch_bounds__(256) join(const float* part, int bn, int tile_rows, const __grid_constant__ Params p) {
     pdl_wait();
     pdl_release();
     const float alpha = p.alpha ? *p.alpha : 1.0f;
-    const int64_t total = (int64_t)p.m * p.n;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float v = 0.0f;
-        for (int s = 0; s < splits; ++s) v += part[s * total + i];
-        const int64_t r = i / p.n, c = i % p.n;
-        if (p.bias) v += load(p.bias, c, p.bias_type);
-        float skip;
-        if (p.act.kind == PCB_ACT_GELU) parts(act2<PCB_ACT_GELU, false>(p.act, both(v)), v, skip);
-        else if (p.act.kind == PCB_ACT_POLY) parts(act2<PCB_ACT_POLY, false>(p.act, both(v)), v, skip);
-        if (p.extra) v += load(p.extra, r * p.extra_pitch + c, p.extra_type);
-        store(p.y_ptr, r * p.y_pitch + c, p.y_type, v * alpha);
+    const int groups = tile_rows / JOIN_ROWS, i = blockIdx.x / groups, r0 = blockIdx.x % groups * JOIN_ROWS;
+    const int tile = p.whole + i, quads = bn / 4;
+    const int64_t row0 = (int64_t)(tile % p.tiles_m) * tile_rows + r0, col0 = (int64_t)(tile / p.tiles_m) * bn;
+    const int64_t step = (int64_t)p.tail * tile_rows * quads;
+    for (int e = threadIdx.x; e < JOIN_ROWS * quads; e += 256) {
+        const int64_t row = row0 + e / quads, col = col0 + e % quads * 4;
+        if (row >= p.m || col >= p.n) continue;
+        const float4* at = (const float4*)part + ((int64_t)i * tile_rows + r0) * quads + e;
+        float4 s = at[0];
+        for (int k = 1; k < p.splits; ++k) {
+            const float4 q = at[k * step];
+            s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+        }
+        const float v4[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (col + j >= p.n) break;
+            float v = v4[j], skip;
+            if (p.bias) v += load(p.bias, col + j, p.bias_type);
+            if (p.act.kind == PCB_ACT_GELU) parts(act2<PCB_ACT_GELU, false>(p.act, both(v)), v, skip);
+            else if (p.act.kind == PCB_ACT_POLY) parts(act2<PCB_ACT_POLY, false>(p.act, both(v)), v, skip);
+            if (p.extra) v += load(p.extra, row * p.extra_pitch + col + j, p.extra_type);
+            store(p.y_ptr, row * p.y_pitch + col + j, p.y_type, v * alpha);
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) copy_rows(const uint16_t* x, int64_t pitch, int64_t rows, int cols, uint16_t* y, int64_t to) {
+// Rows of 16-bit values to rows on 16 bytes, zeros up to the pitch; a warp per row, up to three matrices (blockIdx.y)
+struct CopyJobs {
+    const uint16_t* x[3];
+    uint32_t* y[3];
+    int64_t pitch[3], rows[3];
+    int cols[3], to[3];
+};
+__global__ void __launch_bounds__(256) copy_rows(const __grid_constant__ CopyJobs j) {
     pdl_wait();
     pdl_release();
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * to; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / to, c = i % to;
-        y[i] = c < cols ? x[r * pitch + c] : (uint16_t)0;
+    const int b = blockIdx.y, lane = threadIdx.x % 32, words = j.to[b] / 2;
+    for (int64_t r = blockIdx.x * 8ll + threadIdx.x / 32; r < j.rows[b]; r += gridDim.x * 8ll) {
+        const uint16_t* x = j.x[b] + r * j.pitch[b];
+        uint32_t* y = j.y[b] + r * words;
+#pragma unroll 4
+        for (int c = lane; c < words; c += 32) {
+            const uint32_t lo = 2 * c < j.cols[b] ? x[2 * c] : 0, hi = 2 * c + 1 < j.cols[b] ? x[2 * c + 1] : 0;
+            y[c] = lo | hi << 16;
+        }
     }
 }
 
@@ -584,45 +676,68 @@ int operand_map(CUtensorMap* map, const Operand& o, int type, int rows, int k, i
     return encode_map(map, type, o.p, 3, size, stride, box);
 }
 
-// Tile and k splits, from estimated cycles: a 64-k block of a tile costs its products (512 cycles at a width of 256, the
-// tensor core's rate) or its bytes into shared memory where they take longer, a tile about 1200 cycles of latency besides, a
-// split its 32-bit traffic and the joining launch.
+// Tile and splitting, from estimated nanoseconds. A 64-k block of a tile costs its products, or its bytes into shared memory
+// at what one SM or all of them together take (measured over 9472 x 4096 x 512: 85 GB/s for each of 148 SMs; 256 x 256 by
+// pairs 393 ns a block, 256 x 128 297, 128 x 128 366, 128 x 64 265). The tiles that do not fill a round over the SMs may split
+// their k; that costs their 32-bit sums' way to L2 and back and a launch.
 struct Plan {
-    int bn, ctas, splits, kper;
+    int bn, ctas, whole, splits, kper;
+    double ns;
 };
-Plan plan(int m, int n, int k, bool may_split) {
-    struct Tile {
-        int bn, ctas;
-        double block;
+struct Tile {
+    int bn, ctas;
+    double products;  // ns of a 64-k block's
+};
+constexpr Tile TILES[] = {{256, 2, 270}, {128, 2, 150}, {128, 1, 150}, {64, 1, 120}};
+double rounds(const Tile& t, int64_t units, int kblocks) {
+    const int64_t slots = SMS / t.ctas, full = units / slots, rest = units % slots;
+    const double bytes = BM * BK * 2 + t.bn / t.ctas * BK * 2;
+    auto block = [&](int64_t active) {
+        const double one = bytes / 150, all = bytes * (double)(active * t.ctas) / 12500;
+        return std::max(t.products, std::max(one, all));
     };
-    static const Tile shapes[] = {{256, 2, 530}, {128, 2, 300}, {128, 1, 330}, {64, 1, 240}};
+    const double ends = 4.0 * t.bn;  // the part of a tile's epilogue and first loads that does not overlap
+    return full * (kblocks * block(slots) + ends) + (rest ? kblocks * block(rest) + ends : 0.0);
+}
+Plan plan(int m, int n, int k, bool may_split) {
     const int kb = (k + BK - 1) / BK;
-    Plan best{256, 2, 1, kb};
-    double least = 1e300;
-    for (const Tile& t : shapes) {
+    Plan best{256, 2, 0, 1, kb, 1e300};
+    for (const Tile& t : TILES) {
         const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
-        for (int sp = 1; sp <= (may_split ? 16 : 1); sp *= 2) {
+        const int64_t tiles = tm * tn, slots = SMS / t.ctas, tail = tiles % slots, whole = tiles - tail;
+        double ns = rounds(t, tiles, kb) + (t.ctas == 2 ? 200 : 0);
+        if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)tiles, 1, kb, ns};
+        for (int sp = 2; may_split && tail && sp <= 16; ++sp) {
             const int per = (kb + sp - 1) / sp;
-            if (sp > 1 && (per < 4 || (sp - 1) * per >= kb)) break;
-            const int slots = SMS / t.ctas;
-            const double waves = (double)((tm * tn * sp + slots - 1) / slots);
-            double cost = waves * (per * t.block + t.bn * 2.0) + 1200 + (t.ctas == 2 ? 300 : 0);
-            if (sp > 1) cost += 5000 + (double)m * n * 4 * sp * 2 / (SMS * 16.0);
-            if (cost < least) least = cost, best = Plan{t.bn, t.ctas, sp, per};
+            if (per < 4 || (sp - 1) * per >= kb) continue;
+            ns = rounds(t, whole, kb) + rounds(t, tail * sp, per) + (t.ctas == 2 ? 200 : 0) + 3500 +
+                 (double)tail * BM * t.ctas * t.bn * 8 * sp / 8000;
+            if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)whole, sp, per, ns};
         }
+    }
+    return best;
+}
+// k in `slices` parts to as many outputs: the tile for that many units
+Plan plan_slices(int m, int n, int k, int slices) {
+    const int kb = (k + BK - 1) / BK, per = (kb + slices - 1) / slices;
+    Plan best{256, 2, 0, slices, per, 1e300};
+    for (const Tile& t : TILES) {
+        const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
+        const double ns = rounds(t, tm * tn * slices, per) + (t.ctas == 2 ? 200 : 0) + (double)m * n * 8 * slices / 8000;
+        if (ns < best.ns) best = Plan{t.bn, t.ctas, 0, slices, per, ns};
     }
     return best;
 }
 
 template <int BN, int CTAS, int EPI, int ACT>
 int launch(const Params& p, cudaStream_t s) {
-    using S = Shape<BN, CTAS>;
+    using S = Shape<BN, CTAS, EPI>;
     static_assert(S::SMEM <= 232448, "shared memory");
     static const cudaError_t set = cudaFuncSetAttribute(product<BN, CTAS, EPI, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     if (set != cudaSuccess) return (int)set;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits, slots = SMS / CTAS;
+    const int64_t units = (int64_t)p.whole + (int64_t)p.tail * p.splits, slots = SMS / CTAS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * CTAS));
+    cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * CTAS));
     cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = s;
@@ -647,59 +762,87 @@ int launch(const Plan& pl, const Params& p, cudaStream_t s) {
 
 size_t gemm_partial(int m, int n, int k) {
     const Plan pl = plan(m, n, k, true);
-    return pl.splits > 1 ? (size_t)pl.splits * m * n : 0;
+    if (pl.splits == 1) return 0;
+    const size_t rows = BM * pl.ctas;
+    const size_t tiles = ((size_t)m + rows - 1) / rows * (((size_t)n + pl.bn - 1) / pl.bn);
+    return (tiles - pl.whole) * pl.splits * rows * pl.bn;
+}
+double gemm_cost(int m, int n, int k, bool may_split) { return plan(m, n, k, may_split).ns; }
+int gemm_slices(int m, int n, int k) {
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= 8; ++s) {
+        const Plan p = plan_slices(m, n, k, s);
+        if (s > 1 && (p.kper < 4 || (s - 1) * p.kper >= (k + BK - 1) / BK)) continue;  // every part has some of k
+        if (p.ns < 0.97 * least) least = p.ns, best = s;
+    }
+    return best;
 }
 int vocab_parts(int m, int n) {
-    const int bn = plan(m, n, 1 << 20, false).bn;
+    const int bn = plan(m, n, 1 << 10, false).bn;
     return (n + bn - 1) / bn * (bn == 64 ? 1 : 2);
 }
 
 int gemm(const Gemm& g, cudaStream_t s) {
     // the column blocks of an EPI_LSE product follow vocab_parts, which does not know k
-    const Plan pl = plan(g.m, g.n, g.epi == EPI_LSE ? 1 << 20 : g.k, g.epi == EPI_STORE && !g.accumulate && !g.whole);
-    const int kb = (g.k + BK - 1) / BK;
+    const Plan pl = g.slices ? plan_slices(g.m, g.n, g.k, g.slices) : plan(g.m, g.n, g.epi == EPI_LSE ? 1 << 10 : g.k, g.epi == EPI_STORE && g.partial);
+    const int rows = BM * pl.ctas;
+    const int64_t tm = ((int64_t)g.m + rows - 1) / rows, tn = ((int64_t)g.n + pl.bn - 1) / pl.bn;
+    if (tm * tn * pl.splits > INT32_MAX) return report(PCB_BAD_ARGS, "a product of %d x %d outputs", g.m, g.n);
     Params p;
     memset(&p, 0, sizeof p);
     if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, BM)) return rc;
     if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn / pl.ctas)) return rc;
     p.m = g.m, p.n = g.n, p.k = g.k;
-    p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.a_panels = panels(g.a, g.m), p.b_panels = panels(g.b, g.n), p.bf16 = g.type == PCB_BF16;
-    p.tiles_m = (int)(((int64_t)g.m + BM * pl.ctas - 1) / (BM * pl.ctas)), p.tiles_n = (g.n + pl.bn - 1) / pl.bn;
-    p.splits = pl.splits, p.kblocks = kb, p.kper = pl.splits > 1 ? pl.kper : kb;
+    p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.a_panels = panels(g.a, g.m), p.b_panels = panels(g.b, g.n);
+    p.bf16 = g.type == PCB_BF16;
+    p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.kblocks = (g.k + BK - 1) / BK;
+    p.whole = pl.whole, p.tail = (int)(tm * tn) - pl.whole, p.splits = pl.splits, p.kper = pl.kper, p.slices = g.slices;
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;
     p.extra = g.extra, p.extra_pitch = g.extra_pitch, p.extra_type = g.extra_type;
     p.y_ptr = g.y, p.y_pitch = g.y_pitch, p.y_type = g.y_type, p.accumulate = g.accumulate;
     p.alpha = g.alpha, p.row_sums = g.row_sums, p.rows = g.rows, p.col0 = g.col0, p.targets = g.targets, p.parts = g.parts, p.hit = g.hit;
-    Params fin = p;
-    if (pl.splits > 1) {  // 32-bit sums of each split, the epilogue in `join`
-        p.act = Act{}, p.bias = nullptr, p.extra = nullptr, p.alpha = nullptr;
-        p.y_ptr = g.partial, p.y_pitch = g.n, p.y_type = PCB_F32;
-    }
     const size_t eb = type_bytes(p.y_type);
     // 16-byte aligned rows go through the TMA engine; others by rows of the staging buffer
     p.y_tma = g.epi != EPI_LSE && ((uintptr_t)p.y_ptr & 15) == 0 && p.y_pitch * eb % 16 == 0;
     if (p.y_tma) {
-        const uint64_t size[3] = {(uint64_t)g.n, (uint64_t)g.m, (uint64_t)pl.splits};
+        const uint64_t size[3] = {(uint64_t)g.n, (uint64_t)g.m, (uint64_t)(g.slices ? g.slices : 1)};
         const uint64_t stride[2] = {(uint64_t)p.y_pitch * eb, (uint64_t)p.y_pitch * eb * g.m};
         const uint32_t box[3] = {(uint32_t)(128 / eb), 32, 1};
         if (int rc = encode_map(&p.y, p.y_type, p.y_ptr, 3, size, stride, box)) return rc;
     }
-    if (p.extra && ((uintptr_t)p.extra & 15) == 0 && p.extra_pitch * type_bytes(p.extra_type) % 16 == 0) {
-        const uint64_t size[2] = {(uint64_t)g.n, (uint64_t)g.m}, stride[1] = {(uint64_t)(p.extra_pitch * type_bytes(p.extra_type))};
-        const uint32_t box[2] = {(uint32_t)(128 / type_bytes(p.extra_type)), 32};
-        if (int rc = encode_map(&p.extra_map, p.extra_type, p.extra, 2, size, stride, box)) return rc;
-        p.extra_tma = 1;
+    if (p.extra) {
+        const size_t ee = type_bytes(p.extra_type);
+        p.extra_mode = p.extra_type == PCB_F32 ? EXTRA_COPY : EXTRA_LOAD;
+        if (((uintptr_t)p.extra & 15) == 0 && p.extra_pitch * ee % 16 == 0) {
+            const uint64_t size[2] = {(uint64_t)g.n, (uint64_t)g.m}, stride[1] = {(uint64_t)(p.extra_pitch * ee)};
+            const uint32_t box[2] = {(uint32_t)(128 / ee), 32};
+            if (int rc = encode_map(&p.extra_map, p.extra_type, p.extra, 2, size, stride, box)) return rc;
+            p.extra_mode = EXTRA_TMA;
+        }
+    }
+    const bool split = !g.slices && pl.splits > 1;
+    if (split) {
+        const uint64_t size[3] = {(uint64_t)pl.bn, (uint64_t)p.tail * p.splits * rows, 1};
+        const uint64_t stride[2] = {(uint64_t)pl.bn * 4, (uint64_t)pl.bn * 4 * size[1]};
+        const uint32_t box[3] = {32, 32, 1};
+        if (int rc = encode_map(&p.part, PCB_F32, g.partial, 3, size, stride, box)) return rc;
     }
     int rc;
-    if (g.epi == EPI_LSE) rc = launch<EPI_LSE, 0>(pl, p, s);
-    else if (g.epi == EPI_DL) rc = launch<EPI_DL, 0>(pl, p, s);
-    else if (g.epi == EPI_DZ) rc = p.act.kind == PCB_ACT_GELU ? launch<EPI_DZ, PCB_ACT_GELU>(pl, p, s) : launch<EPI_DZ, PCB_ACT_POLY>(pl, p, s);
-    else if (p.act.kind == PCB_ACT_GELU) rc = launch<EPI_STORE, PCB_ACT_GELU>(pl, p, s);
-    else if (p.act.kind == PCB_ACT_POLY) rc = launch<EPI_STORE, PCB_ACT_POLY>(pl, p, s);
-    else rc = launch<EPI_STORE, PCB_ACT_NONE>(pl, p, s);
-    if (rc || pl.splits == 1) return rc;
-    const int64_t blocks = ((int64_t)g.m * g.n + 255) / 256;
-    launch_pdl(join, dim3((unsigned)(blocks < 8 * SMS ? blocks : 8 * SMS)), dim3(256), s, (const float*)g.partial, pl.splits, fin);
+    const int act = p.act.kind;
+    if (g.epi == EPI_LSE) rc = launch<KERNEL_LSE, 0>(pl, p, s);
+    else if (g.epi == EPI_DL) rc = launch<KERNEL_DL, 0>(pl, p, s);
+    else if (g.epi == EPI_DZ) rc = act == PCB_ACT_GELU ? launch<KERNEL_DZ, PCB_ACT_GELU>(pl, p, s) : launch<KERNEL_DZ, PCB_ACT_POLY>(pl, p, s);
+    else if (p.extra)
+        rc = act == PCB_ACT_GELU   ? launch<KERNEL_ADD, PCB_ACT_GELU>(pl, p, s)
+             : act == PCB_ACT_POLY ? launch<KERNEL_ADD, PCB_ACT_POLY>(pl, p, s)
+                                   : launch<KERNEL_ADD, PCB_ACT_NONE>(pl, p, s);
+    else
+        rc = act == PCB_ACT_GELU   ? launch<KERNEL_STORE, PCB_ACT_GELU>(pl, p, s)
+             : act == PCB_ACT_POLY ? launch<KERNEL_STORE, PCB_ACT_POLY>(pl, p, s)
+                                   : launch<KERNEL_STORE, PCB_ACT_NONE>(pl, p, s);
+    if (rc || !split) return rc;
+    launch_pdl(join, dim3((unsigned)(p.tail * (rows / JOIN_ROWS))), dim3(256), s, (const float*)g.partial, pl.bn, rows, p);
     return PCB_LAUNCH_RESULT();
 }
 
@@ -707,14 +850,22 @@ size_t aligned_bytes(const void* p, int64_t pitch, int64_t rows, int64_t cols) {
     if (((uintptr_t)p & 15) == 0 && pitch % 8 == 0) return 0;
     return (size_t)rows * ((cols + 7) / 8 * 8) * 2;
 }
-int align_rows(const void** p, int64_t* pitch, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
-    if (!aligned_bytes(*p, *pitch, rows, cols)) return 0;
-    const int64_t np = (cols + 7) / 8 * 8;
-    const int64_t blocks = (rows * np + 255) / 256;
-    launch_pdl(copy_rows, dim3((unsigned)(blocks < 16 * SMS ? blocks : 16 * SMS)), dim3(256), s, (const uint16_t*)*p, *pitch, rows,
-               (int)cols, (uint16_t*)to, np);
-    *p = to;
-    *pitch = np;
+int align_rows(const Rows* r, int n, cudaStream_t s) {
+    CopyJobs j;
+    memset(&j, 0, sizeof j);
+    int jobs = 0;
+    int64_t most = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!aligned_bytes(*r[i].p, *r[i].pitch, r[i].rows, r[i].cols)) continue;
+        const int64_t to = (r[i].cols + 7) / 8 * 8;
+        j.x[jobs] = (const uint16_t*)*r[i].p, j.y[jobs] = (uint32_t*)r[i].to, j.pitch[jobs] = *r[i].pitch;
+        j.rows[jobs] = r[i].rows, j.cols[jobs] = (int)r[i].cols, j.to[jobs] = (int)to;
+        most = std::max(most, r[i].rows);
+        *r[i].p = r[i].to, *r[i].pitch = to;
+        ++jobs;
+    }
+    if (!jobs) return 0;
+    launch_pdl(copy_rows, dim3((unsigned)std::min<int64_t>((most + 7) / 8, 8 * SMS), jobs), dim3(256), s, j);
     return PCB_LAUNCH_RESULT();
 }
 

@@ -35,8 +35,8 @@ struct Gemm {
     void* y;
     int64_t y_pitch;
     int y_type;
-    bool accumulate;  // EPI_STORE in 32 bits: y += (one writer per element)
-    bool whole;       // EPI_STORE: k is not split (as under accumulate)
+    int slices;       // EPI_STORE into 32 bits: > 0: k in this many parts, part i's sums at y + i m y_pitch
+    bool accumulate;  // with slices: y += (one writer per element; a part without k is left as it is)
     Act act;
     const void* bias;
     int bias_type;
@@ -50,19 +50,29 @@ struct Gemm {
     const int64_t* targets; // EPI_LSE
     float2* parts;          // EPI_LSE: [vocab_parts(n)][m] (maximum in base 2, sum)
     float* hit;             // EPI_LSE: [m], written where the target lies in this product's columns
-    float* partial;         // workspace of gemm_partial() values (null when that is 0)
+    float* partial;         // EPI_STORE: workspace of gemm_partial() values; null: no splitting
 };
 
-// 32-bit values of workspace that an EPI_STORE product wants (it splits a long k over the SMs when there are few tiles)
+// 32-bit values of workspace that an EPI_STORE product wants (the tiles of its last, partly filled round over the SMs split
+// their k), and the estimated time of a product in nanoseconds
 size_t gemm_partial(int m, int n, int k);
+double gemm_cost(int m, int n, int k, bool may_split);
+// parts of k that fill the SMs for an m x n product (for `slices`)
+int gemm_slices(int m, int n, int k);
 int gemm(const Gemm& g, cudaStream_t s);
 // column blocks of an EPI_LSE product over n columns
 int vocab_parts(int m, int n);
 
 // An operand as the TMA engine can read it: first element and pitch on 16 bytes, as it lies or copied to `to` (null when
 // only counting). aligned_bytes: the copy's size, 0 where none is needed.
+struct Rows {
+    const void** p;
+    int64_t* pitch;
+    int64_t rows, cols;
+    void* to;
+};
 size_t aligned_bytes(const void* p, int64_t pitch, int64_t rows, int64_t cols);
-int align_rows(const void** p, int64_t* pitch, int64_t rows, int64_t cols, void* to, cudaStream_t s);
+int align_rows(const Rows* r, int n, cudaStream_t s);  // n <= 3, one launch
 
 unsigned int gemm_timeouts();
 
