@@ -10,31 +10,56 @@ namespace pcb {
 namespace clear {
 
 // ------------------------------------------------------------------------------------------------ column sums
-// Sums over the rows of a matrix, in two launches of fixed order: 256 rows of 32 columns per block (a warp along the
-// columns, eight row lanes joined in shared memory), then the blocks' sums the same way.
+// Sums over the rows of a matrix, in two launches of fixed order: 256 rows of 64 columns per block (a warp along the columns,
+// two per lane, eight row lanes joined in shared memory), then the blocks' sums the same way. The first may run beside the
+// product launched before it, from which it reads nothing (`beside`): it then waits for that one only before it ends.
 constexpr int SUM_ROWS = 256;
 __global__ void __launch_bounds__(256) sum_rows(const void* x, int64_t pitch, int type, int m, int n, int rows, float* part, void* out,
-                                                int out_type) {
-    __shared__ float red[8][32];
-    pdl_wait();
+                                                int out_type, bool beside) {
+    __shared__ float2 red[8][32];
+    if (!beside) pdl_wait();
     pdl_release();
     const int c = threadIdx.x % 32, r = threadIdx.x / 32;
-    const int64_t col = blockIdx.x * 32ll + c, r0 = (int64_t)blockIdx.y * rows, r1 = min((int64_t)m, r0 + rows);
-    float s = 0.0f;
-    if (col < n) {
+    const int64_t col = blockIdx.x * 64ll + 2 * c, r0 = (int64_t)blockIdx.y * rows, r1 = min((int64_t)m, r0 + rows);
+    float2 s = make_float2(0.0f, 0.0f);
+    const bool wide = type == PCB_F32, pairs = pitch % 2 == 0 && ((uintptr_t)x & (wide ? 7 : 3)) == 0 && col + 1 < n;
+    if (pairs && wide) {
 #pragma unroll 8
-        for (int64_t i = r0 + r; i < r1; i += 8) s += load(x, i * pitch + col, type);
+        for (int64_t i = r0 + r; i < r1; i += 8) {
+            const float2 v = *(const float2*)((const float*)x + i * pitch + col);
+            s.x += v.x, s.y += v.y;
+        }
+    } else if (pairs) {
+#pragma unroll 8
+        for (int64_t i = r0 + r; i < r1; i += 8) {
+            const uint32_t w = *(const uint32_t*)((const uint16_t*)x + i * pitch + col);
+            float2 v;
+            if (type == PCB_BF16) v = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+            else v = __half22float2(*(const __half2*)&w);
+            s.x += v.x, s.y += v.y;
+        }
+    } else {
+#pragma unroll 4
+        for (int64_t i = r0 + r; i < r1; i += 8) {
+            if (col < n) s.x += load(x, i * pitch + col, type);
+            if (col + 1 < n) s.y += load(x, i * pitch + col + 1, type);
+        }
     }
     red[r][c] = s;
     __syncthreads();
-    if (r || col >= n) return;
-    for (int i = 1; i < 8; ++i) s += red[i][c];
-    if (part) part[(int64_t)blockIdx.y * n + col] = s;
-    else store(out, col, out_type, s);
+    if (r == 0) {
+        for (int i = 1; i < 8; ++i) s.x += red[i][c].x, s.y += red[i][c].y;
+        for (int e = 0; e < 2; ++e)
+            if (col + e < n) {
+                if (part) part[(int64_t)blockIdx.y * n + col + e] = e ? s.y : s.x;
+                else store(out, col + e, out_type, e ? s.y : s.x);
+            }
+    }
+    if (beside) pdl_wait();  // later launches may rely on everything before this one
 }
-int run_sum(const void* x, int64_t pitch, int type, int m, int n, float* part, void* out, int out_type, cudaStream_t s) {
-    const dim3 g((n + 31) / 32, part ? (m + SUM_ROWS - 1) / SUM_ROWS : 1);
-    launch_pdl(sum_rows, g, dim3(256), s, x, pitch, type, m, n, part ? SUM_ROWS : m, part, out, out_type);
+int run_sum(const void* x, int64_t pitch, int type, int m, int n, float* part, void* out, int out_type, bool beside, cudaStream_t s) {
+    const dim3 g((n + 63) / 64, part ? (m + SUM_ROWS - 1) / SUM_ROWS : 1);
+    launch_pdl(sum_rows, g, dim3(256), s, x, pitch, type, m, n, part ? SUM_ROWS : m, part, out, out_type, beside);
     return PCB_LAUNCH_RESULT();
 }
 
@@ -51,34 +76,36 @@ int run_zero(void* y, int64_t rows, int64_t cols, int64_t pitch, int type, cudaS
 }
 
 // ------------------------------------------------------------------------------------------------ vocabulary
-// lse and loss from the column blocks' maxima (base 2) and sums: 32 rows per block, 32 lanes over the column blocks
+// A maximum (base 2) and a sum of exponentials below it, joined with another. A side without terms, or whose terms are all
+// -inf, adds nothing; NaN goes through the sum.
+__device__ __forceinline__ float2 join_lse(float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    const float fa = a.x == -INFINITY ? (a.y == a.y ? 0.0f : a.y) : a.y * exp2f(a.x - top);
+    const float fb = b.x == -INFINITY ? (b.y == b.y ? 0.0f : b.y) : b.y * exp2f(b.x - top);
+    return make_float2(top, fa + fb);
+}
+// lse and loss from the column blocks' maxima and sums: 8 rows per block, 128 lanes over the column blocks (few rows against a
+// large vocabulary are all latency: 16 rows against 50000 took 5 us of 28 with 32 lanes)
 __global__ void __launch_bounds__(1024) join_parts(const float2* part, int nparts, const float* hit, PcbClearVocab a) {
-    __shared__ float2 red[32][33];
+    __shared__ float2 red[32][8];
     pdl_wait();
     pdl_release();
-    const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-    const int64_t row = blockIdx.x * 32ll + x;
-    float top = -INFINITY, sum = 0.0f;
+    const int x = threadIdx.x % 8, y = threadIdx.x / 8, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t row = blockIdx.x * 8ll + x;
+    float2 v = make_float2(-INFINITY, 0.0f);
     if (row < a.rows) {
 #pragma unroll 4
-        for (int i = y; i < nparts; i += 32) {
-            const float2 v = part[(int64_t)i * a.rows + row];
-            const float nt = fmaxf(top, v.x);
-            // a column block whose logits are all -inf, or none, adds nothing; NaN goes through the sum
-            sum = (top == -INFINITY ? 0.0f : sum * exp2f(top - nt)) + (v.x == -INFINITY ? (v.y == v.y ? 0.0f : v.y) : v.y * exp2f(v.x - nt));
-            top = nt;
-        }
+        for (int i = y; i < nparts; i += 128) v = join_lse(v, part[(int64_t)i * a.rows + row]);
     }
-    red[y][x] = make_float2(top, sum);
+    for (int w = 8; w < 32; w *= 2) v = join_lse(v, make_float2(__shfl_xor_sync(~0u, v.x, w), __shfl_xor_sync(~0u, v.y, w)));
+    if (lane < 8) red[warp][lane] = v;
     __syncthreads();
-    if (y || row >= a.rows) return;
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, red[i][x].x);
-    sum = 0.0f;
-    for (int i = 0; i < 32; ++i) {
-        const float2 v = red[i][x];
-        sum += v.x == -INFINITY ? (v.y == v.y ? 0.0f : v.y) : v.y * exp2f(v.x - top);
-    }
-    const float lse = (top + log2f(sum)) * 0.69314718055994531f;
+    if (warp) return;
+    v = red[lane / 8][x];
+    for (int i = 4 + lane / 8; i < 32; i += 4) v = join_lse(v, red[i][x]);
+    for (int w = 8; w < 32; w *= 2) v = join_lse(v, make_float2(__shfl_xor_sync(~0u, v.x, w), __shfl_xor_sync(~0u, v.y, w)));
+    if (lane >= 8 || row >= a.rows) return;
+    const float lse = (v.x + log2f(v.y)) * 0.69314718055994531f;
     const int64_t t = a.targets[row];
     a.lse[row] = lse;
     a.loss[row] = t == a.ignore ? 0.0f : t >= 0 && t < a.vocab ? lse - hit[row] : NAN;
@@ -302,17 +329,16 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
         if (int rc = gemm(g, s)) return rc;
         dz = Operand{w.dz, w.dz_pitch, true};
         if (a->db)
-            if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + 31) / 32, a->n, nullptr, a->db, a->db_type, s)) return rc;
-    } else {
-        if (a->db) {
-            if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, w.sums, nullptr, 0, s)) return rc;
-            if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, s)) return rc;
-        }
+            if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + 31) / 32, a->n, nullptr, a->db, a->db_type, false, s)) return rc;
     }
     if (a->dx) {
         Gemm g = product_of(dz, Operand{wt.p, wt.pitch, a->w_cols == 0}, a->m, a->k, a->n, a->type);
         g.y = a->dx, g.y_pitch = a->dx_pitch, g.partial = w.partial;
         if (int rc = gemm(g, s)) return rc;
+    }
+    if (a->db && !a->act) {  // beside the product before it, if there is one
+        if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, w.sums, nullptr, 0, a->dx != nullptr, s)) return rc;
+        if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, false, s)) return rc;
     }
     if (!a->dw) return 0;
     const Operand xr{x.p, x.pitch, false}, dr{dz.p, dz.pitch, false};
@@ -338,7 +364,7 @@ int pcb_clear_vocab_loss(const PcbClearVocab* a, void* ws, size_t ws_bytes, cuda
     g.epi = EPI_LSE;
     g.targets = a->targets, g.parts = w.parts, g.hit = w.hit;
     if (int rc = gemm(g, s)) return rc;
-    launch_pdl(join_parts, dim3((a->rows + 31) / 32), dim3(1024), s, (const float2*)w.parts, vocab_parts(a->rows, a->vocab),
+    launch_pdl(join_parts, dim3((a->rows + 7) / 8), dim3(1024), s, (const float2*)w.parts, vocab_parts(a->rows, a->vocab),
                (const float*)w.hit, *a);
     return PCB_LAUNCH_RESULT();
 }

@@ -380,7 +380,6 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                 const int64_t at = p.targets[row] - first;
                 target = at >= 0 && at < S::COLS ? (int)at : -1;
             }
-            uint32_t held[16];
             auto put_wide = [&](const float* v) {  // the lane's 32 values into the staging buffer
                 if (lane == 0) bulk_wait_read();
                 __syncwarp();
@@ -508,35 +507,29 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                         for (int j = 0; j < 32; ++j) v[j] = target == 32 * c + j ? v[j] - weight : v[j];
                     }
                 }
-                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
-                // 64 columns of 16 bits fill it (the first 32 wait in registers: the buffer also serves `extra`)
-                const bool narrow = p.y_type != PCB_F32;
-                uint32_t now[16];
-                if (narrow) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) now[j] = pack2(v[2 * j], v[2 * j + 1], p.y_type == PCB_BF16);
-                }
                 if (EPI == KERNEL_DZ && p.row_sums) {
-                    const float s = lane_sums(v);
+                    float t32[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) t32[j] = v[j];
+                    const float s = lane_sums(t32);
                     if (col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
                 }
-                if (narrow && c % 2 == 0 && c + 1 < chunks) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) held[j] = now[j];
-                    continue;
-                }
+                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
+                // 64 columns of 16 bits fill it
+                const bool narrow = p.y_type != PCB_F32;
                 if (narrow) {
-                    if (lane == 0) bulk_wait_read();
-                    __syncwarp();
-                    uint4* srow = (uint4*)(stage + lane * 128);
-                    if (c % 2) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            srow[j ^ (lane & 7)] = make_uint4(held[4 * j], held[4 * j + 1], held[4 * j + 2], held[4 * j + 3]);
+                    if (c % 2 == 0) {
+                        if (lane == 0) bulk_wait_read();
+                        __syncwarp();
                     }
+                    uint4* srow = (uint4*)(stage + lane * 128);
+                    const bool bf16 = p.y_type == PCB_BF16;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        srow[(j + (c % 2) * 4) ^ (lane & 7)] = make_uint4(now[4 * j], now[4 * j + 1], now[4 * j + 2], now[4 * j + 3]);
+                        srow[(j + (c % 2) * 4) ^ (lane & 7)] =
+                            make_uint4(pack2(v[8 * j], v[8 * j + 1], bf16), pack2(v[8 * j + 2], v[8 * j + 3], bf16),
+                                       pack2(v[8 * j + 4], v[8 * j + 5], bf16), pack2(v[8 * j + 6], v[8 * j + 7], bf16));
+                    if (c % 2 == 0 && c + 1 < chunks) continue;
                     fence_async_smem();
                     __syncwarp();
                 } else {
