@@ -363,8 +363,11 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             const int m0 = (w.tile % p.tiles_m * CTAS + rank) * BM, tn = w.tile / p.tiles_m, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
             auto bias_of = [&](int col) { return col + lane < p.n ? load(p.bias, col + lane, p.bias_type) : 0.0f; };
-            float next_bias = 0.0f;
-            if (AFFINE && p.bias && !w.partial) next_bias = bias_of(first);
+            float biases[S::COLS / 32];  // the lane's column of each 32, read while the products still run
+            if (AFFINE && p.bias && !w.partial) {
+#pragma unroll
+                for (int i = 0; i < S::COLS / 32; ++i) biases[i] = bias_of(first + 32 * i);
+            }
             if (!wait_warp<true>(&acc_full[buf], (t / 2) & 1, dead, &g_gemm_timeouts)) break;
             ++t;
             fence_after();
@@ -437,9 +440,11 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                 if (AFFINE) {
                     if (p.bias) {
                         __syncwarp();
-                        bias[lane] = next_bias;
+                        float b = biases[0];
+#pragma unroll
+                        for (int i = 1; i < S::COLS / 32; ++i) b = c == i ? biases[i] : b;
+                        bias[lane] = b;
                         __syncwarp();
-                        if (c + 1 < chunks) next_bias = bias_of(col0 + 32);
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 q = *(const float4*)(bias + j);
