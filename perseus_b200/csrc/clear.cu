@@ -13,7 +13,7 @@ namespace clear {
 // Sums over the rows of a matrix, in two launches of fixed order: 256 rows of 64 columns per block (a warp along the columns,
 // two per lane, eight row lanes joined in shared memory), then the blocks' sums the same way. The first may run beside the
 // product launched before it, from which it reads nothing (`beside`): it then waits for that one only before it ends.
-constexpr int SUM_ROWS = 256;
+constexpr int SUM_ROWS = 256, SUM_ONCE = 1024;  // up to SUM_ONCE rows one launch does: beside a product it costs no time
 __global__ void __launch_bounds__(256) sum_rows(const void* x, int64_t pitch, int type, int m, int n, int rows, float* part, void* out,
                                                 int out_type, bool beside) {
     __shared__ float2 red[8][32];
@@ -337,8 +337,10 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
         if (int rc = gemm(g, s)) return rc;
     }
     if (a->db && !a->act) {  // beside the product before it, if there is one
-        if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, w.sums, nullptr, 0, a->dx != nullptr, s)) return rc;
-        if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, false, s)) return rc;
+        const bool once = a->m <= SUM_ONCE;
+        if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, once ? nullptr : w.sums, a->db, a->db_type, a->dx != nullptr, s)) return rc;
+        if (!once)
+            if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, false, s)) return rc;
     }
     if (!a->dw) return 0;
     const Operand xr{x.p, x.pitch, false}, dr{dz.p, dz.pitch, false};

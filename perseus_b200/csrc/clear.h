@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -136,6 +137,19 @@ inline int bad_vocab_grad(const PcbClearVocabGrad* a) {
     if ((a->dh && a->dh_pitch < a->v.dim) || (a->dw && a->dw_pitch < a->v.dim))
         return report(PCB_BAD_ARGS, "clear_vocab_grad: a pitch is below its row's elements");
     return 0;
+}
+
+// ------------------------------------------------------------------------------------------------ launching
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once per device (`done`: the kernel's own)
+inline int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return (int)e;
 }
 
 // ------------------------------------------------------------------------------------------------ workspace

@@ -569,8 +569,8 @@ template <int DP, bool POLY>
 int launch(const Params& p, int64_t blocks, cudaStream_t s) {
     using S = Shape<DP>;
     static_assert(2 * (S::SMEM + 1024) <= 233472, "two blocks per SM");
-    static const cudaError_t set = cudaFuncSetAttribute(attend<DP, POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
-    if (set != cudaSuccess) return (int)set;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_smem((const void*)attend<DP, POLY>, S::SMEM, done)) return rc;
     launch_pdl_smem(attend<DP, POLY>, dim3((unsigned)blocks), dim3(THREADS), S::SMEM, s, p);
     return PCB_LAUNCH_RESULT();
 }

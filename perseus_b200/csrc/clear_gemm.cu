@@ -731,8 +731,8 @@ template <int BN, int CTAS, int EPI, int ACT>
 int launch(const Params& p, cudaStream_t s) {
     using S = Shape<BN, CTAS, EPI>;
     static_assert(S::SMEM <= 232448, "shared memory");
-    static const cudaError_t set = cudaFuncSetAttribute(product<BN, CTAS, EPI, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
-    if (set != cudaSuccess) return (int)set;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_smem((const void*)product<BN, CTAS, EPI, ACT>, S::SMEM, done)) return rc;
     const int64_t units = (int64_t)p.whole + (int64_t)p.tail * p.splits, slots = SMS / CTAS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * CTAS));
@@ -845,7 +845,7 @@ int gemm(const Gemm& g, cudaStream_t s) {
 }
 
 size_t aligned_bytes(const void* p, int64_t pitch, int64_t rows, int64_t cols) {
-    if (((uintptr_t)p & 15) == 0 && pitch % 8 == 0) return 0;
+    if (((uintptr_t)p & 15) == 0 && pitch % 8 == 0 && pitch < (1ll << 38)) return 0;  // a map's strides are below 2^40 bytes
     return (size_t)rows * ((cols + 7) / 8 * 8) * 2;
 }
 int align_rows(const Rows* r, int n, cudaStream_t s) {

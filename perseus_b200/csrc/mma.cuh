@@ -90,7 +90,9 @@ __device__ __forceinline__ bool peek(uint64_t* bar, uint32_t parity) {
 }
 // A bounded wait of a whole warp that also gives up when another role of the block has (`dead`, shared memory): false then,
 // and counted. RELAXED waits (for a tile's worth of work, not for the next block) poll from one lane and sleep in between,
-// so that the epilogue's warps leave the barriers' unit to the warps that feed the products.
+// so that the epilogue's warps leave the barriers' unit to the warps that feed the products; their limit leaves a tile some
+// seconds (k may be millions).
+constexpr uint32_t RELAXED_WAIT_LIMIT = 1u << 27;
 template <bool RELAXED = false>
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned int* timeouts) {
     bool ok = true;
@@ -101,7 +103,7 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
                 ok = false;
                 break;
             }
-            if (it >= MBAR_WAIT_LIMIT) {
+            if (it >= (RELAXED ? RELAXED_WAIT_LIMIT : MBAR_WAIT_LIMIT)) {
                 *dead = 1;
                 atomicAdd(timeouts, 1u);
                 ok = false;

@@ -162,6 +162,37 @@ def test_linear_is_the_same_every_time():
         assert all(torch.equal(a, b) for a, b in zip(one, clear.linear_grad(dy, x, w, bias=rnd(4, 384), act="gelu")))
 
 
+def test_linear_far_offsets():
+    """Inputs and results past 2^31 elements."""
+    m, n = 1_500_000, 200
+    x = torch.zeros(m, 1536, dtype=BF, device="cuda")
+    x[-n:] = rnd(1, n, 1536)
+    w = rnd(2, 1536, 8, std=0.03)
+    y = clear.linear(x, w)
+    assert not y[:-n].any()
+    R.close(y[-n:], R.linear(x[-n:], w, None, None, None, BF))
+    dx, dw, _ = clear.linear_grad(y, x, w)
+    want = R.linear_grad(y[-n:], x[-n:], w, None, None, BF)
+    R.close(dx[-n:], want[0])
+    R.close(dw, want[1])
+    del x, y, dx
+    x = torch.zeros(m, 64, dtype=BF, device="cuda")
+    x[-n:] = rnd(3, n, 64)
+    w, b = rnd(4, 64, 1536, std=0.1), rnd(5, 1536, dtype=F32)
+    y = clear.linear(x, w, bias=b, act="gelu")
+    R.close(y[-n:], R.linear(x[-n:], w, b, "gelu", None, BF))
+    R.close(y[:n], R.linear(x[:n], w, b, "gelu", None, BF))
+
+
+def test_linear_grad_long_sums():
+    """Sums over many rows, some thousands of 64-row blocks, split and not."""
+    x, dy, w = rnd(1, 300_001, 72), rnd(2, 300_001, 136), rnd(3, 72, 136, std=0.1)
+    for act in (None, GELU_POLY):
+        for got, want in zip(clear.linear_grad(dy, x, w, bias=rnd(4, 136, dtype=F32), act=act),
+                             R.linear_grad(dy, x, w, rnd(4, 136, dtype=F32), act, F32)):
+            R.close(got, want)
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def attend(q_lens, k_lens, heads, kv, dim, dtype=BF, weights=None, causal=True, std=1.0, scale=None, seed=0):
     q = rnd(seed + 1, sum(q_lens), heads, dim, std=std, dtype=dtype)
@@ -266,6 +297,31 @@ def test_attention_masked_keys_stay_out(weights, bad):
     got = clear.prompt_attention(q, k, v, [200], weights=weights)
     R.close(got[:bad], (want[0][:bad], want[1][:bad]))
     assert not torch.isfinite(got[bad]).any()
+
+
+def test_attention_split_keys_not_finite():
+    """Few queries against many keys, which are split over blocks: a key that only the last query sees."""
+    n = 5000
+    q, k, v = rnd(1, 2, 4, 64, std=0.5), rnd(2, n, 2, 64, std=0.5), rnd(3, n, 2, 64)
+    want = R.attention(q, k, v, [2], [n], 0.125, True, None)
+    v[n - 1] = math.inf
+    got = clear.prompt_attention(q, k, v, [2], [n])
+    R.close(got[:1], (want[0][:1], want[1][:1]))
+    assert not torch.isfinite(got[1]).any()
+    k[n - 1] = math.nan
+    got = clear.prompt_attention(q, k, v, [2], [n])
+    R.close(got[:1], (want[0][:1], want[1][:1]))
+    assert torch.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_is_the_same_every_time(dim):
+    lens = [1300, 7, 900, 2100]
+    q, k, v = rnd(1, sum(lens), 6, dim), rnd(2, sum(lens), 2, dim), rnd(3, sum(lens), 2, dim)
+    one = clear.prompt_attention(q, k, v, lens)
+    R.close(one, R.attention(q, k, v, lens, lens, dim**-0.5, True, None))
+    for _ in range(20):
+        assert torch.equal(clear.prompt_attention(q, k, v, lens), one)
 
 
 def test_attention_far_offsets():
@@ -410,6 +466,33 @@ def test_vocab_nonfinite_row():
     R.close(loss[rows], tuple(x[rows] for x in want[0]))
     dh, _ = clear.vocab_loss_grad(h, w, t, lse, weight)
     R.close(dh[rows], tuple(x[rows] for x in want[2]))
+
+
+def test_vocab_far_offsets():
+    """A vocabulary past 2^31 elements: zeros but for its last entries."""
+    vocab, dim, n = 2_900_000, 768, 64
+    w = torch.zeros(vocab, dim, dtype=BF, device="cuda")
+    w[-n:] = rnd(1, n, dim, std=0.1)
+    h = rnd(2, 5, dim)
+    t = torch.tensor([vocab - 1, 0, vocab - n, -100, vocab - 2], device="cuda")
+    loss, lse = clear.vocab_loss(h, w, t)
+    lg = h.double() @ w[-n:].double().t()
+    want = torch.log(vocab - n + torch.exp(lg).sum(1))
+    hit = torch.zeros(5, dtype=torch.float64, device="cuda")
+    hit[0], hit[2], hit[4] = lg[0, -1], lg[2, 0], lg[4, -2]
+    # a sum of 2.9e6 ones in blocks of 128 and their joining, and the logits' error
+    err = (dim + 4) * R.S * (h.double().abs() @ w[-n:].double().abs().t()).amax(1) + 2.0**-16
+    R.close(lse, (want, err))
+    R.close(loss, (torch.where(t == -100, 0.0, want - hit), 2 * err))
+    weight = torch.full((5,), 0.25, device="cuda")
+    dh, dw = clear.vocab_loss_grad(h, w, t, lse, weight)
+    p = torch.exp(lg - want[:, None])
+    hot = torch.zeros(5, n, dtype=torch.float64, device="cuda")
+    hot[0, -1] = hot[2, 0] = hot[4, -2] = 1.0
+    d = (p - hot) * torch.where(t == -100, 0.0, 0.25).double()[:, None]
+    ed = 2 * err[:, None] * p * 0.25 + R.U[BF] * d.abs() + 2.0**-133
+    R.close(dh, (d @ w[-n:].double(), ed @ w[-n:].double().abs() + (n + 4) * R.S * (d.abs() @ w[-n:].double().abs()) + R.U[BF] * (d @ w[-n:].double()).abs() + 2.0**-133))
+    R.close(dw[-n:], (d.t() @ h.double(), ed.t() @ h.double().abs() + 9 * R.S * (d.abs().t() @ h.double().abs()) + R.U[BF] * (d.t() @ h.double()).abs() + 2.0**-133))
 
 
 def test_vocab_is_the_same_every_time():
