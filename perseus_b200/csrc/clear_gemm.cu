@@ -132,11 +132,12 @@ __device__ __forceinline__ f32x2 act2(const Act& a, f32x2 z) {
     return z;
 }
 
-// Sum over the warp's lanes of each of 32 values: lane l returns the sum of v[l], in a fixed order
+// Sum over the warp's lanes of each of N values, in a fixed order: lane l returns the sum of v[l % N]
+template <int N>
 __device__ __forceinline__ float lane_sums(float* v) {
     const int lane = threadIdx.x % 32;
 #pragma unroll
-    for (int w = 16; w; w >>= 1) {
+    for (int w = N / 2; w; w >>= 1) {
         const bool up = lane & w;
 #pragma unroll
         for (int j = 0; j < w; ++j) {
@@ -144,6 +145,8 @@ __device__ __forceinline__ float lane_sums(float* v) {
             v[j] = keep + __shfl_xor_sync(~0u, give, w);
         }
     }
+#pragma unroll
+    for (int w = N; w < 32; w <<= 1) v[0] += __shfl_xor_sync(~0u, v[0], w);
     return v[0];
 }
 
@@ -332,6 +335,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             else mbar_arrive(&acc_empty[buf]);
         };
         // the boxes of `extra` in the order that they are used: box e of a tile covers columns [e ecols, ...) of the warp's
+        constexpr int W = 32;  // columns at a time (16: 5 to 15 % slower)
         constexpr bool HAS_EXTRA = S::BUFFERS == 2, AFFINE = HAS_EXTRA || EPI == KERNEL_STORE;
         const bool extra_wide = p.extra_mode != EXTRA_TMA || p.extra_type == PCB_F32;
         const int ecols = extra_wide ? 32 : 64;
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             ++t;
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
-            const int chunks = min(S::COLS / 32, max(0, (p.n - first + 31) / 32));
+            const int chunks = min(S::COLS / W, max(0, (p.n - first + W - 1) / W));
             float top = -INFINITY, sum = 0.0f, lse2 = 0.0f, weight = 0.0f;
             int target = -1;  // the row's column among this warp's, if it is there
             if (EPI == KERNEL_DL && row < p.m) {
@@ -383,41 +387,30 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                 const int64_t at = p.targets[row] - first;
                 target = at >= 0 && at < S::COLS ? (int)at : -1;
             }
-            auto put_wide = [&](const float* v) {  // the lane's 32 values into the staging buffer
-                if (lane == 0) bulk_wait_read();
-                __syncwarp();
-                uint4* srow = (uint4*)(stage + lane * 128);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    srow[j ^ (lane & 7)] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                      __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-                fence_async_smem();
-                __syncwarp();
-            };
             for (int c = 0; c < chunks; ++c) {
-                const int col0 = first + 32 * c;
-                float v[32];
-                tmem_ld32(acc + 32 * c, v);
+                const int col0 = first + W * c;
+                float v[W];
+                tmem_ld32(acc + W * c, v);
                 ld_wait();
                 if (c == chunks - 1) release(buf);
-                const bool has_target = (EPI == KERNEL_LSE || EPI == KERNEL_DL) && __any_sync(~0u, (unsigned)(target - 32 * c) < 32u);
+                const bool has_target = (EPI == KERNEL_LSE || EPI == KERNEL_DL) && __any_sync(~0u, (unsigned)(target - W * c) < (unsigned)W);
                 if (EPI == KERNEL_LSE) {
                     if (has_target) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (target == 32 * c + j && col0 + j < p.n) p.hit[row] = v[j];
+                        for (int j = 0; j < W; ++j)
+                            if (target == W * c + j && col0 + j < p.n) p.hit[row] = v[j];
                     }
-                    if (col0 + 32 > p.n) {
+                    if (col0 + W > p.n) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = col0 + j < p.n ? v[j] : -INFINITY;
+                        for (int j = 0; j < W; ++j) v[j] = col0 + j < p.n ? v[j] : -INFINITY;
                     }
                     float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int j = 4; j < 32; ++j) m4[j % 4] = fmaxf(m4[j % 4], v[j]);
+                    for (int j = 4; j < W; ++j) m4[j % 4] = fmaxf(m4[j % 4], v[j]);
                     const float nt = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * LOG2E);
                     f32x2 s2[2] = {0, 0};
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int j = 0; j < W; j += 2) {
                         float a, b;
                         parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-nt)), a, b);
                         s2[j / 2 % 2] = add2(s2[j / 2 % 2], two(ex2(a), ex2(b)));
@@ -428,39 +421,34 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                     top = nt;
                     continue;
                 }
-                if (AFFINE && w.partial) {  // 32-bit sums for `join`, in tiles of their own
-                    put_wide(v);
-                    if (lane == 0 && row0 < p.m) {
-                        const int at = ((w.split * p.tail + w.tile - p.whole) * CTAS + (int)rank) * BM + quad * 32;
-                        tma_store(&p.part, half * S::COLS + 32 * c, at, 0, stage);
-                        bulk_commit();
-                    }
-                    continue;
-                }
-                if (AFFINE) {
+                const bool partial = AFFINE && w.partial;  // 32-bit sums for `join`, in tiles of their own
+                if (AFFINE && !partial) {
                     if (p.bias) {
-                        __syncwarp();
-                        float b = biases[0];
+                        if (W * c % 32 == 0) {
+                            __syncwarp();
+                            float b = biases[0];
 #pragma unroll
-                        for (int i = 1; i < S::COLS / 32; ++i) b = c == i ? biases[i] : b;
-                        bias[lane] = b;
-                        __syncwarp();
+                            for (int i = 1; i < S::COLS / 32; ++i) b = W * c / 32 == i ? biases[i] : b;
+                            bias[lane] = b;
+                            __syncwarp();
+                        }
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 q = *(const float4*)(bias + j);
+                        for (int j = 0; j < W; j += 4) {
+                            const float4 q = *(const float4*)(bias + W * c % 32 + j);
                             parts(add2(two(v[j], v[j + 1]), two(q.x, q.y)), v[j], v[j + 1]);
                             parts(add2(two(v[j + 2], v[j + 3]), two(q.z, q.w)), v[j + 2], v[j + 3]);
                         }
                     }
                     if (ACT != PCB_ACT_NONE) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) parts(act2<ACT, EPI == KERNEL_DZ>(p.act, two(v[j], v[j + 1])), v[j], v[j + 1]);
+                        for (int j = 0; j < W; j += 2) parts(act2<ACT, EPI == KERNEL_DZ>(p.act, two(v[j], v[j + 1])), v[j], v[j + 1]);
                     }
                     if constexpr (HAS_EXTRA) {
-                        if (p.extra_mode == EXTRA_LOAD) {
-                            load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, in);
-                        } else if (extra_wide || c % 2 == 0) {
-                            if (p.extra_mode == EXTRA_COPY) {
+                        const int per = ecols / W, part = c % per;  // of a box
+                        if (part == 0) {
+                            if (p.extra_mode == EXTRA_LOAD) {
+                                load_block(p.extra, p.extra_pitch, p.extra_type, row0, col0, p.m, p.n, in);
+                            } else if (p.extra_mode == EXTRA_COPY) {
                                 copy_wait();
                                 __syncwarp();
                             } else if (!wait_warp(&extra_full[ew], fetched++ & 1, dead, &g_gemm_timeouts)) {
@@ -474,15 +462,15 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                         };
                         if (extra_wide) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const uint4 q = irow[j ^ (lane & 7)];
+                            for (int j = 0; j < W / 4; ++j) {
+                                const uint4 q = irow[(j + part * (W / 4)) ^ (lane & 7)];
                                 join(4 * j, __uint_as_float(q.x), __uint_as_float(q.y));
                                 join(4 * j + 2, __uint_as_float(q.z), __uint_as_float(q.w));
                             }
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint4 q = irow[(j + (c % 2) * 4) ^ (lane & 7)];
+                            for (int j = 0; j < W / 8; ++j) {
+                                const uint4 q = irow[(j + part * (W / 8)) ^ (lane & 7)];
                                 const uint32_t x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
@@ -493,55 +481,66 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                             }
                         }
                         __syncwarp();
-                        if (extra_wide || c % 2 || c + 1 == chunks) fetch(u, extra_wide ? c + 1 : c / 2 + 1);
+                        if (part + 1 == per || c + 1 == chunks) fetch(u, c / per + 1);
                     }
                     if (EPI != KERNEL_DZ && p.alpha) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= alpha;
+                        for (int j = 0; j < W; ++j) v[j] *= alpha;
                     }
                 }
                 if (EPI == KERNEL_DL) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int j = 0; j < W; j += 2) {
                         float a, b;
                         parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-lse2)), a, b);
                         parts(mul2(two(ex2(a), ex2(b)), both(weight)), v[j], v[j + 1]);
                     }
                     if (has_target) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = target == 32 * c + j ? v[j] - weight : v[j];
+                        for (int j = 0; j < W; ++j) v[j] = target == W * c + j ? v[j] - weight : v[j];
                     }
                 }
                 if (EPI == KERNEL_DZ && p.row_sums) {
-                    float t32[32];
+                    float t[W];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) t32[j] = v[j];
-                    const float s = lane_sums(t32);
-                    if (col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
+                    for (int j = 0; j < W; ++j) t[j] = v[j];
+                    const float s = lane_sums<W>(t);
+                    if (lane < W && col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
                 }
-                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row;
-                // 64 columns of 16 bits fill it
-                const bool narrow = p.y_type != PCB_F32;
+                // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row: 64
+                // columns of 16 bits or 32 of 32 fill it
+                const bool narrow = p.y_type != PCB_F32 && !partial;
+                const int per = (narrow ? 64 : 32) / W, part = c % per;
+                if (part == 0) {
+                    if (lane == 0) bulk_wait_read();
+                    __syncwarp();
+                }
+                uint4* srow = (uint4*)(stage + lane * 128);
                 if (narrow) {
-                    if (c % 2 == 0) {
-                        if (lane == 0) bulk_wait_read();
-                        __syncwarp();
-                    }
-                    uint4* srow = (uint4*)(stage + lane * 128);
                     const bool bf16 = p.y_type == PCB_BF16;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        srow[(j + (c % 2) * 4) ^ (lane & 7)] =
+                    for (int j = 0; j < W / 8; ++j)
+                        srow[(j + part * (W / 8)) ^ (lane & 7)] =
                             make_uint4(pack2(v[8 * j], v[8 * j + 1], bf16), pack2(v[8 * j + 2], v[8 * j + 3], bf16),
                                        pack2(v[8 * j + 4], v[8 * j + 5], bf16), pack2(v[8 * j + 6], v[8 * j + 7], bf16));
-                    if (c % 2 == 0 && c + 1 < chunks) continue;
-                    fence_async_smem();
-                    __syncwarp();
                 } else {
-                    put_wide(v);
+#pragma unroll
+                    for (int j = 0; j < W / 4; ++j)
+                        srow[(j + part * (W / 4)) ^ (lane & 7)] =
+                            make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                                       __float_as_uint(v[4 * j + 3]));
                 }
-                const int box0 = narrow ? col0 - (c % 2) * 32 : col0;
-                if (p.y_tma) {
+                if (part + 1 < per && c + 1 < chunks) continue;
+                fence_async_smem();
+                __syncwarp();
+                const int box0 = col0 - part * W;
+                if (partial) {
+                    if (lane == 0 && row0 < p.m) {
+                        const int at = ((w.split * p.tail + w.tile - p.whole) * CTAS + (int)rank) * BM + quad * 32;
+                        tma_store(&p.part, box0 - n0, at, 0, stage);
+                        bulk_commit();
+                    }
+                } else if (p.y_tma) {
                     if (lane == 0 && row0 < p.m) {
                         if (p.accumulate) tma_add(&p.y, box0, row0, w.split, stage);
                         else tma_store(&p.y, box0, row0, w.split, stage);
