@@ -51,6 +51,7 @@ struct alignas(64) Params {
     CUtensorMap a, b, y, extra_map, part;
     int m, n, k;
     int a_mn, b_mn, a_panels, b_panels, bf16;
+    int stage_bytes;  // of one block's loads: fewer than the stage's where A has few rows
     int tiles_m, tiles_n, kblocks;
     // Units of work: tiles [0, whole) entire, then the other `tail` tiles in `splits` parts of `kper` k blocks: to 32-bit
     // sums that `join` finishes, or (slices) each part to its own y
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                 // a pair's loads all complete on the first block's barrier, whose warp issues the products
                 const uint32_t pair_bar = CTAS == 2 ? cluster_addr(bar, 0) : 0;
                 if (elect()) {
-                    if (rank == 0) mbar_expect(bar, CTAS * S::STAGE);
+                    if (rank == 0) mbar_expect(bar, CTAS * p.stage_bytes);
                     auto box = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
                         if (CTAS == 2) tma_load_pair(dst, map, x, y, z, pair_bar);
                         else tma_load(dst, map, x, y, z, bar);
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                 if (EPI == KERNEL_DZ && p.row_sums) {
                     float t[W];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) t[j] = v[j];
+                    for (int j = 0; j < W; ++j) t[j] = row < p.m ? v[j] : 0.0f;  // rows past the end hold anything
                     const float s = lane_sums<W>(t);
                     if (lane < W && col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
                 }
@@ -686,9 +687,10 @@ struct Tile {
     double products;  // ns of a 64-k block's
 };
 constexpr Tile TILES[] = {{256, 2, 270}, {128, 2, 150}, {128, 1, 150}, {64, 1, 120}};
-double rounds(const Tile& t, int64_t units, int kblocks) {
+int a_rows(int m) { return m < BM ? (m + 7) / 8 * 8 : BM; }  // rows of A that a tile loads: what lies past them is not used
+double rounds(const Tile& t, int m, int64_t units, int kblocks) {
     const int64_t slots = SMS / t.ctas, full = units / slots, rest = units % slots;
-    const double bytes = BM * BK * 2 + t.bn / t.ctas * BK * 2;
+    const double bytes = a_rows(m) * BK * 2 + t.bn / t.ctas * BK * 2;
     auto block = [&](int64_t active) {
         const double one = bytes / 150, all = bytes * (double)(active * t.ctas) / 12500;
         return std::max(t.products, std::max(one, all));
@@ -702,12 +704,12 @@ Plan plan(int m, int n, int k, bool may_split) {
     for (const Tile& t : TILES) {
         const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
         const int64_t tiles = tm * tn, slots = SMS / t.ctas, tail = tiles % slots, whole = tiles - tail;
-        double ns = rounds(t, tiles, kb) + (t.ctas == 2 ? 200 : 0);
+        double ns = rounds(t, m, tiles, kb) + (t.ctas == 2 ? 200 : 0);
         if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)tiles, 1, kb, ns};
         for (int sp = 2; may_split && tail && sp <= 16; ++sp) {
             const int per = (kb + sp - 1) / sp;
             if (per < 4 || (sp - 1) * per >= kb) continue;
-            ns = rounds(t, whole, kb) + rounds(t, tail * sp, per) + (t.ctas == 2 ? 200 : 0) + 3500 +
+            ns = rounds(t, m, whole, kb) + rounds(t, m, tail * sp, per) + (t.ctas == 2 ? 200 : 0) + 3500 +
                  (double)tail * BM * t.ctas * t.bn * 8 * sp / 8000;
             if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)whole, sp, per, ns};
         }
@@ -720,7 +722,7 @@ Plan plan_slices(int m, int n, int k, int slices) {
     Plan best{256, 2, 0, slices, per, 1e300};
     for (const Tile& t : TILES) {
         const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
-        const double ns = rounds(t, tm * tn * slices, per) + (t.ctas == 2 ? 200 : 0) + (double)m * n * 8 * slices / 8000;
+        const double ns = rounds(t, m, tm * tn * slices, per) + (t.ctas == 2 ? 200 : 0) + (double)m * n * 8 * slices / 8000;
         if (ns < best.ns) best = Plan{t.bn, t.ctas, 0, slices, per, ns};
     }
     return best;
@@ -788,11 +790,13 @@ int gemm(const Gemm& g, cudaStream_t s) {
     if (tm * tn * pl.splits > INT32_MAX) return report(PCB_BAD_ARGS, "a product of %d x %d outputs", g.m, g.n);
     Params p;
     memset(&p, 0, sizeof p);
-    if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, BM)) return rc;
+    const int arows = g.a.k_adjacent && pl.ctas == 1 ? a_rows(g.m) : BM;
+    if (int rc = operand_map(&p.a, g.a, g.type, g.m, g.k, arows)) return rc;
     if (int rc = operand_map(&p.b, g.b, g.type, g.n, g.k, pl.bn / pl.ctas)) return rc;
     p.m = g.m, p.n = g.n, p.k = g.k;
     p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.a_panels = panels(g.a, g.m), p.b_panels = panels(g.b, g.n);
     p.bf16 = g.type == PCB_BF16;
+    p.stage_bytes = (arows + pl.bn / pl.ctas) * BK * 2;
     p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.kblocks = (g.k + BK - 1) / BK;
     p.whole = pl.whole, p.tail = (int)(tm * tn) - pl.whole, p.splits = pl.splits, p.kper = pl.kper, p.slices = g.slices;
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;
