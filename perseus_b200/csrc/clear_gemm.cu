@@ -178,19 +178,33 @@ __device__ __noinline__ void load_block(const void* p, int64_t pitch, int type, 
     for (int r = 0; r < 32; ++r) *(float*)(to + block_at(r, lane)) = v[r];
     __syncwarp();
 }
-// A box of the staging buffer (32 rows x 128 bytes, 16-byte pieces swizzled by the row) to rows that the engine cannot write
+// A box of the staging buffer (32 rows x 128 bytes, 16-byte pieces swizzled by the row) to rows that the engine cannot write,
+// eight rows at a time
 __device__ __noinline__ void store_block(const unsigned char* stage, bool narrow, void* y, int64_t pitch, int rows, int cols, bool add) {
     const int lane = threadIdx.x % 32;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-        const unsigned char* row = stage + r * 128;
-        for (int c = lane; c < min(cols, narrow ? 64 : 32); c += 32) {
-            if (narrow) {
-                ((uint16_t*)y)[r * pitch + c] = *(const uint16_t*)(row + ((c / 8) ^ (r & 7)) * 16 + c % 8 * 2);
-            } else {
-                const float v = *(const float*)(row + ((c / 4) ^ (r & 7)) * 16 + c % 4 * 4);
-                float* at = (float*)y + r * pitch + c;
-                *at = add ? *at + v : v;
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        if (narrow) {
+            uint16_t v[2][8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = lane + 32 * h;
+                    v[h][r] = *(const uint16_t*)(stage + (r0 + r) * 128 + ((c / 8) ^ r) * 16 + c % 8 * 2);
+                }
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (r0 + r < rows && lane + 32 * h < cols) ((uint16_t*)y)[(r0 + r) * pitch + lane + 32 * h] = v[h][r];
+        } else {
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = *(const float*)(stage + block_at(r0 + r, lane));
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                float* at = (float*)y + (r0 + r) * pitch + lane;
+                if (r0 + r < rows && lane < cols) *at = add ? *at + v[r] : v[r];
             }
         }
     }
@@ -555,7 +569,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             if (chunks == 0) release(buf);
             if (EPI == KERNEL_LSE && row < p.m) p.parts[(int64_t)(tn * (S::EWARPS / 4) + half) * p.m + row] = make_float2(top, sum);
         }
-        if (lane == 0) bulk_wait();
+        if (lane == 0) bulk_wait_read();  // the staging buffer stays until it is read; the grid's end completes the writes
         if (HAS_EXTRA) {  // the box in flight, where the warp gave up
             copy_wait();
             if (*dead && p.extra_mode == EXTRA_TMA && lane == 0) mbar_wait(&extra_full[ew], fetched & 1);
