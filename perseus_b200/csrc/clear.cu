@@ -111,10 +111,10 @@ __global__ void __launch_bounds__(1024) join_parts(const float2* part, int npart
     a.loss[row] = t == a.ignore ? 0.0f : t >= 0 && t < a.vocab ? lse - hit[row] : NAN;
 }
 
-// What the gradient's pieces need of each row, and the factor that brings the largest weight to 8191 (the products, in 32
+// What the gradient's pieces need of each row, and the factor that brings the largest weight to 8192 (the products, in 32
 // bits, are scaled back): f16 slopes then keep their relative precision down to 2^-27 of the largest, and the largest ones,
-// the targets' (p - 1) weight, which are much alike, lie just below a power of two, where rounding to 16 bits errs least (a
-// power of two as the factor left them anywhere in the binade: up to twice the error)
+// the targets' (p - 1) weight, which are much alike, lie just below a power of two, where rounding to 16 bits errs least (with
+// a power of two as the factor they lay anywhere in the binade: up to twice the error)
 __global__ void __launch_bounds__(1024) prepare_rows(PcbClearVocab a, const float* weight, VocabRow* rows, float* unscale) {
     __shared__ float red[32];
     pdl_wait();
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(1024) prepare_rows(PcbClearVocab a, const floa
     __syncthreads();
     big = red[threadIdx.x % 32];
     for (int w = 16; w; w >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, w));
-    const float scale = big > 0.0f && big <= 3.4e38f ? fminf(8191.0f / big, 1e38f) : 1.0f;
+    const float scale = big > 0.0f && big <= 3.4e38f ? fminf(8192.0f / big, 1e38f) : 1.0f;
     const int64_t i = blockIdx.x * 1024ll + threadIdx.x;
     if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = 1.0f / scale;
     if (i >= a.rows) return;

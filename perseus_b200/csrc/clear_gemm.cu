@@ -1,12 +1,19 @@
-// The clear half's matrix product on the fifth-generation tensor cores.
+// The clear half's matrix product D = A B^T on the fifth-generation tensor cores, with the operators' epilogues.
 //
-// One persistent block per SM walks 128 x BN output tiles. Warp 0 streams the operands' 64-k blocks through a ring of
-// shared-memory stages with the TMA engine (either operand may have k or its rows adjacent in memory: the instruction
-// descriptor says which, nothing is transposed on the way); warp 1 issues the products (tcgen05.mma, 128 x BN x 16) into
-// one of two TMEM accumulators; the other warps take the finished accumulator out of TMEM, apply the epilogue in 32 bits
-// and store through shared memory, while the next tile's products run.
+// Persistent blocks, one per SM, walk output tiles of 256 x 256 or 256 x 128 (by pairs of blocks) or 128 x 128 or 128 x 64 (by
+// one). Warp 0 streams the operands' 64-k blocks through a ring of shared-memory stages with the TMA engine (either operand
+// may have k or its rows adjacent in memory: the instruction descriptor says which, nothing is transposed on the way); warp 1
+// issues the products (tcgen05.mma) into one of two TMEM accumulators; eight warps (four for 64 columns) take the finished
+// accumulator out of TMEM 32 columns at a time, apply the epilogue in 32 bits and store through shared memory, while the next
+// tile's products run.
 //
-// Waits are bounded (mma::wait): a role that gives up tells the others, the loads and products in flight are waited for
+// What bounds it: a pair's 64-k block of a 256 x 256 tile takes 512 cycles of products and 32 KB into each SM's shared memory,
+// for which all SMs together got 12.5 TB/s out of L2 (393 ns a block over 9472 x 4096 x 512, 270 of them products). So 8192 x
+// 8192 x 8192 runs at 1.45 PFLOP/s, 89 % of the measured library rate; at k = 768 the epilogue shares the time: 8192 x 768 x
+// 3072 31.8 us plain, 33.6 under the polynomial, 41 under GELU (two special functions per value), 44 with a residual.
+// The accumulators are 32-bit and truncate: the error of a result grows with k, about 1.2e-9 k of it.
+//
+// Waits are bounded (mma::wait_warp): a role that gives up tells the others, the loads and products in flight are waited for
 // (bounded as well), TMEM is freed and the block ends; pcb_device_timeouts counts it.
 #include "clear_gemm.h"
 
