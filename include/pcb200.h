@@ -619,9 +619,10 @@ const PcbKernelTable* pcb_kernel_table(int32_t log_n);
 
 /* Kernels this library has launched since it was loaded (all threads, all devices). */
 uint64_t pcb_launch_count(void);
-/* Bounded waits in this library's pipelined kernels (the NTT's bulk-copy stages) that ran out on the current device
- * since the library was loaded: 0 in normal operation; a nonzero count means a copy never completed and the affected
- * rows were left untransformed (synchronizes the device). No counterpart in the reference. */
+/* Bounded waits in this library's pipelined kernels (the NTT's bulk-copy stages, the clear half's products and
+ * attention) that ran out on the current device since the library was loaded: 0 in normal operation; a nonzero count
+ * means a copy or a product never completed and the affected rows were left unwritten (synchronizes the device). No
+ * counterpart in the reference. */
 uint32_t pcb_device_timeouts(void);
 /* Measurement: iters x 8 dependent-chain FP64 FMAs on every thread of 4 x 256-thread blocks per SM, on stream s; returns
  * the FMA count (negative: a cudaError_t). Timed by the caller with CUDA events, it gives the FP64 pipe's throughput

@@ -1,16 +1,19 @@
 // The clear half's matrix product D = A B^T on the fifth-generation tensor cores, with the operators' epilogues.
 //
 // Persistent blocks, one per SM, walk output tiles of 256 x 256 or 256 x 128 (by pairs of blocks) or 128 x 128 or 128 x 64 (by
-// one). Warp 0 streams the operands' 64-k blocks through a ring of shared-memory stages with the TMA engine (either operand
-// may have k or its rows adjacent in memory: the instruction descriptor says which, nothing is transposed on the way); warp 1
-// issues the products (tcgen05.mma) into one of two TMEM accumulators; eight warps (four for 64 columns) take the finished
-// accumulator out of TMEM 32 columns at a time, apply the epilogue in 32 bits and store through shared memory, while the next
-// tile's products run.
+// one). Two warps stream the operands' 64-k blocks, A's and B's, through a ring of shared-memory stages with the TMA engine
+// (either operand may have k or its rows adjacent in memory: the instruction descriptor says which, nothing is transposed on
+// the way; one warp for both took 520 cycles a block, as long as a large tile's products); warp 1 issues the products
+// (tcgen05.mma) into one of two TMEM accumulators; eight warps (four for 64 columns) take the finished accumulator out of
+// TMEM 32 columns at a time, apply the epilogue in 32 bits and store through shared memory, while the next tile's products
+// run.
 //
-// What bounds it: a pair's 64-k block of a 256 x 256 tile takes 512 cycles of products and 32 KB into each SM's shared memory,
-// for which all SMs together got 12.5 TB/s out of L2 (393 ns a block over 9472 x 4096 x 512, 270 of them products). So 8192 x
-// 8192 x 8192 runs at 1.45 PFLOP/s, 89 % of the measured library rate; at k = 768 the epilogue shares the time: 8192 x 768 x
-// 3072 31.8 us plain, 33.6 under the polynomial, 41 under GELU (two special functions per value), 44 with a residual.
+// What bounds it: a pair's 64-k block of a 256 x 256 tile takes 512 cycles of products, and the loop keeps to 505 to 520 of
+// them; what falls is the clock (1.5 to 1.6 GHz with all tensor cores busy), so what costs energy costs time: 8192 x 8192 x
+// 8192 721 us (1.52 PFLOP/s, 94 % of the measured library rate) with tiles in bands, 790 reading A again for each column.
+// At k = 768 the epilogue shares the time: 8192 x 768 x 3072 31 us plain, 33.8 under the polynomial, 40 under GELU (two
+// special functions per value), 43 with a residual. Short products (1024 x 1024 x 1024 8.4 us) are set-up, one tile's loads
+// and its epilogue.
 // The accumulators are 32-bit and truncate: the error of a result grows with k, about 1.2e-9 k of it.
 //
 // Waits are bounded (mma::wait_warp): a role that gives up tells the others, the loads and products in flight are waited for
@@ -46,7 +49,11 @@ struct Shape {
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int EWARPS = BN == 64 ? 4 : 8;         // epilogue warps: 4 cover the 128 lanes, 8 halve the columns
     static constexpr int COLS = BN / (EWARPS / 4);          // columns of one epilogue warp
-    static constexpr int THREADS = 64 + 32 * EWARPS;
+    // 64-k blocks that one turn of the products' loop takes. A turn's waiting, electing and committing cost some 150 cycles, a
+    // product's issue 40: a block of a tile of 256 columns keeps the tensor core longer than that (512 cycles), one of 128
+    // columns does not (2048 x 3072 x 768: 15.5 us by twos, 16.5 by ones; 8192 x 768 x 3072 by 256 columns 32.1 and 31.0)
+    static constexpr int AT_ONCE = BN == 256 ? 1 : 2;
+    static constexpr int THREADS = 96 + 32 * EWARPS;
     static constexpr int TMEM = 2 * BN;
     static constexpr int STAGING = 4096;                    // per epilogue warp and direction: 32 rows x 128 bytes
     static constexpr int BUFFERS = EPI == KERNEL_ADD || EPI == KERNEL_DZ ? 2 : 1;
@@ -58,8 +65,8 @@ struct alignas(64) Params {
     CUtensorMap a, b, y, extra_map, part;
     int m, n, k;
     int a_mn, b_mn, a_panels, b_panels, bf16;
-    int stage_bytes;  // of one block's loads: fewer than the stage's where A has few rows
-    int tiles_m, tiles_n, kblocks;
+    int a_bytes;  // of one block's loads of A: fewer than the stage's where A has few rows
+    int tiles_m, tiles_n, band, kblocks;
     // Units of work: tiles [0, whole) entire, then the other `tail` tiles in `splits` parts of `kper` k blocks: to 32-bit
     // sums that `join` finishes, or (slices) each part to its own y
     int whole, tail, splits, kper, slices;
@@ -79,11 +86,24 @@ struct alignas(64) Params {
 };
 
 struct Unit {
-    int tile, split, kb0, kb1;
+    int tile, split, kb0, kb1, tm, tn;
     bool partial;
 };
+// Tile number `tile`'s row and column of tiles: down all rows of tiles, or (BANDS) down `band` of them at a time, column
+// after column (`gemm` says when)
+template <bool BANDS>
+__device__ __forceinline__ void place(const Params& p, int tile, int& tm, int& tn) {
+    int at = 0, h = p.tiles_m;
+    if (BANDS) {
+        const int per = p.band * p.tiles_n, b = tile / per;
+        at = b * p.band, h = min(p.band, p.tiles_m - at), tile -= b * per;
+    }
+    tn = tile / h;
+    tm = at + tile - tn * h;
+}
+template <bool BANDS>
 __device__ __forceinline__ Unit unit_of(const Params& p, int u) {
-    Unit w = {u, 0, 0, p.kblocks, false};
+    Unit w = {u, 0, 0, p.kblocks, 0, 0, false};
     if (u >= p.whole) {
         w.split = (u - p.whole) / p.tail;
         w.tile = u - w.split * p.tail;
@@ -91,6 +111,7 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u) {
         w.kb1 = min(p.kblocks, w.kb0 + p.kper);
         w.partial = !p.slices;
     }
+    place<BANDS>(p, w.tile, w.tm, w.tn);
     return w;
 }
 
@@ -219,7 +240,7 @@ __device__ __noinline__ void store_block(const unsigned char* stage, bool narrow
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
-template <int BN, int CTAS, int EPI, int ACT>
+template <int BN, int CTAS, int EPI, int ACT, bool BANDS>
 __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(const __grid_constant__ Params p) {
     using S = Shape<BN, CTAS, EPI>;
     extern __shared__ unsigned char raw[];
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 2);  // A's warp and B's
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -264,40 +285,41 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
 
     const int units = p.whole + p.tail * p.splits;
     const int first_unit = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {  // A's blocks and B's
+        const bool b_side = warp == 2;
+        const CUtensorMap* map = b_side ? &p.b : &p.a;
+        // rows adjacent: 64 x 64 panels, together in one box where the rows are whole panels (operand_map)
+        const int mn = b_side ? p.b_mn : p.a_mn, panels = b_side ? p.b_panels : p.a_panels;
+        const int boxes = mn && !panels ? (b_side ? S::B_ROWS : BM) / 64 : 1;
+        const uint32_t bytes = CTAS * (b_side ? S::B_BYTES : p.a_bytes);
+        unsigned char* to = base + (b_side ? S::A_BYTES : 0);
         Ring<S::STAGES> r;
         int loaded = 0;
         bool ok = true, ready = true;
         for (int u = first_unit; u < units && ok; u += stride) {
-            const Unit w = unit_of(p, u);
-            const int m0 = (w.tile % p.tiles_m * CTAS + rank) * BM, n0 = w.tile / p.tiles_m * BN + rank * S::B_ROWS;
-            for (int kb = w.kb0; kb < w.kb1; ++kb, ++loaded, r.next()) {
+            const Unit w = unit_of<BANDS>(p, u);
+            const int row = b_side ? w.tn * BN + rank * S::B_ROWS : (w.tm * CTAS + rank) * BM;
+            int x = !mn ? w.kb0 * BK : panels ? 0 : row, y = mn ? w.kb0 * BK : row;
+            const int z = mn && panels ? row / 64 : 0, dx = mn ? 0 : BK, dy = mn ? BK : 0;
+            for (int kb = w.kb0; kb < w.kb1; ++kb, ++loaded, x += dx, y += dy, r.next()) {
                 // a fresh barrier's preceding phase counts as done: the first round does not wait
                 if (!__all_sync(~0u, ready)) ok = wait_warp(&empty[r.stage], r.phase ^ 1, dead, &g_gemm_timeouts);
                 if (!ok) break;
                 Ring<S::STAGES> ahead = r;
                 ahead.next();
                 ready = peek(&empty[ahead.stage], ahead.phase ^ 1);
-                unsigned char* sa = base + r.stage * S::STAGE;
-                unsigned char* sb = sa + S::A_BYTES;
+                unsigned char* at = to + r.stage * S::STAGE;
                 uint64_t* bar = &full[r.stage];
                 // a pair's loads all complete on the first block's barrier, whose warp issues the products
                 const uint32_t pair_bar = CTAS == 2 ? cluster_addr(bar, 0) : 0;
                 if (elect()) {
-                    if (rank == 0) mbar_expect(bar, CTAS * p.stage_bytes);
-                    auto box = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
-                        if (CTAS == 2) tma_load_pair(dst, map, x, y, z, pair_bar);
-                        else tma_load(dst, map, x, y, z, bar);
+                    if (rank == 0) mbar_expect(bar, bytes);
+                    auto box = [&](int j) {
+                        if (CTAS == 2) tma_load_pair(at + j * 8192, map, x + 64 * j, y, z, pair_bar);
+                        else tma_load(at + j * 8192, map, x + 64 * j, y, z, bar);
                     };
-                    // rows adjacent: 64 x 64 panels, together in one box where the rows are whole panels (operand_map)
-                    if (!p.a_mn) box(sa, &p.a, kb * BK, m0, 0);
-                    else if (p.a_panels) box(sa, &p.a, 0, kb * BK, m0 / 64);
-                    else
-                        for (int j = 0; j < BM / 64; ++j) box(sa + j * 8192, &p.a, m0 + 64 * j, kb * BK, 0);
-                    if (!p.b_mn) box(sb, &p.b, kb * BK, n0, 0);
-                    else if (p.b_panels) box(sb, &p.b, 0, kb * BK, n0 / 64);
-                    else
-                        for (int j = 0; j < S::B_ROWS / 64; ++j) box(sb + j * 8192, &p.b, n0 + 64 * j, kb * BK, 0);
+                    box(0);
+                    for (int j = 1; j < boxes; ++j) box(j);
                 }
                 __syncwarp();
             }
@@ -314,25 +336,43 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             Ring<2> out;
             bool ok = true, ready = false;
             for (int u = first_unit; u < units && ok; u += stride) {
-                const Unit w = unit_of(p, u);
+                const Unit w = unit_of<BANDS>(p, u);
                 if (w.kb0 >= w.kb1) continue;
                 ok = wait_warp(&acc_empty[out.stage], out.phase ^ 1, dead, &g_gemm_timeouts);
                 if (!ok) break;
                 fence_after();
                 const uint32_t acc = tmem + out.stage * BN;
-                for (int kb = w.kb0; kb < w.kb1; ++kb, r.next()) {
-                    if (!__all_sync(~0u, ready)) ok = wait_warp(&full[r.stage], r.phase, dead, &g_gemm_timeouts);
+                for (int kb = w.kb0; kb < w.kb1; kb += S::AT_ONCE) {
+                    const bool two = S::AT_ONCE == 2 && kb + 1 < w.kb1;
+                    Ring<S::STAGES> second = r;
+                    second.next();
+                    if (!__all_sync(~0u, ready)) {
+                        ok = wait_warp(&full[r.stage], r.phase, dead, &g_gemm_timeouts);
+                        if (two) ok = ok && wait_warp(&full[second.stage], second.phase, dead, &g_gemm_timeouts);
+                    }
                     if (!ok) break;
                     fence_after();
-                    Ring<S::STAGES> ahead = r;
-                    ahead.next();
-                    ready = peek(&full[ahead.stage], ahead.phase);
                     const uint64_t da = a_desc + (uint32_t)(r.stage * (S::STAGE >> 4)), db = b_desc + (uint32_t)(r.stage * (S::STAGE >> 4));
+                    const uint64_t da2 = a_desc + (uint32_t)(second.stage * (S::STAGE >> 4)), db2 = b_desc + (uint32_t)(second.stage * (S::STAGE >> 4));
+                    uint64_t* done[2] = {&empty[r.stage], &empty[second.stage]};
+                    r = second;
+                    if (two) r.next();
+                    ready = peek(&full[r.stage], r.phase);
+                    if (S::AT_ONCE == 2) {
+                        Ring<S::STAGES> ahead = r;
+                        ahead.next();
+                        ready = ready && peek(&full[ahead.stage], ahead.phase);
+                    }
                     if (elect()) {
 #pragma unroll
                         for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da + q * a_step, db + q * b_step, idesc, kb > w.kb0 || q > 0);
-                        mma_commit<CTAS>(&empty[r.stage]);
-                        if (kb + 1 == w.kb1) mma_commit<CTAS>(&acc_full[out.stage]);
+                        mma_commit<CTAS>(done[0]);
+                        if (two) {
+#pragma unroll
+                            for (int q = 0; q < BK / 16; ++q) mma_ss<CTAS>(acc, da2 + q * a_step, db2 + q * b_step, idesc, true);
+                            mma_commit<CTAS>(done[1]);
+                        }
+                        if (kb + S::AT_ONCE >= w.kb1) mma_commit<CTAS>(&acc_full[out.stage]);
                     }
                     __syncwarp();
                 }
@@ -344,7 +384,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             }
         }
     } else {
-        const int ew = warp - 2, quad = warp % 4, half = ew / 4;
+        const int ew = warp - 3, quad = warp % 4, half = ew / 4;
         unsigned char* stage = staging + ew * S::BUFFERS * S::STAGING;
         unsigned char* in = stage + (S::BUFFERS - 1) * S::STAGING;  // `extra`'s boxes: 32 rows x 128 bytes, the next one on its way
         float* bias = bias_s + ew * 32;
@@ -365,10 +405,10 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
         auto fetch = [&](int u, int e) {
             if (p.extra_mode == EXTRA_LOAD) return;
             for (; HAS_EXTRA && u < units; u += stride, e = 0) {  // the next box with columns inside: of this unit, or the first of a later one
-                const Unit w = unit_of(p, u);
-                const int x = w.tile / p.tiles_m * BN + half * S::COLS + e * ecols;
+                const Unit w = unit_of<BANDS>(p, u);
+                const int x = w.tn * BN + half * S::COLS + e * ecols;
                 if (w.partial || e * ecols >= S::COLS || x >= p.n) continue;
-                const int y = (w.tile % p.tiles_m * CTAS + rank) * BM + quad * 32;
+                const int y = (w.tm * CTAS + rank) * BM + quad * 32;
                 if (p.extra_mode == EXTRA_TMA) {
                     if (lane == 0) {
                         fence_async_smem();
@@ -384,9 +424,9 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
         if constexpr (HAS_EXTRA) fetch(first_unit, 0);
         int t = 0;
         for (int u = first_unit; u < units; u += stride) {
-            const Unit w = unit_of(p, u);
+            const Unit w = unit_of<BANDS>(p, u);
             if (w.kb0 >= w.kb1) continue;
-            const int m0 = (w.tile % p.tiles_m * CTAS + rank) * BM, tn = w.tile / p.tiles_m, n0 = tn * BN;
+            const int m0 = (w.tm * CTAS + rank) * BM, tn = w.tn, n0 = tn * BN;
             const int buf = t & 1, row0 = m0 + quad * 32, row = row0 + lane, first = n0 + half * S::COLS;
             auto bias_of = [&](int col) { return col + lane < p.n ? load(p.bias, col + lane, p.bias_type) : 0.0f; };
             float biases[S::COLS / 32];  // the lane's column of each 32, read while the products still run
@@ -598,7 +638,10 @@ __global__ void __launch_bounds__(256) join(const float* part, int bn, int tile_
     const float alpha = p.alpha ? *p.alpha : 1.0f;
     const int groups = tile_rows / JOIN_ROWS, i = blockIdx.x / groups, r0 = blockIdx.x % groups * JOIN_ROWS;
     const int tile = p.whole + i, quads = bn / 4;
-    const int64_t row0 = (int64_t)(tile % p.tiles_m) * tile_rows + r0, col0 = (int64_t)(tile / p.tiles_m) * bn;
+    int tm, tn;
+    if (p.band) place<true>(p, tile, tm, tn);
+    else place<false>(p, tile, tm, tn);
+    const int64_t row0 = (int64_t)tm * tile_rows + r0, col0 = (int64_t)tn * bn;
     const int64_t step = (int64_t)p.tail * tile_rows * quads;
     for (int e = threadIdx.x; e < JOIN_ROWS * quads; e += 256) {
         const int64_t row = row0 + e / quads, col = col0 + e % quads * 4;
@@ -749,12 +792,12 @@ Plan plan_slices(int m, int n, int k, int slices) {
     return best;
 }
 
-template <int BN, int CTAS, int EPI, int ACT>
+template <int BN, int CTAS, int EPI, int ACT, bool BANDS = false>
 int launch(const Params& p, cudaStream_t s) {
     using S = Shape<BN, CTAS, EPI>;
     static_assert(S::SMEM <= 232448, "shared memory");
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_smem((const void*)product<BN, CTAS, EPI, ACT>, S::SMEM, done)) return rc;
+    if (int rc = allow_smem((const void*)product<BN, CTAS, EPI, ACT, BANDS>, S::SMEM, done)) return rc;
     const int64_t units = (int64_t)p.whole + (int64_t)p.tail * p.splits, slots = SMS / CTAS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((units < slots ? units : slots) * CTAS));
@@ -769,11 +812,12 @@ int launch(const Params& p, cudaStream_t s) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, product<BN, CTAS, EPI, ACT>, p);
+    cudaLaunchKernelEx(&cfg, product<BN, CTAS, EPI, ACT, BANDS>, p);
     return PCB_LAUNCH_RESULT();
 }
 template <int EPI, int ACT>
 int launch(const Plan& pl, const Params& p, cudaStream_t s) {
+    if (p.band) return launch<256, 2, EPI, ACT, true>(p, s);
     if (pl.ctas == 2) return pl.bn == 256 ? launch<256, 2, EPI, ACT>(p, s) : launch<128, 2, EPI, ACT>(p, s);
     return pl.bn == 128 ? launch<128, 1, EPI, ACT>(p, s) : launch<64, 1, EPI, ACT>(p, s);
 }
@@ -817,7 +861,11 @@ int gemm(const Gemm& g, cudaStream_t s) {
     p.m = g.m, p.n = g.n, p.k = g.k;
     p.a_mn = !g.a.k_adjacent, p.b_mn = !g.b.k_adjacent, p.a_panels = panels(g.a, g.m), p.b_panels = panels(g.b, g.n);
     p.bf16 = g.type == PCB_BF16;
-    p.stage_bytes = (arows + pl.bn / pl.ctas) * BK * 2;
+    p.a_bytes = arows * BK * 2;
+    // Where A stays in L2, tiles go down all of its rows, column after column; a larger A is read again for each column, and
+    // bands of 2048 rows, about square over a round, read less of both (8192 x 8192 x 8192: 722 us against 790,
+    // 50000 x 4096 x 768: 225 against 263; 4096 x 768 x 50000, whose A takes 6 MB, 245 down all rows against 252)
+    p.band = pl.bn == 256 && tm > 8 && 2.0 * g.m * g.k > 64e6 ? 8 : 0;
     p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.kblocks = (g.k + BK - 1) / BK;
     p.whole = pl.whole, p.tail = (int)(tm * tn) - pl.whole, p.splits = pl.splits, p.kper = pl.kper, p.slices = g.slices;
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;

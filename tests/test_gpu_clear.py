@@ -56,6 +56,26 @@ def test_linear_epilogues(act, bias, residual, out):
     R.close(y, R.linear(x, w, b, act, r, out))
 
 
+@pytest.mark.parametrize("act,residual", [(None, None), (None, BF), ("gelu", None), (GELU_POLY, F32)],
+                         ids=["none", "residual", "gelu", "poly"])
+def test_linear_operand_beyond_l2(act, residual):
+    """An A above 64 MB: its tiles go in bands of 2048 rows, the last one lower."""
+    m, k, n = 4900, 6600, 1000
+    x, w = rnd(1, m, k), rnd(2, k, n, std=0.5 * k**-0.5)
+    r = None if residual is None else rnd(3, m, n, dtype=residual)
+    R.close(clear.linear(x, w, act=act, residual=r), R.linear(x, w, None, act, r, BF))
+
+
+@pytest.mark.parametrize("act", [None, GELU_POLY], ids=["none", "poly"])
+def test_linear_grad_operands_beyond_l2(act):
+    m, k, n = 6600, 4900, 1000
+    x, w, dy = rnd(1, m, k), rnd(2, k, n, std=0.5 * k**-0.5), rnd(3, m, n)
+    dx, dw, _ = clear.linear_grad(dy, x, w, act=act, needs=(True, True, False))
+    want = R.linear_grad(dy, x, w, None, act, BF)
+    R.close(dx, want[0])
+    R.close(dw, want[1])
+
+
 def test_linear_strides_and_order():
     """Rows of a wider tensor, a transposed weight, an odd first element, a broadcast row, a 4-d batch."""
     big = rnd(1, 150, 400)
@@ -249,7 +269,7 @@ def test_attention_strides():
     qkv = rnd(1, 203, 3, 12, 64)
     q, k, v = qkv.unbind(1)
     R.close(clear.prompt_attention(q, k, v, lens), R.attention(q, k, v, lens, lens, 0.125, True, None))
-    odd = rnd(2, 203, 12 * 67 + 5)[:, 5:].view(203, 12, 67) if False else rnd(2, 203 * 12 * 67).view(203, 12, 67)
+    odd = rnd(2, 203 * 12 * 67).view(203, 12, 67)
     q, k, v = odd[..., :64], odd[..., 1:65], odd[..., 3:67]
     R.close(clear.prompt_attention(q, k, v, lens), R.attention(q, k, v, lens, lens, 0.125, True, None))
     t = rnd(3, 12, 203, 64).transpose(0, 1)
@@ -377,6 +397,14 @@ def test_vocab(rows, vocab, dim, dtype):
     dh, dw = clear.vocab_loss_grad(h, w, t, lse, weight)
     R.close(dh, want[2])
     R.close(dw, want[3])
+
+
+def test_vocab_slopes_beyond_l2():
+    h, w, targets, weight = vocab_case(1100, 40000, 320, BF)
+    loss, lse = clear.vocab_loss(h, w, targets)
+    dh, dw = clear.vocab_loss_grad(h, w, targets, lse, weight)
+    for got, want in zip((loss, lse, dh, dw), R.vocab(h, w, targets, weight, -100)):
+        R.close(got, want)
 
 
 def test_vocab_strides_and_needs():
