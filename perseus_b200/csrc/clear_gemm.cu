@@ -630,40 +630,50 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
     if (warp == 1) tmem_free<CTAS>(tmem, S::TMEM);
 }
 
-// The split tiles: y = alpha (act(sum of the parts in order + bias) + extra). Sixteen rows of a tile per block.
-constexpr int JOIN_ROWS = 16;
-__global__ void __launch_bounds__(256) join(const float* part, int bn, int tile_rows, const __grid_constant__ Params p) {
-    pdl_wait();
-    pdl_release();
-    const float alpha = p.alpha ? *p.alpha : 1.0f;
-    const int groups = tile_rows / JOIN_ROWS, i = blockIdx.x / groups, r0 = blockIdx.x % groups * JOIN_ROWS;
-    const int tile = p.whole + i, quads = bn / 4;
+// The split tiles: y = alpha (act(sum of the parts in order + bias) + extra). Four adjacent columns per thread, the parts
+// read four at a time so that their latencies overlap (one after another, six parts cost 3 us of a 9 us call).
+constexpr int JOIN_VALUES = 1024;  // of a tile per block
+__global__ void __launch_bounds__(JOIN_VALUES / 4) join(const float* part, int bn, int tile_rows, const __grid_constant__ Params p) {
+    const int groups = tile_rows * bn / JOIN_VALUES, i = blockIdx.x / groups, quads = bn / 4;
+    const int e = blockIdx.x % groups * (JOIN_VALUES / 4) + threadIdx.x, tile = p.whole + i;
     int tm, tn;
     if (p.band) place<true>(p, tile, tm, tn);
     else place<false>(p, tile, tm, tn);
-    const int64_t row0 = (int64_t)tm * tile_rows + r0, col0 = (int64_t)tn * bn;
+    const int64_t row = (int64_t)tm * tile_rows + e / quads, col = (int64_t)tn * bn + e % quads * 4;
     const int64_t step = (int64_t)p.tail * tile_rows * quads;
-    for (int e = threadIdx.x; e < JOIN_ROWS * quads; e += 256) {
-        const int64_t row = row0 + e / quads, col = col0 + e % quads * 4;
-        if (row >= p.m || col >= p.n) continue;
-        const float4* at = (const float4*)part + ((int64_t)i * tile_rows + r0) * quads + e;
-        float4 s = at[0];
-        for (int k = 1; k < p.splits; ++k) {
-            const float4 q = at[k * step];
-            s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
-        }
-        const float v4[4] = {s.x, s.y, s.z, s.w};
+    pdl_wait();
+    pdl_release();
+    if (row >= p.m || col >= p.n) return;
+    const float alpha = p.alpha ? *p.alpha : 1.0f;
+    const float4* at = (const float4*)part + (int64_t)i * tile_rows * quads + e;
+    float4 s = at[0];
+    for (int k = 1; k < p.splits; k += 4) {
+        float4 q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (col + j >= p.n) break;
-            float v = v4[j], skip;
-            if (p.bias) v += load(p.bias, col + j, p.bias_type);
-            if (p.act.kind == PCB_ACT_GELU) parts(act2<PCB_ACT_GELU, false>(p.act, both(v)), v, skip);
-            else if (p.act.kind == PCB_ACT_POLY) parts(act2<PCB_ACT_POLY, false>(p.act, both(v)), v, skip);
-            if (p.extra) v += load(p.extra, row * p.extra_pitch + col + j, p.extra_type);
-            store(p.y_ptr, row * p.y_pitch + col + j, p.y_type, v * alpha);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (k + j < p.splits) q[j] = at[(k + j) * step];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < p.splits) s.x += q[j].x, s.y += q[j].y, s.z += q[j].z, s.w += q[j].w;
     }
+    float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float skip;
+        if (col + j >= p.n) break;
+        if (p.bias) v[j] += load(p.bias, col + j, p.bias_type);
+        if (p.act.kind == PCB_ACT_GELU) parts(act2<PCB_ACT_GELU, false>(p.act, both(v[j])), v[j], skip);
+        else if (p.act.kind == PCB_ACT_POLY) parts(act2<PCB_ACT_POLY, false>(p.act, both(v[j])), v[j], skip);
+        if (p.extra) v[j] += load(p.extra, row * p.extra_pitch + col + j, p.extra_type);
+        v[j] *= alpha;
+    }
+    const int64_t to = row * p.y_pitch + col;
+    if (p.y_tma && col + 3 < p.n) {  // rows on 16 bytes
+        if (p.y_type == PCB_F32) ((float4*)p.y_ptr)[to / 4] = make_float4(v[0], v[1], v[2], v[3]);
+        else ((uint2*)p.y_ptr)[to / 4] = make_uint2(pack2(v[0], v[1], p.bf16), pack2(v[2], v[3], p.bf16));
+        return;
+    }
+    for (int j = 0; j < 4 && col + j < p.n; ++j) store(p.y_ptr, to + j, p.y_type, v[j]);
 }
 
 // Rows of 16-bit values to rows on 16 bytes, zeros up to the pitch; a warp per row, up to three matrices (blockIdx.y)
@@ -738,43 +748,44 @@ int operand_map(CUtensorMap* map, const Operand& o, int type, int rows, int k, i
     return encode_map(map, type, o.p, 3, size, stride, box);
 }
 
-// Tile and splitting, from estimated nanoseconds. A 64-k block of a tile costs its products, or its bytes into shared memory
-// at what one SM or all of them together take (measured over 9472 x 4096 x 512: 85 GB/s for each of 148 SMs; 256 x 256 by
-// pairs 393 ns a block, 256 x 128 297, 128 x 128 366, 128 x 64 265). The tiles that do not fill a round over the SMs may split
-// their k; that costs their 32-bit sums' way to L2 and back and a launch.
+// Tile and splitting, from estimated nanoseconds, fitted to every tile and splitting of 20 shapes of 1 to 8192 rows, k 509 to
+// 8192, 768 to 50000 columns (the choice is within 7 % of the fastest there). A 64-k block of a tile costs its
+// products or their issue, up to a fifth more as more SMs are busy and the clock falls, or its bytes into shared memory at
+// 16.5 TB/s for all SMs together. The tiles that do not fill a round over the SMs may split their k; that costs their 32-bit
+// sums' way to L2 and back and a launch.
 struct Plan {
     int bn, ctas, whole, splits, kper;
     double ns;
 };
 struct Tile {
     int bn, ctas;
-    double products;  // ns of a 64-k block's
+    double block;      // ns of a 64-k block
+    double next, last; // ns of what one tile, and the last one, add: first loads and the epilogue that does not overlap
 };
-constexpr Tile TILES[] = {{256, 2, 270}, {128, 2, 150}, {128, 1, 150}, {64, 1, 120}};
+constexpr Tile TILES[] = {{256, 2, 270, 600, 1800}, {128, 2, 175, 400, 1200}, {128, 1, 230, 400, 700}, {64, 1, 150, 300, 400}};
 int a_rows(int m) { return m < BM ? (m + 7) / 8 * 8 : BM; }  // rows of A that a tile loads: what lies past them is not used
+double block_ns(const Tile& t, int m, int64_t active) {
+    const double sms = (double)(active * t.ctas), bytes = (a_rows(m) + t.bn / t.ctas) * BK * 2;
+    return std::max(t.block * (1.0 + 0.2 * std::min(1.0, sms / 96)), bytes * sms / 16500);
+}
 double rounds(const Tile& t, int m, int64_t units, int kblocks) {
     const int64_t slots = SMS / t.ctas, full = units / slots, rest = units % slots;
-    const double bytes = a_rows(m) * BK * 2 + t.bn / t.ctas * BK * 2;
-    auto block = [&](int64_t active) {
-        const double one = bytes / 150, all = bytes * (double)(active * t.ctas) / 12500;
-        return std::max(t.products, std::max(one, all));
-    };
-    const double ends = 4.0 * t.bn;  // the part of a tile's epilogue and first loads that does not overlap
-    return full * (kblocks * block(slots) + ends) + (rest ? kblocks * block(rest) + ends : 0.0);
+    return full * (kblocks * block_ns(t, m, slots) + t.next) + (rest ? kblocks * block_ns(t, m, rest) + t.last : t.last - t.next);
 }
+// the way of `parts` tiles' 32-bit sums to L2 and back, and the launch that joins them
+double join_cost(const Tile& t, int64_t parts) { return 1000.0 + 8.0 * t.bn + (double)parts * BM * t.ctas * t.bn * 8 / 13500; }
 Plan plan(int m, int n, int k, bool may_split) {
     const int kb = (k + BK - 1) / BK;
     Plan best{256, 2, 0, 1, kb, 1e300};
     for (const Tile& t : TILES) {
         const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
         const int64_t tiles = tm * tn, slots = SMS / t.ctas, tail = tiles % slots, whole = tiles - tail;
-        double ns = rounds(t, m, tiles, kb) + (t.ctas == 2 ? 200 : 0);
+        double ns = rounds(t, m, tiles, kb);
         if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)tiles, 1, kb, ns};
         for (int sp = 2; may_split && tail && sp <= 16; ++sp) {
             const int per = (kb + sp - 1) / sp;
             if (per < 4 || (sp - 1) * per >= kb) continue;
-            ns = rounds(t, m, whole, kb) + rounds(t, m, tail * sp, per) + (t.ctas == 2 ? 200 : 0) + 3500 +
-                 (double)tail * BM * t.ctas * t.bn * 8 * sp / 8000;
+            ns = whole / slots * (kb * block_ns(t, m, slots) + t.next) + rounds(t, m, tail * sp, per) + join_cost(t, tail * sp);
             if (ns < best.ns) best = Plan{t.bn, t.ctas, (int)whole, sp, per, ns};
         }
     }
@@ -786,7 +797,7 @@ Plan plan_slices(int m, int n, int k, int slices) {
     Plan best{256, 2, 0, slices, per, 1e300};
     for (const Tile& t : TILES) {
         const int64_t tm = ((int64_t)m + BM * t.ctas - 1) / (BM * t.ctas), tn = ((int64_t)n + t.bn - 1) / t.bn;
-        const double ns = rounds(t, m, tm * tn * slices, per) + (t.ctas == 2 ? 200 : 0) + (double)m * n * 8 * slices / 8000;
+        const double ns = rounds(t, m, tm * tn * slices, per) + (double)m * n * 8 * slices / 8000;
         if (ns < best.ns) best = Plan{t.bn, t.ctas, 0, slices, per, ns};
     }
     return best;
@@ -912,7 +923,7 @@ int gemm(const Gemm& g, cudaStream_t s) {
              : act == PCB_ACT_POLY ? launch<KERNEL_STORE, PCB_ACT_POLY>(pl, p, s)
                                    : launch<KERNEL_STORE, PCB_ACT_NONE>(pl, p, s);
     if (rc || !split) return rc;
-    launch_pdl(join, dim3((unsigned)(p.tail * (rows / JOIN_ROWS))), dim3(256), s, (const float*)g.partial, pl.bn, rows, p);
+    launch_pdl(join, dim3((unsigned)((int64_t)p.tail * rows * pl.bn / JOIN_VALUES)), dim3(JOIN_VALUES / 4), s, (const float*)g.partial, pl.bn, rows, p);
     return PCB_LAUNCH_RESULT();
 }
 
