@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256) finish(const float* x, int slices, int64_
 // The pieces of the vocabulary: at most 256 MiB of slopes (16 bits) each, and of the widths that fit, alike but for the last and
 // multiples of 256, the one whose three products fill the SMs best (rows x columns, columns x dim, and rows x dim with k in
 // `slices` parts). Pieces that stay in L2 are no faster, and each costs some 20 us of products starting and ending: the
-// gradients of 4096 x 50000 x 768 take 1190 us at 24 MiB, 835 at 48, 821 at 96, 785 at 256 and 731 in one piece of 410.
+// gradients of 4096 x 50000 x 768 take 1040 us at 24 MiB, 818 at 48, 790 at 96, 722 at 256 and 703 in one piece of 410.
 struct Pieces {
     int cols, slices;
 };

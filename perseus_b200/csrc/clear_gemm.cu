@@ -12,7 +12,7 @@
 // them; what falls is the clock (1.5 to 1.6 GHz with all tensor cores busy), so what costs energy costs time: 8192 x 8192 x
 // 8192 721 us (1.52 PFLOP/s, 94 % of the measured library rate) with tiles in bands, 790 reading A again for each column.
 // At k = 768 the epilogue shares the time: 8192 x 768 x 3072 31 us plain, 33.8 under the polynomial, 40 under GELU (two
-// special functions per value), 43 with a residual. Short products (1024 x 1024 x 1024 8.4 us) are set-up, one tile's loads
+// special functions per value), 43 with a residual. Short products (1024 x 1024 x 1024 7.5 us) are set-up, one tile's loads
 // and its epilogue.
 // The accumulators are 32-bit and truncate: the error of a result grows with k, about 1.2e-9 k of it.
 //
