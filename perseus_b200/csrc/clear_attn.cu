@@ -120,8 +120,9 @@ __device__ __noinline__ void attend_row(const PcbClearAttention& a, int64_t qrow
 // the products need at 64 dims, so a quarter of them is computed here (8192 tokens, 12 heads over 4: 164 us without, 156 with
 // a quarter, 166 with half; at 128 dims the products take as long as the exponentials, and it costs 1 %). x = n + f with n the nearest integer (in the low bits of
 // x + 1.5 2^23), |f| <= 1/2; 2^f by the polynomial of least relative error of degree 4 (2.6e-6, a thousandth of the weights'
-// rounding), 2^n added to its exponent. Below -126 it stays at 2^-126, which a masked key then weighs
-// against at least 2^-8 (a row that sees nothing is told by its limit); NaN gives a value that is not finite in 16 bits.
+// rounding), 2^n added to its exponent. x stays at -126 from below, and the result there is subtracted from all: a key that
+// is masked (x = -inf) or far below weighs exactly 0, or V values near bfloat16's largest would show through 2^-126. NaN gives
+// a value that is not finite in 16 bits.
 __device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
     float x0, x1, t0, t1, p0, p1;
     parts(x, x0, x1);
@@ -136,8 +137,9 @@ __device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
     p = fma2(p, f, both(0.9999992847442627f));
     parts(t, t0, t1);
     parts(p, p0, p1);
-    return two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
-               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+    const f32x2 e = two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
+                        __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+    return add2(e, both(__uint_as_float(0x807FFFF4u)));  // -0.9999992847442627 2^-126: f = 0, n = -126
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel

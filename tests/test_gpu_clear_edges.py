@@ -1,0 +1,51 @@
+"""The clear half's operators (perseus_b200.clear) where values, sizes or masks are at their ends, against the 64-bit forms
+of tests/_clear_ref.py."""
+import pytest
+import torch
+
+from perseus_b200 import attention as A
+from perseus_b200 import clear
+from tests import _clear_ref as R
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def rnd(seed, *shape, std=1.0, dtype=BF):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("weights", [None, tuple(A.softmax_poly(256))], ids=["softmax", "poly"])
+@pytest.mark.parametrize("dim", [64, 40, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_masked_large_values_stay_out(weights, dim, dtype):
+    """The type's largest finite values in V where they are masked: a later token's, the neighbouring sequence's."""
+    big = torch.finfo(dtype).max
+    lens, scale = [77, 50, 90], dim**-0.5
+    q, k, v = rnd(1, 217, 4, dim, std=0.5, dtype=dtype), rnd(2, 217, 4, dim, std=0.5, dtype=dtype), rnd(3, 217, 4, dim, dtype=dtype)
+    want = R.attention(q, k, v, lens, lens, scale, True, weights)
+    v[77:127] = big
+    got = clear.prompt_attention(q, k, v, lens, weights=weights)
+    for s in (slice(0, 77), slice(127, 217)):
+        R.close(got[s], (want[0][s], want[1][s]))
+    for bad in (6, 71, 150):
+        v = rnd(3, 217, 4, dim, dtype=dtype)
+        want = R.attention(q, k, v, [217], [217], scale, True, weights)
+        v[bad:bad + 2] = -big
+        got = clear.prompt_attention(q, k, v, [217], weights=weights)
+        R.close(got[:bad], (want[0][:bad], want[1][:bad]))
+
+
+@pytest.mark.parametrize("past", [0, 4000])
+def test_attention_weights_that_vanish(past):
+    """Visible keys whose weight is below 2^-150 of the largest: nothing of their values, up to the type's largest."""
+    n = 9 + past
+    q, k, v = torch.zeros(1, 1, 64, dtype=BF, device="cuda"), torch.zeros(n, 1, 64, dtype=BF, device="cuda"), rnd(3, n, 1, 64)
+    q[0, 0, 0] = 8.0
+    k[1:, 0, 0] = -3000.0
+    v[1:] = 3.0e38
+    got = clear.prompt_attention(q, k, v, [1], [n], causal=False)
+    assert torch.equal(got, v[:1])
