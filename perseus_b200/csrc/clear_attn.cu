@@ -403,11 +403,12 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         fence_after();
         if (ok) {
             const int64_t qrow = q0 + tok;
-            const bool blind = limit <= b0 * KEYS;  // sees none of these keys
-            const float scale = POLY ? p.out_scale : blind ? 0.0f : p.splits > 1 ? 1.0f : 1.0f / sum;
+            // sees none of these keys: zeros, whatever the keys that other rows see have left in O (0 x Inf)
+            const bool blind = limit <= b0 * KEYS;
+            const float scale = POLY ? p.out_scale : p.splits > 1 ? 1.0f : 1.0f / sum;
             const int64_t prow = ((int64_t)split * p.a.q_rows + qrow) * p.a.heads + head;
             const int64_t orow = qrow * p.a.out_pitch + head * p.a.out_head;
-            bool odd = !(fabsf(sum) <= 3.4e38f);
+            bool odd = !blind && !(fabsf(sum) <= 3.4e38f);
 #pragma unroll 1
             for (int h = 0; h < DP / 32; ++h) {
                 float o[32];
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                 }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    o[i] = n > 0 ? o[i] * scale : 0.0f;
+                    o[i] = blind ? 0.0f : o[i] * scale;
                     odd |= !(fabsf(o[i]) <= 3.4e38f) && 32 * h + i < p.a.dim;
                 }
                 if (!mine) continue;

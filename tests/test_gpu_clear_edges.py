@@ -1,5 +1,7 @@
 """The clear half's operators (perseus_b200.clear) where values, sizes or masks are at their ends, against the 64-bit forms
 of tests/_clear_ref.py."""
+import math
+
 import pytest
 import torch
 
@@ -49,3 +51,25 @@ def test_attention_weights_that_vanish(past):
     v[1:] = 3.0e38
     got = clear.prompt_attention(q, k, v, [1], [n], causal=False)
     assert torch.equal(got, v[:1])
+
+
+@pytest.mark.parametrize("weights", [None, tuple(A.softmax_poly(256))], ids=["softmax", "poly"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_attention_blind_rows_beside_values_that_are_not_finite(weights, dim, bad):
+    """Queries that see no key are zero whatever the keys that others see, and the next sequence's, hold."""
+    q_lens, k_lens = [100, 50], [60, 50]
+    q, k, v = rnd(1, 150, 4, dim, std=0.5), rnd(2, 110, 2, dim, std=0.5), rnd(3, 110, 2, dim)
+    want = R.attention(q, k, v, q_lens, k_lens, dim**-0.5, True, weights)
+    v[60:] = bad  # the second sequence's
+    got = clear.prompt_attention(q, k, v, q_lens, k_lens, weights=weights)
+    assert not got[:40].any()
+    R.close(got[:100], (want[0][:100], want[1][:100]))
+    v[59] = bad  # a key that the last query alone sees
+    got = clear.prompt_attention(q, k, v, q_lens, k_lens, weights=weights)
+    assert not got[:40].any()
+    R.close(got[:99], (want[0][:99], want[1][:99]))
+    k[58:] = bad
+    got = clear.prompt_attention(q, k, v, q_lens, k_lens, weights=weights)
+    assert not got[:40].any()
+    R.close(got[:98], (want[0][:98], want[1][:98]))
