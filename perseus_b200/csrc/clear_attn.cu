@@ -57,7 +57,7 @@ struct alignas(64) Params {
     float coef[8];        // of the raw scores, the largest of the polynomial's own brought to 1
     float out_scale;
     float* part_o;        // splits > 1: [split][q row][head][dim] sums, and (maximum in base 2, sum of weights)
-    float2* part_ml;
+    float2* part_ml;      // of a split whose visible scores are all -inf: (-inf, -1); of one that the row does not see: (-inf, 0)
     int out_vec;          // out's rows take 16-byte stores
     Work w;
 };
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                         if (32 * h + i < p.a.dim) store(p.a.out, orow + 32 * h + i, p.a.type, o[i]);
                 }
             }
-            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(blind ? -INFINITY : top, blind ? 0.0f : sum);
+            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(blind ? -INFINITY : top, blind ? 0.0f : sum == 0.0f ? -1.0f : sum);
             for (uint32_t again = __ballot_sync(~0u, mine && odd); again; again &= again - 1) {
                 const int src = __ffs(again) - 1;
                 const int tk = __shfl_sync(~0u, tok, src), hd = __shfl_sync(~0u, head, src), lim = __shfl_sync(~0u, limit, src);
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                     if (p.splits > 1) p.part_o[pr * p.a.dim + d] = o[t];
                     else store(p.a.out, qr * p.a.out_pitch + hd * p.a.out_head + d, p.a.type, POLY ? o[t] : o[t] / sm);
                 }
-                if (p.splits > 1 && lane == 0) p.part_ml[pr] = make_float2(tp, sm);
+                if (p.splits > 1 && lane == 0) p.part_ml[pr] = make_float2(tp, sm == 0.0f ? -1.0f : sm);
             }
         }
     }
@@ -470,18 +470,20 @@ __global__ void __launch_bounds__(256) join_splits(PcbClearAttention a, int spli
     if (row >= rows) return;
     const int lane = threadIdx.x % 32;
     float top = -INFINITY, sum = 0.0f, o[4] = {};
+    bool seen = false;
     if (!a.ncoef)
         for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[s * rows + row].x);
     for (int s = 0; s < splits; ++s) {
         const float2 ml = part_ml[s * rows + row];
         const float f = a.ncoef ? 1.0f : ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : exp2f(ml.x - top);
+        seen |= ml.y != 0.0f;
         if (f == 0.0f) continue;
         sum += ml.y * f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
             if (lane + 32 * t < a.dim) o[t] = fmaf(f, part_o[(s * rows + row) * a.dim + lane + 32 * t], o[t]);
     }
-    const float f = a.ncoef ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float f = a.ncoef ? 1.0f : sum == 0.0f ? (seen ? NAN : 0.0f) : 1.0f / sum;  // scores of -inf alone have no softmax
     const int64_t at = row / a.heads * a.out_pitch + row % a.heads * a.out_head;
     for (int t = 0; t < 4; ++t)
         if (lane + 32 * t < a.dim) store(a.out, at + lane + 32 * t, a.type, o[t] * f);

@@ -53,6 +53,25 @@ def test_attention_weights_that_vanish(past):
     assert torch.equal(got, v[:1])
 
 
+@pytest.mark.parametrize("n", [5, 200, 5000])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_scores_of_minus_infinity(n, dim):
+    """A key whose score is -inf weighs nothing; where every visible score is -inf there is no softmax (NaN), however the
+    keys are split over blocks; a query that sees no key has zeros."""
+    q, k, v = rnd(1, 3, 2, dim), rnd(2, n, 2, dim), rnd(3, n, 2, dim)
+    want = R.attention(q[:, :, 1:], k[1:, :, 1:], v[1:, :, 1:], [3], [n - 1], dim**-0.5, False, None)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[0, :, 0] = -math.inf
+    got = clear.prompt_attention(q, k, v, [3], [n], causal=False)
+    R.close(got[..., 1:], want)
+    k[..., 0] = -math.inf
+    assert torch.isnan(clear.prompt_attention(q, k, v, [3], [n], causal=False)).all()
+    q = rnd(4, n + 2, 2, dim)
+    q[..., 0] = 1.0
+    got = clear.prompt_attention(q, k, v, [n + 2], [n])
+    assert not got[:2].any() and torch.isnan(got[2:]).all()
+
+
 @pytest.mark.parametrize("weights", [None, tuple(A.softmax_poly(256))], ids=["softmax", "poly"])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
