@@ -76,12 +76,13 @@ int run_zero(void* y, int64_t rows, int64_t cols, int64_t pitch, int type, cudaS
 }
 
 // ------------------------------------------------------------------------------------------------ vocabulary
-// A maximum (base 2) and a sum of exponentials below it, joined with another. A side without terms, or whose terms are all
+// A maximum and a sum of exponentials below it, joined with another. A side without terms, or whose terms are all
 // -inf, adds nothing; NaN goes through the sum.
+constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float2 join_lse(float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
-    const float fa = a.x == -INFINITY ? (a.y == a.y ? 0.0f : a.y) : a.y * exp2f(a.x - top);
-    const float fb = b.x == -INFINITY ? (b.y == b.y ? 0.0f : b.y) : b.y * exp2f(b.x - top);
+    const float fa = a.x == -INFINITY ? (a.y == a.y ? 0.0f : a.y) : a.y * exp2f((a.x - top) * LOG2E);
+    const float fb = b.x == -INFINITY ? (b.y == b.y ? 0.0f : b.y) : b.y * exp2f((b.x - top) * LOG2E);
     return make_float2(top, fa + fb);
 }
 // lse and loss from the column blocks' maxima and sums: 8 rows per block, 128 lanes over the column blocks (few rows against a
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(1024) join_parts(const float2* part, int npart
     for (int i = 4 + lane / 8; i < 32; i += 4) v = join_lse(v, red[i][x]);
     for (int w = 8; w < 32; w *= 2) v = join_lse(v, make_float2(__shfl_xor_sync(~0u, v.x, w), __shfl_xor_sync(~0u, v.y, w)));
     if (lane >= 8 || row >= a.rows) return;
-    const float lse = (v.x + log2f(v.y)) * 0.69314718055994531f;
+    const float lse = v.x + logf(v.y);
     const int64_t t = a.targets[row];
     a.lse[row] = lse;
     a.loss[row] = t == a.ignore ? 0.0f : t >= 0 && t < a.vocab ? lse - hit[row] : NAN;
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(1024) prepare_rows(PcbClearVocab a, const floa
     if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = 1.0f / scale;
     if (i >= a.rows) return;
     const int64_t t = a.targets[i];
-    rows[i] = VocabRow{a.lse[i] * 1.4426950408889634f, t == a.ignore ? 0.0f : weight[i] * scale,
+    rows[i] = VocabRow{a.lse[i], t == a.ignore ? 0.0f : weight[i] * scale,
                        t >= 0 && t < a.vocab ? (int32_t)t : -1, 0};
 }
 // y = factor * (the sum of `slices` matrices x of pitch `from`, in order), rounded

@@ -439,11 +439,11 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             fence_after();
             const uint32_t acc = tmem + buf * BN + half * S::COLS + ((uint32_t)(quad * 32) << 16);
             const int chunks = min(S::COLS / W, max(0, (p.n - first + W - 1) / W));
-            float top = -INFINITY, sum = 0.0f, lse2 = 0.0f, weight = 0.0f;
+            float top = -INFINITY, sum = 0.0f, lse = 0.0f, weight = 0.0f;
             int target = -1;  // the row's column among this warp's, if it is there
             if (EPI == KERNEL_DL && row < p.m) {
                 const VocabRow vr = p.rows[row];
-                lse2 = vr.lse2, weight = vr.weight, target = vr.target - p.col0 - first;
+                lse = vr.lse, weight = vr.weight, target = vr.target - p.col0 - first;
             }
             if (EPI == KERNEL_LSE && row < p.m) {
                 const int64_t at = p.targets[row] - first;
@@ -469,17 +469,19 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                     float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
                     for (int j = 4; j < W; ++j) m4[j % 4] = fmaxf(m4[j % 4], v[j]);
-                    const float nt = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * LOG2E);
+                    // Differences first, to base 2 after: a finite logit times log2 e may not be finite. Where all are -inf so
+                    // far, 0 in place of the maximum: they weigh nothing
+                    const float nt = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))), sub = nt == -INFINITY ? 0.0f : nt;
                     f32x2 s2[2] = {0, 0};
 #pragma unroll
                     for (int j = 0; j < W; j += 2) {
                         float a, b;
-                        parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-nt)), a, b);
+                        parts(mul2(add2(two(v[j], v[j + 1]), both(-sub)), both(LOG2E)), a, b);
                         s2[j / 2 % 2] = add2(s2[j / 2 % 2], two(ex2(a), ex2(b)));
                     }
                     float a, b;
                     parts(add2(s2[0], s2[1]), a, b);
-                    sum = fmaf(sum, ex2(top - nt), a + b);
+                    sum = fmaf(sum, ex2((top - sub) * LOG2E), a + b);
                     top = nt;
                     continue;
                 }
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
 #pragma unroll
                     for (int j = 0; j < W; j += 2) {
                         float a, b;
-                        parts(fma2(two(v[j], v[j + 1]), both(LOG2E), both(-lse2)), a, b);
+                        parts(mul2(add2(two(v[j], v[j + 1]), both(-lse)), both(LOG2E)), a, b);
                         parts(mul2(two(ex2(a), ex2(b)), both(weight)), v[j], v[j + 1]);
                     }
                     if (has_target) {

@@ -20,9 +20,9 @@ enum Epilogue {
     EPI_DL,     // y = weight (exp(D - lse) - [n = target])
 };
 
-// What EPI_DL needs of a row, in base 2: exp(l - lse) = 2^(l log2 e - lse2)
+// What EPI_DL needs of a row
 struct VocabRow {
-    float lse2, weight;
+    float lse, weight;
     int32_t target;  // -1: none
     int32_t pad;
 };
@@ -48,7 +48,7 @@ struct Gemm {
     const VocabRow* rows;   // EPI_DL
     int col0;               // EPI_DL: the vocabulary entry of this product's first column
     const int64_t* targets; // EPI_LSE
-    float2* parts;          // EPI_LSE: [vocab_parts(n)][m] (maximum in base 2, sum)
+    float2* parts;          // EPI_LSE: [vocab_parts(n)][m] (maximum, sum of exponentials below it)
     float* hit;             // EPI_LSE: [m], written where the target lies in this product's columns
     float* partial;         // EPI_STORE: workspace of gemm_partial() values; null: no splitting
 };

@@ -92,3 +92,49 @@ def test_attention_blind_rows_beside_values_that_are_not_finite(weights, dim, ba
     got = clear.prompt_attention(q, k, v, q_lens, k_lens, weights=weights)
     assert not got[:40].any()
     R.close(got[:98], (want[0][:98], want[1][:98]))
+
+
+# ------------------------------------------------------------------------------------------------ vocabulary
+def vocab_case(rows, vocab, dim, dtype, std=2.0, seed=0):
+    h, w = rnd(seed + 1, rows, dim, dtype=dtype), rnd(seed + 2, vocab, dim, std=std * dim**-0.5, dtype=dtype)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    t[1::4] = -100
+    weight = torch.rand(rows, generator=g, device="cuda") / rows
+    return h, w, t, weight
+
+
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+@pytest.mark.parametrize("rows,vocab", [(20, 700), (300, 5000)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_vocab_masked_entries(low, rows, vocab, dtype):
+    """Entries that a constant channel masks with the type's lowest value or -inf, whole column blocks of them: the loss and
+    the gradients are those of the vocabulary without them."""
+    h, w, t, weight = vocab_case(rows, vocab, 64, dtype)
+    out = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    out[:300] = out[320:333] = out[384:448] = out[-50:] = True
+    out[:512:64] = True
+    keep = (~out).nonzero()[:, 0]
+    t = torch.where(t == -100, t, keep[t % len(keep)])
+    h[:, 0], w[:, 0] = 1.0, 0.0
+    within = torch.where(t == -100, t, torch.searchsorted(keep, t.clamp_min(0)))
+    want = R.vocab(h, w[keep], within, weight, -100)
+    w[out, 0] = torch.finfo(dtype).min if low == "lowest" else -math.inf
+    loss, lse = clear.vocab_loss(h, w, t)
+    R.close(loss, want[0])
+    R.close(lse, want[1])
+    dh, dw = clear.vocab_loss_grad(h, w, t, lse, weight)
+    assert not dw[out].any()
+    R.close(dw[keep], want[3])
+    if low == "lowest":  # (a slope of zero times -inf is no number in dh's own product)
+        R.close(dh, want[2])
+
+
+def test_vocab_all_entries_alike_at_the_ends():
+    """Rows whose logits are all the type's lowest, or all its largest, value."""
+    ends = torch.tensor([torch.finfo(BF).min, torch.finfo(BF).max], device="cuda").to(BF)
+    h, w = torch.zeros(2, 64, dtype=BF, device="cuda"), torch.zeros(500, 64, dtype=BF, device="cuda")
+    h[:, 0], w[:, 0] = ends, 1.0
+    loss, lse = clear.vocab_loss(h, w, torch.tensor([3, 499], device="cuda"))
+    # log 500 is below a unit in the last place of 3.4e38
+    assert torch.equal(lse, ends.float()) and not loss.any()
