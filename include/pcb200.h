@@ -931,8 +931,8 @@ int64_t pcb_clear_vocab_loss_ws(const PcbClearVocab* a);
 int pcb_clear_vocab_loss(const PcbClearVocab* a, void* ws, size_t ws_bytes, cudaStream_t s);
 
 /* The gradients of sum_r weight[r] loss[r]: dl[r][v] = weight[r] (exp(l[r][v] - lse[r]) - [v = targets[r]]), 0 on ignored
- * rows; dh = dl w (rows x dim), dw = dl^T h (vocab x dim), formed over pieces of the vocabulary. lse from the forward
- * call; loss is not read. */
+ * rows, whatever their h and lse hold (dw still takes their h times 0: NaN where h is not finite); dh = dl w (rows x dim),
+ * dw = dl^T h (vocab x dim), formed over pieces of the vocabulary. lse from the forward call; loss is not read. */
 typedef struct PcbClearVocabGrad {
     PcbClearVocab v;
     const float* weight;

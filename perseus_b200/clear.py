@@ -267,7 +267,8 @@ def vocab_loss(h, w, targets, ignore=-100):
 def vocab_loss_grad(h, w, targets, lse, weight, ignore=-100, needs=(True, True)):
     """The gradients (dh, dw), of h's and w's shape and type, of sum_r weight[r] loss[r] (weight [rows] float32: 1 /
     count for the mean); lse from vocab_loss on the same h and w. The logits are formed again, a piece of the vocabulary
-    at a time. needs: which of the two are wanted, the other is None."""
+    at a time. An ignored row's dh is 0 whatever the row holds; its h has to be finite for dw. needs: which of the two are
+    wanted, the other is None."""
     args, keep = _vocab_args("vocab_loss_grad", h, w, targets, lse, None, ignore)
     rows, dim = h.shape
     for name, t in (("lse", lse), ("weight", weight)):

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(1024) prepare_rows(PcbClearVocab a, const floa
     if (i >= a.rows) return;
     const int64_t t = a.targets[i];
     rows[i] = VocabRow{a.lse[i], t == a.ignore ? 0.0f : weight[i] * scale,
-                       t >= 0 && t < a.vocab ? (int32_t)t : -1, 0};
+                       t >= 0 && t < a.vocab ? (int32_t)t : -1, t == a.ignore && !isfinite(a.lse[i])};
 }
 // y = factor * (the sum of `slices` matrices x of pitch `from`, in order), rounded
 __global__ void __launch_bounds__(256) finish(const float* x, int slices, int64_t rows, int cols, int64_t from, const float* factor, void* y,

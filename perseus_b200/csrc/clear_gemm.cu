@@ -441,10 +441,12 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
             const int chunks = min(S::COLS / W, max(0, (p.n - first + W - 1) / W));
             float top = -INFINITY, sum = 0.0f, lse = 0.0f, weight = 0.0f;
             int target = -1;  // the row's column among this warp's, if it is there
+            bool off = false, any_off = false;
             if (EPI == KERNEL_DL && row < p.m) {
                 const VocabRow vr = p.rows[row];
-                lse = vr.lse, weight = vr.weight, target = vr.target - p.col0 - first;
+                lse = vr.lse, weight = vr.weight, target = vr.target - p.col0 - first, off = vr.off;
             }
+            if (EPI == KERNEL_DL) any_off = __any_sync(~0u, off);
             if (EPI == KERNEL_LSE && row < p.m) {
                 const int64_t at = p.targets[row] - first;
                 target = at >= 0 && at < S::COLS ? (int)at : -1;
@@ -562,6 +564,10 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                     if (has_target) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) v[j] = target == W * c + j ? v[j] - weight : v[j];
+                    }
+                    if (any_off) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) v[j] = off ? 0.0f : v[j];
                     }
                 }
                 if (EPI == KERNEL_DZ && p.row_sums) {

@@ -24,7 +24,7 @@ enum Epilogue {
 struct VocabRow {
     float lse, weight;
     int32_t target;  // -1: none
-    int32_t pad;
+    int32_t off;     // an ignored row whose lse is not finite: its slopes are 0, not 0 x NaN
 };
 
 struct Gemm {

@@ -138,3 +138,16 @@ def test_vocab_all_entries_alike_at_the_ends():
     loss, lse = clear.vocab_loss(h, w, torch.tensor([3, 499], device="cuda"))
     # log 500 is below a unit in the last place of 3.4e38
     assert torch.equal(lse, ends.float()) and not loss.any()
+
+
+def test_vocab_ignored_rows_that_are_not_finite():
+    """dl is 0 on ignored rows, whatever their hidden states and lse hold: dh there is 0 and the other rows' stays."""
+    h, w, t, weight = vocab_case(200, 900, 64, BF)
+    want = R.vocab(h, w, t, weight, -100)
+    h[1], h[5, 3], h[9, 0] = math.nan, math.inf, -math.inf
+    assert (t[[1, 5, 9]] == -100).all()
+    loss, lse = clear.vocab_loss(h, w, t)
+    assert not loss[[1, 5, 9]].any() and not torch.isfinite(lse[[1, 5, 9]]).any()
+    dh, _ = clear.vocab_loss_grad(h, w, t, lse, weight, needs=(True, False))
+    assert not dh[1::4].any()
+    R.close(dh, want[2])
