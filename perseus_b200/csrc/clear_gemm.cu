@@ -132,12 +132,14 @@ __device__ __forceinline__ f32x2 half_erfc(f32x2 z, f32x2 size, f32x2& gauss) {
     return mul2(mul2(q, t), gauss);
 }
 __device__ __forceinline__ f32x2 gelu2(f32x2 z) {
-    float z0, z1;
+    float z0, z1, f0, f1;
     parts(z, z0, z1);
-    const f32x2 size = two(fabsf(z0), fabsf(z1));
     f32x2 g;
-    const f32x2 h = half_erfc(z, size, g);
-    return fma2(mul2(size, both(-1.0f)), h, two(fmaxf(z0, 0.0f), fmaxf(z1, 0.0f)));
+    const f32x2 h = half_erfc(z, two(fabsf(z0), fabsf(z1)), g);
+    // |z| h at +inf is 0: a finite value for it there (-inf and NaN go through to NaN)
+    asm("min.NaN.f32 %0, %1, 0f7F7FFFFF;" : "=f"(f0) : "f"(z0));
+    asm("min.NaN.f32 %0, %1, 0f7F7FFFFF;" : "=f"(f1) : "f"(z1));
+    return fma2(two(-fabsf(f0), -fabsf(f1)), h, two(fmaxf(z0, 0.0f), fmaxf(z1, 0.0f)));
 }
 __device__ __forceinline__ f32x2 gelu_slope2(f32x2 z) {
     float z0, z1, r0, r1;

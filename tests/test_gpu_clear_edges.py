@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from perseus_b200 import _lib as L
 from perseus_b200 import attention as A
 from perseus_b200 import clear
 from tests import _clear_ref as R
@@ -151,3 +152,20 @@ def test_vocab_ignored_rows_that_are_not_finite():
     dh, _ = clear.vocab_loss_grad(h, w, t, lse, weight, needs=(True, False))
     assert not dh[1::4].any()
     R.close(dh, want[2])
+
+
+# ------------------------------------------------------------------------------------------------ linear
+@pytest.mark.parametrize("m,k,n,splits", [(200, 136, 328, False), (9, 8192, 768, True)])
+@pytest.mark.parametrize("out", [BF, F32], ids=str)
+def test_linear_gelu_of_infinity(m, k, n, splits, out):
+    """z Phi(z) of +inf is +inf, of NaN and (0 times inf) of -inf NaN; with the sums of k in parts and whole."""
+    x, w = rnd(1, m, k), rnd(2, k, n, std=k**-0.5)
+    w[5] = w[5].abs() + 0.01
+    x[1, 5], x[3, 5], x[4, 6] = math.inf, -math.inf, math.nan
+    need = L.lib().pcb_clear_linear_ws(L.ClearLinear(x.data_ptr(), w.data_ptr(), None, None, x.data_ptr(), k, n, 0, n, m, k, n, 0,
+                                                     0, 0, 0, 0, 1, 1.0))
+    assert (need > 0) == splits
+    y = clear.linear(x, w, act="gelu", out_dtype=out)
+    assert (y[1] == math.inf).all() and torch.isnan(y[3:5]).all()
+    rows = [i for i in range(m) if i not in (1, 3, 4)]
+    R.close(y[rows], R.linear(x[rows], w, None, "gelu", None, out))
