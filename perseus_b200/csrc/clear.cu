@@ -10,10 +10,13 @@ namespace pcb {
 namespace clear {
 
 // ------------------------------------------------------------------------------------------------ column sums
-// Sums over the rows of a matrix, in two launches of fixed order: 256 rows of 64 columns per block (a warp along the columns,
-// two per lane, eight row lanes joined in shared memory), then the blocks' sums the same way. The first may run beside the
+// Sums over the rows of a matrix, in two launches of fixed order: 256 rows of 64 columns per block, more where a grid would
+// have over 65535 blocks along the rows (a warp along the columns, two per lane, eight row lanes joined in shared memory),
+// then the blocks' sums the same way. The first may run beside the
 // product launched before it, from which it reads nothing (`beside`): it then waits for that one only before it ends.
-constexpr int SUM_ROWS = 256, SUM_ONCE = 1024;  // up to SUM_ONCE rows one launch does: beside a product it costs no time
+constexpr int SUM_ONCE = 1024;  // up to SUM_ONCE rows one launch does: beside a product it costs no time
+constexpr int sum_rows_of(int m) { return std::max(256, m / 65535 + 1); }
+constexpr int sum_parts(int m) { return m / sum_rows_of(m) + (m % sum_rows_of(m) != 0); }
 __global__ void __launch_bounds__(256) sum_rows(const void* x, int64_t pitch, int type, int m, int n, int rows, float* part, void* out,
                                                 int out_type, bool beside) {
     __shared__ float2 red[8][32];
@@ -58,8 +61,8 @@ __global__ void __launch_bounds__(256) sum_rows(const void* x, int64_t pitch, in
     if (beside) pdl_wait();  // later launches may rely on everything before this one
 }
 int run_sum(const void* x, int64_t pitch, int type, int m, int n, float* part, void* out, int out_type, bool beside, cudaStream_t s) {
-    const dim3 g((n + 63) / 64, part ? (m + SUM_ROWS - 1) / SUM_ROWS : 1);
-    launch_pdl(sum_rows, g, dim3(256), s, x, pitch, type, m, n, part ? SUM_ROWS : m, part, out, out_type, beside);
+    const dim3 g((n + 63) / 64, part ? sum_parts(m) : 1);
+    launch_pdl(sum_rows, g, dim3(256), s, x, pitch, type, m, n, part ? sum_rows_of(m) : m, part, out, out_type, beside);
     return PCB_LAUNCH_RESULT();
 }
 
@@ -213,8 +216,7 @@ GradWs grad_ws(const PcbClearLinearGrad* a, void* ws) {
     r.w = c.take<char>(a->dx || a->act ? aligned_bytes(a->w, a->w_pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n) : 0);
     r.dz_pitch = ((int64_t)a->n + 7) / 8 * 8;
     r.dz = c.take<uint16_t>(a->act ? (size_t)a->m * r.dz_pitch : 0);
-    const int rows = a->act ? 32 : SUM_ROWS;
-    r.sums = c.take<float>(a->db ? (size_t)((a->m + rows - 1) / rows) * a->n : 0);
+    r.sums = c.take<float>(a->db ? ((size_t)(a->act ? ((int64_t)a->m + 31) / 32 : sum_parts(a->m)) * a->n) : 0);
     const size_t px = a->dx ? gemm_partial(a->m, a->k, a->n) : 0;
     const size_t pw = !a->dw ? 0 : a->w_cols ? gemm_partial(a->n, a->k, a->m) : gemm_partial(a->k, a->n, a->m);
     r.partial = c.take<float>(px > pw ? px : pw);  // the products run one after the other
@@ -342,7 +344,7 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
         const bool once = a->m <= SUM_ONCE;
         if (int rc = run_sum(a->dy, a->dy_pitch, a->type, a->m, a->n, once ? nullptr : w.sums, a->db, a->db_type, a->dx != nullptr, s)) return rc;
         if (!once)
-            if (int rc = run_sum(w.sums, a->n, PCB_F32, (a->m + SUM_ROWS - 1) / SUM_ROWS, a->n, nullptr, a->db, a->db_type, false, s)) return rc;
+            if (int rc = run_sum(w.sums, a->n, PCB_F32, sum_parts(a->m), a->n, nullptr, a->db, a->db_type, false, s)) return rc;
     }
     if (!a->dw) return 0;
     const Operand xr{x.p, x.pitch, false}, dr{dz.p, dz.pitch, false};

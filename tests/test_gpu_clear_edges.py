@@ -169,3 +169,18 @@ def test_linear_gelu_of_infinity(m, k, n, splits, out):
     assert (y[1] == math.inf).all() and torch.isnan(y[3:5]).all()
     rows = [i for i in range(m) if i not in (1, 3, 4)]
     R.close(y[rows], R.linear(x[rows], w, None, "gelu", None, out))
+
+
+def test_linear_grad_more_rows_than_a_launch_has_blocks():
+    """Column sums of more than 65535 x 256 rows, of whole numbers whose sums are exact in 32 bits."""
+    m = 65535 * 256 + 258
+    x, w, row = rnd(1, m, 8, dtype=HF), rnd(2, 8, 3, dtype=HF), torch.arange(m, device="cuda")
+    dy = torch.stack([row % 4 == 0, row >= m - 1000, row % 2 == 0], 1).to(HF)
+    dy[:, 2] = 1 - 2 * dy[:, 2]
+    b = torch.zeros(3, device="cuda")
+    for needs in ((False, False, True), (True, False, True)):
+        dx, _, db = clear.linear_grad(dy, x, w, bias=b, needs=needs)
+        assert torch.equal(db, dy.double().sum(0).float())
+    for part in (slice(0, 1000), slice(m - 1000, m)):
+        want = dy[part].double() @ w.double().t()
+        R.close(dx[part], (want, (2.0**-11 + 8 * R.S) * (dy[part].double().abs() @ w.double().abs().t())))
