@@ -66,6 +66,40 @@ int run_sum(const void* x, int64_t pitch, int type, int m, int n, float* part, v
     return PCB_LAUNCH_RESULT();
 }
 
+// The largest finite size of a float16 matrix's values, one per block: a warp along a row, eight adjacent values per lane
+// where the rows lie on 16 bytes. The operand dz of a gradient is scaled by it (linear_grad below).
+constexpr int SIZE_BLOCKS = 296;
+__global__ void __launch_bounds__(1024) largest(const uint16_t* x, int64_t pitch, int m, int n, float* sizes) {
+    __shared__ uint32_t red[32];
+    pdl_wait();
+    pdl_release();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const bool wide = ((uintptr_t)x & 15) == 0 && pitch % 8 == 0;
+    uint32_t big = 0;
+    auto take = [&](uint32_t bits) {
+        bits &= 0x7FFF;
+        if (bits < 0x7C00) big = max(big, bits);
+    };
+    for (int64_t r = blockIdx.x * 32ll + warp; r < m; r += gridDim.x * 32ll) {
+        const uint16_t* row = x + r * pitch;
+        const int whole = wide ? n / 8 * 8 : 0;
+#pragma unroll 4
+        for (int c = 8 * lane; c < whole; c += 256) {
+            const uint4 q = *(const uint4*)(row + c);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) take(w[i]), take(w[i] >> 16);
+        }
+        for (int c = whole + lane; c < n; c += 32) take(row[c]);
+    }
+    big = __reduce_max_sync(~0u, big);
+    if (lane == 0) red[warp] = big;
+    __syncthreads();
+    if (warp) return;
+    big = __reduce_max_sync(~0u, red[lane]);
+    if (lane == 0) sizes[blockIdx.x] = __half2float(__ushort_as_half((unsigned short)big));
+}
+
 // zeros: the gradients of no rows
 __global__ void __launch_bounds__(256) zero_rows(void* y, int64_t rows, int64_t cols, int64_t pitch, int type) {
     pdl_wait();
@@ -205,7 +239,7 @@ struct GradWs {
     size_t bytes;
     void *dy, *x, *w, *dz;
     int64_t dz_pitch;
-    float *sums, *partial;
+    float *sums, *partial, *sizes, *unscale;  // sizes, unscale: null unless dz is scaled
 };
 GradWs grad_ws(const PcbClearLinearGrad* a, void* ws) {
     Carve c(ws);
@@ -220,6 +254,9 @@ GradWs grad_ws(const PcbClearLinearGrad* a, void* ws) {
     const size_t px = a->dx ? gemm_partial(a->m, a->k, a->n) : 0;
     const size_t pw = !a->dw ? 0 : a->w_cols ? gemm_partial(a->n, a->k, a->m) : gemm_partial(a->k, a->n, a->m);
     r.partial = c.take<float>(px > pw ? px : pw);  // the products run one after the other
+    const bool scaled = a->act && products && a->type == PCB_F16;
+    r.sizes = scaled ? c.take<float>(SIZE_BLOCKS) : nullptr;
+    r.unscale = scaled ? c.take<float>(1) : nullptr;
     r.bytes = c.used;
     return r;
 }
@@ -322,7 +359,11 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
     if (a->dx || a->act) rows[nrows++] = Rows{&wt.p, &wt.pitch, a->w_cols ? a->n : a->k, a->w_cols ? a->k : a->n, w.w};
     if (!a->act && (a->dx || a->dw)) rows[nrows++] = Rows{&dz.p, &dz.pitch, a->m, a->n, w.dy};
     if (int rc = align_rows(rows, nrows, s)) return rc;
-    if (a->act) {  // dz, and the sums of its rows from the same 32-bit values
+    if (a->act) {
+        // dz in 16 bits (its one rounding: the products with x and W take 16-bit operands), and the sums of its rows from the
+        // same 32-bit values. dy of a mean over thousands of rows lies where float16 has few bits left or none, so dz is
+        // scaled by a power of two that brings the largest dy, times the largest slope, to 2^8: 2^-22 of it still has all
+        // bits, and slopes past the polynomial's bound have a factor of 256 left. The products are scaled back in 32 bits.
         Gemm g = product_of(x, wt, a->m, a->n, a->k, a->type);
         g.epi = EPI_DZ;
         g.y = w.dz, g.y_pitch = w.dz_pitch;
@@ -330,6 +371,14 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
         g.bias = a->bias, g.bias_type = a->bias_type;
         g.extra = a->dy, g.extra_pitch = a->dy_pitch, g.extra_type = a->type;
         g.row_sums = a->db ? w.sums : nullptr;
+        if (w.sizes) {
+            const int blocks = std::min(a->m / 32 + 1, SIZE_BLOCKS);
+            launch_pdl(largest, dim3(blocks), dim3(1024), s, (const uint16_t*)a->dy, a->dy_pitch, a->m, a->n, w.sizes);
+            if (int rc = PCB_LAUNCH_RESULT()) return rc;
+            g.sizes = w.sizes, g.nsizes = blocks, g.unscale = w.unscale;
+            g.slope = a->act == PCB_ACT_GELU ? 1.13f : 0.0f;
+            for (int i = 0; i < 7; ++i) g.slope += std::fabs(g.act.d[i]);
+        }
         if (int rc = gemm(g, s)) return rc;
         dz = Operand{w.dz, w.dz_pitch, true};
         if (a->db)
@@ -337,7 +386,7 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
     }
     if (a->dx) {
         Gemm g = product_of(dz, Operand{wt.p, wt.pitch, a->w_cols == 0}, a->m, a->k, a->n, a->type);
-        g.y = a->dx, g.y_pitch = a->dx_pitch, g.partial = w.partial;
+        g.y = a->dx, g.y_pitch = a->dx_pitch, g.partial = w.partial, g.alpha = w.unscale;
         if (int rc = gemm(g, s)) return rc;
     }
     if (a->db && !a->act) {  // beside the product before it, if there is one
@@ -349,7 +398,7 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
     if (!a->dw) return 0;
     const Operand xr{x.p, x.pitch, false}, dr{dz.p, dz.pitch, false};
     Gemm g = a->w_cols ? product_of(dr, xr, a->n, a->k, a->m, a->type) : product_of(xr, dr, a->k, a->n, a->m, a->type);
-    g.y = a->dw, g.y_pitch = a->dw_pitch, g.partial = w.partial;
+    g.y = a->dw, g.y_pitch = a->dw_pitch, g.partial = w.partial, g.alpha = w.unscale;
     return gemm(g, s);
 }
 

@@ -78,6 +78,10 @@ struct alignas(64) Params {
     int bias_type, extra_type, y_type, y_tma, extra_mode, accumulate;
     const float* alpha;
     float* row_sums;
+    const float* sizes;
+    int nsizes;
+    float slope;
+    float* unscale;
     const VocabRow* rows;
     int col0;
     const int64_t* targets;
@@ -391,6 +395,16 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
         unsigned char* in = stage + (S::BUFFERS - 1) * S::STAGING;  // `extra`'s boxes: 32 rows x 128 bytes, the next one on its way
         float* bias = bias_s + ew * 32;
         const float alpha = p.alpha ? *p.alpha : 1.0f;
+        float factor = 1.0f;
+        if (EPI == KERNEL_DZ && p.sizes) {
+            float big = 0.0f;
+            for (int i = lane; i < p.nsizes; i += 32) big = fmaxf(big, p.sizes[i]);
+            for (int i = 16; i; i >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, i));
+            big *= p.slope;
+            const int e = big > 0.0f ? max(-100, min(100, 134 - (int)(__float_as_uint(big) >> 23))) : 0;  // big in [2^(7-e), 2^(8-e))
+            factor = __uint_as_float((127 + e) << 23);
+            if (blockIdx.x == 0 && ew == 0 && lane == 0) *p.unscale = __uint_as_float((127 - e) << 23);
+        }
         const uint32_t leader_empty[2] = {CTAS == 2 ? cluster_addr(&acc_empty[0], 0) : 0, CTAS == 2 ? cluster_addr(&acc_empty[1], 0) : 0};
         auto release = [&](int buf) {  // this warp has the accumulator's values
             fence_before();
@@ -578,6 +592,10 @@ __global__ void __launch_bounds__(Shape<BN, CTAS, EPI>::THREADS, 1) product(cons
                     for (int j = 0; j < W; ++j) t[j] = row < p.m ? v[j] : 0.0f;  // rows past the end hold anything
                     const float s = lane_sums<W>(t);
                     if (lane < W && col0 + lane < p.n && row0 < p.m) p.row_sums[(int64_t)(row0 / 32) * p.n + col0 + lane] = s;
+                }
+                if (EPI == KERNEL_DZ) {
+#pragma unroll
+                    for (int j = 0; j < W; j += 2) parts(mul2(two(v[j], v[j + 1]), both(factor)), v[j], v[j + 1]);
                 }
                 // ---- to memory: the lane's row of 128 bytes in the staging buffer, 16-byte pieces swizzled by the row: 64
                 // columns of 16 bits or 32 of 32 fill it
@@ -892,7 +910,7 @@ int gemm(const Gemm& g, cudaStream_t s) {
     p.act = g.act, p.bias = g.bias, p.bias_type = g.bias_type;
     p.extra = g.extra, p.extra_pitch = g.extra_pitch, p.extra_type = g.extra_type;
     p.y_ptr = g.y, p.y_pitch = g.y_pitch, p.y_type = g.y_type, p.accumulate = g.accumulate;
-    p.alpha = g.alpha, p.row_sums = g.row_sums, p.rows = g.rows, p.col0 = g.col0, p.targets = g.targets, p.parts = g.parts, p.hit = g.hit;
+    p.alpha = g.alpha, p.row_sums = g.row_sums, p.sizes = g.sizes, p.nsizes = g.nsizes, p.slope = g.slope, p.unscale = g.unscale, p.rows = g.rows, p.col0 = g.col0, p.targets = g.targets, p.parts = g.parts, p.hit = g.hit;
     const size_t eb = type_bytes(p.y_type);
     // 16-byte aligned rows go through the TMA engine; others by rows of the staging buffer
     p.y_tma = g.epi != EPI_LSE && ((uintptr_t)p.y_ptr & 15) == 0 && p.y_pitch * eb % 16 == 0;

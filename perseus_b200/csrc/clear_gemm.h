@@ -15,7 +15,8 @@ struct Operand {
 
 enum Epilogue {
     EPI_STORE,  // y = alpha * (act(D + bias) + extra)
-    EPI_DZ,     // y = extra * act'(D + bias), and the sums of each 32 rows of its columns in 32 bits
+    EPI_DZ,     // y = extra * act'(D + bias), times a power of two if `sizes` is given, and the sums of each 32 rows of its
+                // columns in 32 bits (without that factor)
     EPI_LSE,    // the maximum and the sum of exponentials of each row of a column block, the target's logit
     EPI_DL,     // y = weight (exp(D - lse) - [n = target])
 };
@@ -45,6 +46,10 @@ struct Gemm {
     int extra_type;
     const float* alpha;     // one value on the device, or null
     float* row_sums;        // EPI_DZ: [ceil(m / 32)][n], or null
+    const float* sizes;     // EPI_DZ: `nsizes` values of which the largest, times `slope`, the factor brings to [2^7, 2^8), or null
+    int nsizes;
+    float slope;
+    float* unscale;         // EPI_DZ with `sizes`: one over the factor
     const VocabRow* rows;   // EPI_DL
     int col0;               // EPI_DL: the vocabulary entry of this product's first column
     const int64_t* targets; // EPI_LSE

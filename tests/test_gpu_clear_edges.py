@@ -8,11 +8,13 @@ import torch
 from perseus_b200 import _lib as L
 from perseus_b200 import attention as A
 from perseus_b200 import clear
+from perseus_b200 import model as M
 from tests import _clear_ref as R
 
 pytestmark = pytest.mark.gpu
 
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+GELU_POLY = clear.Poly(tuple(M.gelu_poly(3.0)), 3.0)
 
 
 def rnd(seed, *shape, std=1.0, dtype=BF):
@@ -169,6 +171,42 @@ def test_linear_gelu_of_infinity(m, k, n, splits, out):
     assert (y[1] == math.inf).all() and torch.isnan(y[3:5]).all()
     rows = [i for i in range(m) if i not in (1, 3, 4)]
     R.close(y[rows], R.linear(x[rows], w, None, "gelu", None, out))
+
+
+def grad_bounds(dy, x, w, bias, kind):
+    """R.linear_grad's bounds where dz, as an operand in float16, errs by its rounding and by no more than 2^-32 of the
+    largest dy times the largest slope that any z within the polynomial's bound (GELU: any z) has."""
+    most = 1.13 if kind == "gelu" else sum(i * abs(c) / kind.bound for i, c in enumerate(kind.coeffs))
+    want = R.linear_grad(dy, x, w, bias, kind, F32)
+    less = R.TINY[HF] - 2.0**-32 * float(dy.double().abs().max()) * most
+    wd, xd = w.double().abs(), x.double().abs()
+    return [(want[0][0], want[0][1] - less * wd.sum(1)), (want[1][0], want[1][1] - less * xd.sum(0)[:, None]), want[2]]
+
+
+@pytest.mark.parametrize("act", ["gelu", GELU_POLY], ids=["gelu", "poly"])
+@pytest.mark.parametrize("size", [1e-6, 1e-4])
+@pytest.mark.parametrize("m,k,n", [(3000, 96, 264), (70, 1024, 1000)])
+def test_linear_grad_small_dy_in_float16(act, size, m, k, n):
+    """Gradients of a mean over many rows: dz stays far below float16's normal range while sums over the rows do not."""
+    x, w = rnd(1, m, k, dtype=HF), rnd(2, k, n, std=0.5 * k**-0.5, dtype=HF)
+    b, dy = rnd(3, n, std=0.2, dtype=F32), rnd(4, m, n, std=size, dtype=HF)
+    for got, want in zip(clear.linear_grad(dy, x, w, bias=b, act=act), grad_bounds(dy, x, w, b, act)):
+        R.close(got, want)
+
+
+def test_linear_grad_large_dy_in_float16():
+    """dz beyond float16's range between operands and results that are within it."""
+    m, n = 300, 136
+    x, w = rnd(1, m, 64, std=0.01, dtype=HF), rnd(2, 64, n, std=0.02, dtype=HF)
+    x[:, 0], w[0] = 1.0, 1.4  # z about 1.4, where GELU's slope is 1.129
+    dy = torch.where(torch.arange(m, device="cuda")[:, None] % 2 == 0, 60000.0, -60000.0).to(HF).repeat(1, n)
+    b = torch.zeros(n, device="cuda")
+    assert (R.slope(x.double() @ w.double(), "gelu") * 60000 > 65520).all()
+    _, dw, db = clear.linear_grad(dy, x, w, bias=b, act="gelu", needs=(False, True, True))
+    want = grad_bounds(dy, x, w, b, "gelu")
+    assert want[1][0].abs().max() < 65504
+    R.close(dw, want[1])
+    R.close(db, want[2])
 
 
 def test_linear_grad_more_rows_than_a_launch_has_blocks():
