@@ -104,7 +104,8 @@ def fit_step(r, targets, tail, cfg, ignore=-100, poly=True):
     """One step's loss and gradients of the tail on residual streams r [rows, d] (float32: a layer's input to its second
     LayerNorm, of prefilled prompts or decrypted): y = r + MLP(LayerNorm(r)), the mean cross entropy of y against the head
     over the targets that are not `ignore`. Returns (loss, {"head", "w_up", "b_up", "w_down", "b_down"}): a scalar tensor
-    and the gradients, nothing updated."""
+    and the gradients, nothing updated. Gradients are of the weights' types, or float32 for float16 layers: a mean over
+    many rows leaves float16's normal range, so those are formed of a multiple of the loss and divided after."""
     w = tail.layer
     act = clear.Poly(M.gelu_poly(cfg.gelu_bound), cfg.gelu_bound) if poly else "gelu"
     n = _norm(r, cfg.norm, poly).to(w.w_up.dtype)
@@ -112,8 +113,15 @@ def fit_step(r, targets, tail, cfg, ignore=-100, poly=True):
     y = clear.linear(u, w.w_down, bias=w.b_down, residual=r)
     loss, lse = clear.vocab_loss(y, tail.head, targets, ignore)
     scored = (targets != ignore).float()
-    weight = scored / scored.sum().clamp_min(1.0)
-    dy, dhead = clear.vocab_loss_grad(y, tail.head, targets, lse, weight, ignore)
+    count = scored.sum().clamp_min(1.0)
+    weight = scored / count
+    # float16 ends at 65504 and loses bits below 2^-14: 64 leaves room for gradients of 1000, and for rows by the thousands
+    half = y.dtype is torch.float16
+    scale = count.clamp_max(64.0)
+    dy, dhead = clear.vocab_loss_grad(y, tail.head, targets, lse, weight * scale if half else weight, ignore)
     du, dw_down, db_down = clear.linear_grad(dy, u, w.w_down, bias=w.b_down)
     _, dw_up, db_up = clear.linear_grad(du, n, w.w_up, bias=w.b_up, act=act, needs=(False, True, True))
-    return (loss * weight).sum(), {"head": dhead, "w_up": dw_up, "b_up": db_up, "w_down": dw_down, "b_down": db_down}
+    grads = {"head": dhead, "w_up": dw_up, "b_up": db_up, "w_down": dw_down, "b_down": db_down}
+    if half:
+        grads = {n: g.float() / scale for n, g in grads.items()}
+    return (loss * weight).sum(), grads

@@ -2,6 +2,7 @@
 of tests/_clear_ref.py."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -9,6 +10,7 @@ from perseus_b200 import _lib as L
 from perseus_b200 import attention as A
 from perseus_b200 import clear
 from perseus_b200 import model as M
+from perseus_b200 import prefill as PF
 from tests import _clear_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -222,3 +224,30 @@ def test_linear_grad_more_rows_than_a_launch_has_blocks():
     for part in (slice(0, 1000), slice(m - 1000, m)):
         want = dy[part].double() @ w.double().t()
         R.close(dx[part], (want, (2.0**-11 + 8 * R.S) * (dy[part].double().abs() @ w.double().abs().t())))
+
+
+# ------------------------------------------------------------------------------------------------ fitting in float16
+@pytest.mark.parametrize("poly", [True, False], ids=["poly", "exact"])
+def test_fit_step_in_float16(poly):
+    """The gradients of a mean over many rows in float16 layers against 64-bit autograd: within a few units of 2^-11 of
+    each gradient's size."""
+    cfg = M.ModelCfg(layers=1, d=128, width=128, heads=2, head_dim=64, mlp=512, tokens=64)
+    layer = PF.load([M.random_layer(np.random.default_rng(1), 128, 512)], dtype=HF)[0]
+    tail = PF.Tail(layer, rnd(1, 500, 128, std=0.02, dtype=HF))
+    rows = 4096
+    r = rnd(2, rows, 128, dtype=F32)
+    t = torch.randint(0, 500, (rows,), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda")
+    t[::9] = -100
+    loss, grads = PF.fit_step(r, t, tail, cfg, poly=poly)
+    p = {n: getattr(layer, n).double().requires_grad_() for n in ("w_up", "b_up", "w_down", "b_down")}
+    p["head"] = tail.head.double().requires_grad_()
+    act = clear.Poly(M.gelu_poly(cfg.gelu_bound), cfg.gelu_bound) if poly else "gelu"
+    n = PF._norm(r.double(), cfg.norm, poly)
+    y = R.act(n @ p["w_up"] + p["b_up"], act) @ p["w_down"] + p["b_down"] + r.double()
+    want = torch.nn.functional.cross_entropy(y @ p["head"].t(), t, ignore_index=-100)
+    want.backward()
+    assert abs(float(loss) - want.item()) < 16 * 2.0**-11 * want.item()
+    for name, g in grads.items():
+        assert g.dtype == F32
+        d = p[name].grad
+        assert (g.double() - d).norm() <= 16 * 2.0**-11 * d.norm(), name
