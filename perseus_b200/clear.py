@@ -91,6 +91,13 @@ def _weight(w):
     return w.contiguous(), n, 0
 
 
+def _flat(name, t):
+    """[..., c] as rows, also where there are none."""
+    if not isinstance(t, torch.Tensor) or t.dim() < 1:
+        raise ValueError(f"{name}: a CUDA tensor [..., columns]")
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
 def _launch(op, args, like):
     dev = like.get_device()
     if dev != torch.cuda.current_device():
@@ -116,10 +123,8 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
     """act(x w + bias) + residual for x [..., k], w [k, n] (a transposed view of an [n, k] matrix is read as it lies).
     act: None, "gelu" (z Phi(z)) or a Poly. bias [n] and residual [..., n] are of x's type or float32; the result is of
     `out_dtype`: x's type (default) or float32."""
-    if not isinstance(x, torch.Tensor) or x.dim() < 1:
-        raise ValueError("linear: x is a CUDA tensor [..., k]")
-    flat = x.dim() == 2
-    x2 = x if flat else x.reshape(-1, x.shape[-1])
+    x2 = _flat("x", x)
+    flat = x2 is x
     _is("x", x2, None, 2)
     _is("w", w, x2, 2)
     m, k = x2.shape
@@ -140,7 +145,7 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
         bias_ptr, bias_type = bias.data_ptr(), _TYPE[bias.dtype]
     if residual is not None:
         _aside("residual", residual, x2, (m, n) if flat else x.shape[:-1] + (n,))
-        residual, res_pitch = _rows(residual if flat else residual.reshape(-1, n))
+        residual, res_pitch = _rows(_flat("residual", residual))
         res_ptr, res_type = residual.data_ptr(), _TYPE[residual.dtype]
     x2, x_pitch = _rows(x2)
     w, w_pitch, w_cols = _weight(w)
@@ -157,9 +162,7 @@ def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
     gradient is dy itself). The product x w + bias is formed again where there is an activation, so the forward call keeps
     nothing. dx is of x's shape, dw of w's (laid out as w is), both of x's type; db [n] is of bias's type, None without a
     bias. needs: which of the three are wanted, the others are None."""
-    if not isinstance(x, torch.Tensor) or x.dim() < 1:
-        raise ValueError("linear_grad: x is a CUDA tensor [..., k]")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    x2 = _flat("x", x)
     _is("x", x2, None, 2)
     _is("w", w, x, 2)
     m, k = x2.shape
@@ -168,7 +171,7 @@ def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
         raise ValueError(f"linear_grad: x {tuple(x.shape)} against w {tuple(w.shape)}")
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape[:-1] + (n,):
         raise ValueError(f"linear_grad: dy of shape {tuple(x.shape[:-1]) + (n,)}")
-    dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n)
+    dy2 = _flat("dy", dy)
     _is("dy", dy2, x, 2)
     kind, bound, coef = _act(act)
     if bias is not None:

@@ -226,6 +226,17 @@ def test_linear_grad_more_rows_than_a_launch_has_blocks():
         R.close(dx[part], (want, (2.0**-11 + 8 * R.S) * (dy[part].double().abs() @ w.double().abs().t())))
 
 
+def test_linear_empty_shapes_of_more_dimensions():
+    x, w = rnd(1, 2, 3, 32), rnd(2, 32, 48)
+    y = clear.linear(x, w[:, :0], residual=rnd(3, 2, 3, 0), bias=rnd(4, 0))
+    assert y.shape == (2, 3, 0)
+    assert clear.linear(x[:, :0], w, residual=rnd(3, 2, 0, 48)).shape == (2, 0, 48)
+    for call in (lambda: clear.linear(x[..., :0], w[:0]), lambda: clear.linear_grad(rnd(1, 2, 3, 48), x[..., :0], w[:0]),
+                 lambda: clear.linear_grad(rnd(1, 2, 3, 0), x, w[:, :0])):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ------------------------------------------------------------------------------------------------ fitting in float16
 @pytest.mark.parametrize("poly", [True, False], ids=["poly", "exact"])
 def test_fit_step_in_float16(poly):
