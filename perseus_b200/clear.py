@@ -91,6 +91,15 @@ def _weight(w):
     return w.contiguous(), n, 0
 
 
+_MOST = 2**31 - 1025
+
+
+def _sizes(op, *sizes):
+    """The entries count in 32 bits; ctypes would cut what is beyond."""
+    if max(sizes) > _MOST:
+        raise ValueError(f"{op}: sizes of at most {_MOST}, got {sizes}")
+
+
 def _flat(name, t):
     """[..., c] as rows, also where there are none."""
     if not isinstance(t, torch.Tensor) or t.dim() < 1:
@@ -131,6 +140,7 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None):
     kw, n = w.shape
     if kw != k or k < 1:
         raise ValueError(f"linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
+    _sizes("linear", m, k, n)
     if out_dtype is None:
         out_dtype = x.dtype
     elif out_dtype is not x.dtype and out_dtype is not torch.float32:
@@ -169,6 +179,7 @@ def linear_grad(dy, x, w, bias=None, act=None, needs=(True, True, True)):
     n = w.shape[1]
     if w.shape[0] != k or k < 1 or n < 1:
         raise ValueError(f"linear_grad: x {tuple(x.shape)} against w {tuple(w.shape)}")
+    _sizes("linear_grad", m, k, n)
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape[:-1] + (n,):
         raise ValueError(f"linear_grad: dy of shape {tuple(x.shape[:-1]) + (n,)}")
     dy2 = _flat("dy", dy)
@@ -218,6 +229,8 @@ def prompt_attention(q, k, v, q_lens, k_lens=None, scale=None, causal=True, weig
     nseq = len(q_lens)
     if len(k_lens) != nseq:
         raise ValueError(f"prompt_attention: {nseq} q_lens, {len(k_lens)} k_lens")
+    if nseq and (max(max(q_lens), max(k_lens)) > _MOST or min(min(q_lens), min(k_lens)) < -_MOST):
+        raise ValueError(f"prompt_attention: lengths of at most {_MOST}")
     coef = () if weights is None else tuple(weights)
     if weights is not None and not 1 <= len(coef) <= 8:
         raise ValueError(f"prompt_attention: 1 to 8 coefficients, got {len(coef)}")
@@ -242,6 +255,7 @@ def _vocab_args(who, h, w, targets, lse, loss, ignore):
     rows, dim = h.shape
     if w.shape[1] != dim or dim < 1 or w.shape[0] < 1:
         raise ValueError(f"{who}: h {tuple(h.shape)} against w {tuple(w.shape)}")
+    _sizes(who, rows, w.shape[0], dim)
     if targets.shape != (rows,) or targets.dtype != torch.int64 or targets.device != h.device:
         raise ValueError(f"{who}: targets of shape ({rows},) in int64 on {h.device}, got {tuple(targets.shape)} of "
                          f"{targets.dtype} on {targets.device}")
@@ -259,6 +273,7 @@ def vocab_loss(h, w, targets, ignore=-100):
     other target outside the vocabulary gives NaN). The logits are never stored whole."""
     _is("h", h, None, 2)
     rows = h.shape[0]
+    _sizes("vocab_loss", rows)
     loss = h.new_empty(rows, dtype=torch.float32)
     lse = h.new_empty(rows, dtype=torch.float32)
     args, keep = _vocab_args("vocab_loss", h, w, targets, lse, loss, ignore)

@@ -46,6 +46,8 @@ inline Act make_act(int kind, float bound, const float* coef) {
 }
 
 // ------------------------------------------------------------------------------------------------ checks
+// The largest size: rows and columns of tiles that reach past the last one are counted in 32 bits
+constexpr int32_t MOST = INT32_MAX - 1024;
 inline bool is16(int type) { return type == PCB_BF16 || type == PCB_F16; }
 inline bool known(int type, int call) { return type == call || type == PCB_F32; }
 inline bool poly_ok(int kind, float bound, const float* coef) {
@@ -57,7 +59,8 @@ inline bool poly_ok(int kind, float bound, const float* coef) {
 }
 inline int bad_linear(const PcbClearLinear* a) {
     if (!a) return report(PCB_BAD_ARGS, "clear_linear: null arguments");
-    if (a->m < 0 || a->k < 1 || a->n < 0) return report(PCB_BAD_ARGS, "clear_linear: m %d, k %d, n %d", a->m, a->k, a->n);
+    if (a->m < 0 || a->k < 1 || a->n < 0 || a->m > MOST || a->k > MOST || a->n > MOST)
+        return report(PCB_BAD_ARGS, "clear_linear: m %d, k %d, n %d", a->m, a->k, a->n);
     if (!is16(a->type)) return report(PCB_BAD_ARGS, "clear_linear: type %d is not PCB_BF16 or PCB_F16", a->type);
     if (a->act < 0 || a->act > PCB_ACT_POLY || !poly_ok(a->act, a->bound, a->coef))
         return report(PCB_BAD_ARGS, "clear_linear: act %d, bound %g", a->act, (double)a->bound);
@@ -73,7 +76,7 @@ inline int bad_linear(const PcbClearLinear* a) {
 }
 inline int bad_grad(const PcbClearLinearGrad* a) {
     if (!a) return report(PCB_BAD_ARGS, "clear_linear_grad: null arguments");
-    if (a->m < 0 || a->k < 1 || a->n < 1)
+    if (a->m < 0 || a->k < 1 || a->n < 1 || a->m > MOST || a->k > MOST || a->n > MOST)
         return report(PCB_BAD_ARGS, "clear_linear_grad: m %d, k %d, n %d", a->m, a->k, a->n);
     if (!is16(a->type)) return report(PCB_BAD_ARGS, "clear_linear_grad: type %d is not PCB_BF16 or PCB_F16", a->type);
     if (a->act < 0 || a->act > PCB_ACT_POLY || !poly_ok(a->act, a->bound, a->coef))
@@ -99,8 +102,7 @@ inline int bad_attention(const PcbClearAttention* a) {
     for (int i = 0; i < a->ncoef; ++i)
         if (!std::isfinite(a->coef[i])) return report(PCB_BAD_ARGS, "clear_attention: coefficient %d is not finite", i);
     if (a->nseq > 0 && (!a->q_lens || !a->k_lens)) return report(PCB_BAD_ARGS, "clear_attention: null lengths");
-    if (a->q_rows > INT32_MAX || a->k_rows > INT32_MAX)
-        return report(PCB_BAD_ARGS, "clear_attention: over 2^31 - 1 tokens");
+    if (a->q_rows > MOST || a->k_rows > MOST) return report(PCB_BAD_ARGS, "clear_attention: over %d tokens", MOST);
     int64_t qs = 0, ks = 0;
     for (int b = 0; b < a->nseq; ++b) {
         if (a->q_lens[b] < 0 || a->k_lens[b] < 0)
@@ -121,7 +123,7 @@ inline int bad_attention(const PcbClearAttention* a) {
 inline int bad_vocab(const PcbClearVocab* a, bool grad) {
     const char* who = grad ? "clear_vocab_grad" : "clear_vocab_loss";
     if (!a) return report(PCB_BAD_ARGS, "%s: null arguments", who);
-    if (a->rows < 0 || a->vocab < 1 || a->dim < 1)
+    if (a->rows < 0 || a->vocab < 1 || a->dim < 1 || a->rows > MOST || a->vocab > MOST || a->dim > MOST)
         return report(PCB_BAD_ARGS, "%s: %d rows, vocabulary of %d, dim %d", who, a->rows, a->vocab, a->dim);
     if (!is16(a->type)) return report(PCB_BAD_ARGS, "%s: type %d is not PCB_BF16 or PCB_F16", who, a->type);
     if (a->rows > 0 && (!a->h || !a->w || !a->targets || !a->lse || (!grad && !a->loss)))

@@ -237,6 +237,22 @@ def test_linear_empty_shapes_of_more_dimensions():
             call()
 
 
+def test_sizes_beyond_31_bits_are_refused():
+    """No size reaches the entries cut to 32 bits."""
+    one = torch.ones(1, 1, dtype=BF, device="cuda")
+    many, few = one.expand(2**32 + 5, 1), rnd(1, 5, 1)
+    t, v = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, device="cuda")
+    q = rnd(2, 10, 1, 64)
+    for call in (lambda: clear.linear(many, one), lambda: clear.linear(one, many.t()), lambda: clear.linear(many.t(), many),
+                 lambda: clear.linear_grad(many, many, one), lambda: clear.linear_grad(many.t(), one, many.t()),
+                 lambda: clear.linear_grad(one, many.t(), many), lambda: clear.vocab_loss(one, many, t),
+                 lambda: clear.vocab_loss(many, few, t.expand(2**32 + 5)),
+                 lambda: clear.vocab_loss_grad(one, many, t, v, v),
+                 lambda: clear.prompt_attention(q, q, q, [2**32 + 10]), lambda: clear.prompt_attention(q, q, q, [10], [10 - 2**32])):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ------------------------------------------------------------------------------------------------ fitting in float16
 @pytest.mark.parametrize("poly", [True, False], ids=["poly", "exact"])
 def test_fit_step_in_float16(poly):
