@@ -50,6 +50,8 @@ inline Act make_act(int kind, float bound, const float* coef) {
 constexpr int32_t MOST = INT32_MAX - 1024;
 inline bool is16(int type) { return type == PCB_BF16 || type == PCB_F16; }
 inline bool known(int type, int call) { return type == call || type == PCB_F32; }
+// a pointer that is not a multiple of its elements' size
+inline bool off(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 inline bool poly_ok(int kind, float bound, const float* coef) {
     if (kind != PCB_ACT_POLY) return true;
     if (!(bound > 0.0f) || !std::isfinite(bound)) return false;
@@ -69,6 +71,9 @@ inline int bad_linear(const PcbClearLinear* a) {
         return report(PCB_BAD_ARGS, "clear_linear: bias, residual and y are of the call's type or PCB_F32");
     if (a->m == 0 || a->n == 0) return 0;
     if (!a->x || !a->w || !a->y) return report(PCB_BAD_ARGS, "clear_linear: null x, w or y");
+    if (off(a->x, 2) || off(a->w, 2) || off(a->y, type_bytes(a->y_type)) || off(a->bias, a->bias ? type_bytes(a->bias_type) : 1) ||
+        off(a->residual, a->residual ? type_bytes(a->residual_type) : 1))
+        return report(PCB_BAD_ARGS, "clear_linear: a pointer is off its elements' size");
     if (a->x_pitch < a->k || a->w_pitch < (a->w_cols ? a->k : a->n) || a->y_pitch < a->n ||
         (a->residual && a->residual_pitch < a->n))
         return report(PCB_BAD_ARGS, "clear_linear: a pitch is below its row's elements");
@@ -84,6 +89,9 @@ inline int bad_grad(const PcbClearLinearGrad* a) {
     if ((a->bias && !known(a->bias_type, a->type)) || (a->db && !known(a->db_type, a->type)))
         return report(PCB_BAD_ARGS, "clear_linear_grad: bias and db are of the call's type or PCB_F32");
     if (a->m > 0 && (!a->dy || !a->x || !a->w)) return report(PCB_BAD_ARGS, "clear_linear_grad: null dy, x or w");
+    if (off(a->dy, 2) || off(a->x, 2) || off(a->w, 2) || off(a->dx, 2) || off(a->dw, 2) ||
+        off(a->bias, a->bias ? type_bytes(a->bias_type) : 1) || off(a->db, a->db ? type_bytes(a->db_type) : 1))
+        return report(PCB_BAD_ARGS, "clear_linear_grad: a pointer is off its elements' size");
     const int64_t wrow = a->w_cols ? a->k : a->n;
     if ((a->m > 0 && (a->dy_pitch < a->n || a->x_pitch < a->k || a->w_pitch < wrow)) || (a->dx && a->dx_pitch < a->k) ||
         (a->dw && a->dw_pitch < wrow))
@@ -115,6 +123,8 @@ inline int bad_attention(const PcbClearAttention* a) {
                       (long long)ks, (long long)a->q_rows, (long long)a->k_rows);
     if ((qs && (!a->q || !a->out)) || (qs && ks && (!a->k || !a->v)))
         return report(PCB_BAD_ARGS, "clear_attention: null q, k, v or out");
+    if (off(a->q, 2) || off(a->k, 2) || off(a->v, 2) || off(a->out, 2))
+        return report(PCB_BAD_ARGS, "clear_attention: a pointer is off its elements' size");
     const int64_t strides[] = {a->q_pitch, a->q_head, a->k_pitch, a->k_head, a->v_pitch, a->v_head, a->out_pitch, a->out_head};
     for (int64_t st : strides)
         if (st < 0) return report(PCB_BAD_ARGS, "clear_attention: negative stride");
@@ -128,6 +138,8 @@ inline int bad_vocab(const PcbClearVocab* a, bool grad) {
     if (!is16(a->type)) return report(PCB_BAD_ARGS, "%s: type %d is not PCB_BF16 or PCB_F16", who, a->type);
     if (a->rows > 0 && (!a->h || !a->w || !a->targets || !a->lse || (!grad && !a->loss)))
         return report(PCB_BAD_ARGS, "%s: null h, w, targets, lse or loss", who);
+    if (off(a->h, 2) || off(a->w, 2) || off(a->targets, 8) || off(a->loss, 4) || off(a->lse, 4))
+        return report(PCB_BAD_ARGS, "%s: a pointer is off its elements' size", who);
     if (a->rows > 0 && (a->h_pitch < a->dim || a->w_pitch < a->dim))
         return report(PCB_BAD_ARGS, "%s: a pitch is below its row's elements", who);
     return 0;
@@ -136,6 +148,8 @@ inline int bad_vocab_grad(const PcbClearVocabGrad* a) {
     if (!a) return report(PCB_BAD_ARGS, "clear_vocab_grad: null arguments");
     if (int rc = bad_vocab(&a->v, true)) return rc;
     if (a->v.rows > 0 && !a->weight) return report(PCB_BAD_ARGS, "clear_vocab_grad: null weight");
+    if (off(a->weight, 4) || off(a->dh, 2) || off(a->dw, 2))
+        return report(PCB_BAD_ARGS, "clear_vocab_grad: a pointer is off its elements' size");
     if ((a->dh && a->dh_pitch < a->v.dim) || (a->dw && a->dw_pitch < a->v.dim))
         return report(PCB_BAD_ARGS, "clear_vocab_grad: a pitch is below its row's elements");
     return 0;
