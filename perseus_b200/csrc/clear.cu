@@ -366,7 +366,7 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
         // bits, and slopes past the polynomial's bound have a factor of 256 left. The products are scaled back in 32 bits.
         Gemm g = product_of(x, wt, a->m, a->n, a->k, a->type);
         g.epi = EPI_DZ;
-        g.y = w.dz, g.y_pitch = w.dz_pitch;
+        g.y = w.dz, g.y_pitch = w.dz_pitch, g.padded = true;
         g.act = make_act(a->act, a->bound, a->coef);
         g.bias = a->bias, g.bias_type = a->bias_type;
         g.extra = a->dy, g.extra_pitch = a->dy_pitch, g.extra_type = a->type;
@@ -445,12 +445,12 @@ int pcb_clear_vocab_grad(const PcbClearVocabGrad* a, void* ws, size_t ws_bytes, 
         const void* wp = (const char*)wt.p + 2 * (int64_t)v0 * wt.pitch;
         Gemm g = product_of(h, Operand{wp, wt.pitch, true}, v.rows, cols, v.dim, v.type);
         g.epi = EPI_DL;
-        g.y = w.slopes, g.y_pitch = w.slope_pitch, g.rows = w.rows, g.col0 = v0;
+        g.y = w.slopes, g.y_pitch = w.slope_pitch, g.padded = true, g.rows = w.rows, g.col0 = v0;
         if (int rc = gemm(g, s)) return rc;
         if (a->dh) {
             g = product_of(Operand{w.slopes, w.slope_pitch, true}, Operand{wp, wt.pitch, false}, v.rows, v.dim, cols, v.type);
             if (whole) g.y = a->dh, g.y_pitch = a->dh_pitch, g.alpha = w.unscale, g.partial = w.partial;
-            else g.y = w.dh, g.y_pitch = w.dh_pitch, g.y_type = PCB_F32, g.slices = w.slices, g.accumulate = v0 > 0;
+            else g.y = w.dh, g.y_pitch = w.dh_pitch, g.y_type = PCB_F32, g.padded = true, g.slices = w.slices, g.accumulate = v0 > 0;
             if (int rc = gemm(g, s)) return rc;
         }
         if (a->dw) {

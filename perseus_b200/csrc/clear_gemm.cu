@@ -912,8 +912,9 @@ int gemm(const Gemm& g, cudaStream_t s) {
     p.y_ptr = g.y, p.y_pitch = g.y_pitch, p.y_type = g.y_type, p.accumulate = g.accumulate;
     p.alpha = g.alpha, p.row_sums = g.row_sums, p.sizes = g.sizes, p.nsizes = g.nsizes, p.slope = g.slope, p.unscale = g.unscale, p.rows = g.rows, p.col0 = g.col0, p.targets = g.targets, p.parts = g.parts, p.hit = g.hit;
     const size_t eb = type_bytes(p.y_type);
-    // 16-byte aligned rows go through the TMA engine; others by rows of the staging buffer
-    p.y_tma = g.epi != EPI_LSE && ((uintptr_t)p.y_ptr & 15) == 0 && p.y_pitch * eb % 16 == 0;
+    // 16-byte aligned rows go through the TMA engine, which writes whole 16 bytes: where a row's last ones are not all its own,
+    // and in rows off 16 bytes, results go by rows of the staging buffer
+    p.y_tma = g.epi != EPI_LSE && ((uintptr_t)p.y_ptr & 15) == 0 && p.y_pitch * eb % 16 == 0 && (g.padded || g.n * eb % 16 == 0);
     if (p.y_tma) {
         const uint64_t size[3] = {(uint64_t)g.n, (uint64_t)g.m, (uint64_t)(g.slices ? g.slices : 1)};
         const uint64_t stride[2] = {(uint64_t)p.y_pitch * eb, (uint64_t)p.y_pitch * eb * g.m};

@@ -36,6 +36,7 @@ struct Gemm {
     void* y;
     int64_t y_pitch;
     int y_type;
+    bool padded;      // y is scratch: its rows may be written past n up to the pitch
     int slices;       // EPI_STORE into 32 bits: > 0: k in this many parts, part i's sums at y + i m y_pitch
     bool accumulate;  // with slices: y += (one writer per element; a part without k is left as it is)
     Act act;

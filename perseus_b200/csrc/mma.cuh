@@ -12,7 +12,8 @@ namespace mma {
 
 // ------------------------------------------------------------------------------------------------ TMA, tiled
 // The box at (x, y) of a two-dimensional map; x times the element size is a multiple of 16 bytes. What lies outside the
-// tensor reads as zero (loads) or is not written (stores).
+// tensor reads as zero (loads) or is not written (stores; but along x they write whole 16 bytes: a tensor whose inner size
+// is no multiple of them has to own what follows in the last).
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(

@@ -226,6 +226,52 @@ def test_linear_grad_more_rows_than_a_launch_has_blocks():
         R.close(dx[part], (want, (2.0**-11 + 8 * R.S) * (dy[part].double().abs() @ w.double().abs().t())))
 
 
+def inside(t, pitch):
+    """(a matrix of t's shape within rows of `pitch`, whether everything around it is untouched)"""
+    whole = torch.full((t.shape[0] + 1, pitch), 77.0, dtype=t.dtype, device="cuda")
+    at = whole[:t.shape[0], :t.shape[1]]
+
+    def untouched():
+        return bool((whole[:, t.shape[1]:] == 77.0).all() and (whole[-1] == 77.0).all())
+    return at, untouched
+
+
+@pytest.mark.parametrize("m,k,n,pitch", [(200, 72, 129, 136), (1, 64, 1, 8), (300, 1100, 271, 272), (9, 8192, 765, 768), (600, 64, 8, 16)])
+@pytest.mark.parametrize("out", [BF, F32], ids=str)
+def test_linear_into_columns_of_a_wider_matrix(m, k, n, pitch, out):
+    """The C entry's results in aligned rows that go on after them: nothing past a row's last column is written."""
+    x, w = rnd(1, m, k), rnd(2, k, n, std=k**-0.5)
+    want = R.linear(x, w, None, None, None, out)
+    y, untouched = inside(want[0].to(out), pitch)
+    clear._launch("linear", L.ClearLinear(x.data_ptr(), w.data_ptr(), None, None, y.data_ptr(), k, n, 0, pitch, m, k, n, 0, 0, 0, 0,
+                                          0 if out == BF else 2, 0, 1.0), x)
+    R.close(y, want)
+    assert untouched()
+
+
+@pytest.mark.parametrize("act", [None, "gelu"], ids=["none", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(70, 33, 45), (600, 129, 257)])
+def test_gradients_into_columns_of_wider_matrices(act, m, k, n):
+    x, w, dy = rnd(1, m, k), rnd(2, k, n, std=k**-0.5), rnd(3, m, n)
+    want = R.linear_grad(dy, x, w, None, act, F32)
+    up = lambda c: c // 8 * 8 + 8  # noqa: E731
+    (dx, dx_ok), (dw, dw_ok) = inside(x, up(k)), inside(w, up(n))
+    clear._launch("linear_grad", L.ClearLinearGrad(dy.data_ptr(), x.data_ptr(), w.data_ptr(), None, dx.data_ptr(), dw.data_ptr(), None,
+                                                   n, k, n, up(k), up(n), m, k, n, 0, 0, 0, 0, 0 if act is None else 1, 1.0), x)
+    R.close(dx, want[0])
+    R.close(dw, want[1])
+    assert dx_ok() and dw_ok()
+    h, v, t, weight = vocab_case(m, 1003, k, BF)
+    loss, lse = clear.vocab_loss(h, v, t)
+    want = R.vocab(h, v, t, weight, -100)
+    (dh, dh_ok), (dv, dv_ok) = inside(h, up(k)), inside(v, up(k))
+    args = L.ClearVocab(h.data_ptr(), v.data_ptr(), t.data_ptr(), None, lse.data_ptr(), k, k, -100, m, 1003, k, 0)
+    clear._launch("vocab_grad", L.ClearVocabGrad(args, weight.data_ptr(), dh.data_ptr(), dv.data_ptr(), up(k), up(k)), h)
+    R.close(dh, want[2])
+    R.close(dv, want[3])
+    assert dh_ok() and dv_ok()
+
+
 def test_linear_empty_shapes_of_more_dimensions():
     x, w = rnd(1, 2, 3, 32), rnd(2, 32, 48)
     y = clear.linear(x, w[:, :0], residual=rnd(3, 2, 3, 0), bias=rnd(4, 0))
