@@ -18,8 +18,8 @@
 // Few rows against many keys (single tokens) split the keys over several blocks, joined in order by `join_splits`.
 //
 // A key block may reach into the next sequence, or hold keys that some rows do not see: their weights are zero, but zero
-// times a value that is not finite is not zero. So rows whose result is not finite are computed again, key by key over
-// the keys that they see (`attend_row`): exact semantics at no cost where all values are finite.
+// times a value that is not finite is not zero. So rows whose result is not finite, and not for the keys that they see,
+// are computed again key by key over those (`redo`): exact semantics at no cost where all values are finite.
 #include <algorithm>
 #include <cstring>
 
@@ -49,7 +49,7 @@ struct Work {
 };
 struct alignas(64) Params {
     CUtensorMap q, k, v;
-    PcbClearAttention a;  // the operands as they lie, for attend_row
+    PcbClearAttention a;  // the operands as they lie, for redo
     int group, tokens;    // query heads of a K/V head, tokens of a 128-row tile
     int splits;
     float c;              // scores to base-2 exponents: |scale| log2 e
@@ -57,7 +57,7 @@ struct alignas(64) Params {
     float coef[8];        // of the raw scores, the largest of the polynomial's own brought to 1
     float out_scale;
     float* part_o;        // splits > 1: [split][q row][head][dim] sums, and (maximum in base 2, sum of weights)
-    float2* part_ml;      // of a split whose visible scores are all -inf: (-inf, -1); of one that the row does not see: (-inf, 0)
+    float2* part_ml;
     int out_vec;          // out's rows take 16-byte stores
     Work w;
 };
@@ -74,57 +74,212 @@ struct Shape {
 };
 constexpr int THREADS = 224;  // loads, scores, sums, and four warps with a row per thread
 
-// ------------------------------------------------------------------------------------------------ one row, key by key
-// A warp computes out = sum of weights x values over keys [j0, j1) of one query in 32 bits: lane l holds dims l + 32 t.
-// Returns the unnormalised sums, the maximum (base 2) and the sum of the weights.
-__device__ __noinline__ void attend_row(const PcbClearAttention& a, int64_t qrow, int head, int64_t k0, int j0, int j1, float c,
-                                        float* o, float* top_out, float* sum_out) {
-    const int lane = threadIdx.x % 32, kh = head / (a.heads / a.kv_heads);
-    float q[4], top = -INFINITY, sum = 0.0f;
-    for (int t = 0; t < 4; ++t) {
-        const int d = lane + 32 * t;
-        q[t] = d < a.dim ? load(a.q, qrow * a.q_pitch + head * a.q_head + d, a.type) : 0.0f;
-        o[t] = 0.0f;
+// A block's tile: the sequence (its rows q0.. and keys k0..), the K/V head, the tokens from t0 (the last ones first), the key blocks
+struct Tile {
+    int split, kh, nq, nk, q0, k0, t0, seen, b0, n;
+};
+__device__ __forceinline__ Tile tile_of(const Params& p) {
+    Tile w;
+    w.split = blockIdx.x % p.splits;
+    const int item = blockIdx.x / p.splits, tile = item / p.a.kv_heads;
+    w.kh = item % p.a.kv_heads;
+    int lo = 0, hi = p.w.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.w.tile0[mid] <= tile) lo = mid;
+        else hi = mid;
     }
-    for (int j = j0; j < j1; ++j) {
-        const int64_t kr = k0 + j;
-        float s = 0.0f;
-        for (int t = 0; t < 4; ++t) {
-            const int d = lane + 32 * t;
-            if (d < a.dim) s = fmaf(q[t], load(a.k, kr * a.k_pitch + kh * a.k_head + d, a.type), s);
+    w.nq = p.w.nq[lo], w.nk = p.w.nk[lo], w.q0 = p.w.q0[lo], w.k0 = p.w.k0[lo];
+    w.t0 = (p.w.tile0[lo + 1] - 1 - tile) * p.tokens;
+    w.seen = p.a.causal ? min(w.nk, max(0, min(w.nq, w.t0 + p.tokens) + w.nk - w.nq)) : w.nk;  // keys of the last token
+    const int blocks = (w.seen + KEYS - 1) / KEYS, per = (blocks + p.splits - 1) / p.splits;
+    w.b0 = min(blocks, w.split * per), w.n = min(blocks, w.b0 + per) - w.b0;
+    return w;
+}
+// Row r of a tile: its token, its query head, and how many keys it sees (0: not a row)
+__device__ __forceinline__ void row_of(const Params& p, const Tile& w, int r, int& tok, int& head, int& limit) {
+    tok = w.t0 + r / p.group, head = w.kh * p.group + r % p.group;
+    limit = r >= p.group * p.tokens || tok >= w.nq ? 0 : p.a.causal ? min(w.nk, max(0, tok + w.nk - w.nq + 1)) : w.nk;
+}
+
+// What a split leaves to the join: the maximum and the sum of its weights. (-inf, 0) where the row sees none of its keys, (-inf,
+// -1) where all scores that it sees are -inf, (-inf, NaN) where the sum is NaN: so is the row, wherever the others' maxima lie.
+__device__ __forceinline__ float2 part_of(bool blind, float top, float sum) {
+    return make_float2(blind || sum != sum ? -INFINITY : top, blind ? 0.0f : sum == 0.0f ? -1.0f : sum);
+}
+
+// ------------------------------------------------------------------------------------------------ rows again, key by key
+// A warp looks at its rows of `again`, whose result is not finite though (under softmax) the sum of their weights is positive.
+// Where keys that a row sees account for that, it stands: every dim that is not finite has a value that is not in V (under
+// polynomial weights also a key or the query itself). The others, which hold 0 x Inf of keys that they do not see, or an overflow,
+// are computed once more, each over those of the block's keys that it sees and nothing else, in 32 bits: two rows at a time,
+// which share the loads, and 32 keys: lane l has key l's scores and weights, then dims l + 32 t of the sums. 8192 tokens, 12 heads
+// over 4, Inf in the 1st value 1.1 ms, in the 4096th 9.8 ms (all rows after it computed again key by key: 468 and 403 ms).
+template <int DP, bool POLY>
+__device__ __forceinline__ void redo(const Params& p, uint32_t again) {
+    constexpr int R = 2, T = DP / 32;  // four rows: 30 % less here, but the whole kernel 1 to 3 % slower
+    const PcbClearAttention& a = p.a;
+    const Tile w = tile_of(p);
+    const int lane = threadIdx.x % 32, kh = w.kh, j0 = w.b0 * KEYS, j1 = (w.b0 + w.n) * KEYS;
+    const int64_t q0 = w.q0, k0 = w.k0;
+    const bool bf16 = a.type == PCB_BF16;
+    int tok, head, limit;
+    row_of(p, w, threadIdx.x / 32 % 4 * 32 + lane, tok, head, limit);
+    {
+        int first_v[T], first_k = INT32_MAX, last = j0;  // the first keys with a value that is not finite: of each dim, of any
+        for (uint32_t i = again; i; i &= i - 1) last = max(last, min(j1, __shfl_sync(~0u, limit, __ffs(i) - 1)));
+        const uint16_t exponent = bf16 ? 0x7F80 : 0x7C00;
+        auto first = [&](const void* x, int64_t pitch, int64_t at, int t) {  // eight keys' loads at a time
+            const uint16_t* col = (const uint16_t*)x + k0 * pitch + at + min(lane + 32 * t, a.dim - 1);
+            int found = INT32_MAX;
+            for (int j = j0; j < last; j += 8) {
+                uint16_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = col[min(j + e, last - 1) * pitch];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((v[e] & exponent) == exponent) found = min(found, j + e);
+            }
+            return found;
+        };
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            first_v[t] = first(a.v, a.v_pitch, kh * a.v_head, t);
+            if (POLY) first_k = min(first_k, first(a.k, a.k_pitch, kh * a.k_head, t));
         }
-        for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(~0u, s, m);
-        float p;
-        if (a.ncoef) {
-            s *= a.scale;
-            p = a.coef[a.ncoef - 1];
-            for (int i = a.ncoef - 2; i >= 0; --i) p = fmaf(p, s, a.coef[i]);
-        } else {
-            s = (a.scale < 0.0f ? -s : s) * c;
-            const float nt = fmaxf(top, s), f = top == -INFINITY ? 0.0f : exp2f(top - nt);
-            p = nt == -INFINITY ? (s == s ? 0.0f : s) : exp2f(s - nt);
-            sum = sum * f + p;
-            for (int t = 0; t < 4; ++t) o[t] *= f;
-            top = nt;
-        }
-        for (int t = 0; t < 4; ++t) {
-            const int d = lane + 32 * t;
-            if (d < a.dim) o[t] = fmaf(p, load(a.v, kr * a.v_pitch + kh * a.v_head + d, a.type), o[t]);
+        first_k = __reduce_min_sync(~0u, first_k);
+        for (uint32_t i = again; i; i &= i - 1) {
+            const int src = __ffs(i) - 1, lim = __shfl_sync(~0u, limit, src), hd = __shfl_sync(~0u, head, src);
+            const int64_t qr = q0 + __shfl_sync(~0u, tok, src), row = ((int64_t)w.split * a.q_rows + qr) * a.heads + hd;
+            bool scores = POLY && first_k < lim, unexplained = false;  // a score that is not finite: with two coefficients, all dims
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int d = lane + 32 * t;
+                if (d >= a.dim) continue;
+                if (POLY) scores |= !isfinite(load(a.q, qr * a.q_pitch + hd * a.q_head + d, a.type));
+                const float y = p.splits > 1 ? p.part_o[row * a.dim + d] : load(a.out, qr * a.out_pitch + hd * a.out_head + d, a.type);
+                unexplained |= !isfinite(y) && first_v[t] >= lim;
+            }
+            if (!__any_sync(~0u, unexplained) || (__any_sync(~0u, scores) && a.ncoef > 1)) again &= ~(1u << src);
         }
     }
-    *top_out = top;
-    *sum_out = sum;
+    const bool wide = (((uintptr_t)a.q | (uintptr_t)a.k) & 15) == 0 && ((a.q_pitch | a.q_head | a.k_pitch | a.k_head | a.dim) & 7) == 0;
+    const uint16_t* v_col[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) v_col[t] = (const uint16_t*)a.v + k0 * a.v_pitch + kh * a.v_head + min(lane + 32 * t, a.dim - 1);
+    while (again) {
+        int64_t qr[R];
+        int hd[R], lim[R], end = j0;
+        bool live[R];
+        float o[R][T] = {}, top[R], sum[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int src = again ? __ffs(again) - 1 : 0;
+            live[r] = again != 0;
+            again &= again - 1;
+            qr[r] = q0 + __shfl_sync(~0u, tok, src);
+            hd[r] = __shfl_sync(~0u, head, src);
+            lim[r] = min(j1, __shfl_sync(~0u, limit, src));
+            if (!live[r]) qr[r] = qr[0], hd[r] = hd[0], lim[r] = j0;
+            end = max(end, lim[r]);
+            top[r] = -INFINITY, sum[r] = 0.0f;
+        }
+        for (int j = j0; j < end; j += 32) {
+            const int n = min(32, end - j);
+            float s[R] = {};
+            if (lane < n) {
+                const int64_t k_at = (k0 + j + lane) * a.k_pitch + kh * a.k_head;
+                if (wide) {
+#pragma unroll 4
+                    for (int d = 0; d < a.dim; d += 8) {
+                        const uint4 y = *(const uint4*)((const uint16_t*)a.k + k_at + d);
+                        const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const uint4 x = *(const uint4*)((const uint16_t*)a.q + qr[r] * a.q_pitch + hd[r] * a.q_head + d);
+                            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float u[2], v[2];
+                                unpack2(xs[i], bf16, u);
+                                unpack2(ys[i], bf16, v);
+                                s[r] = fmaf(u[1], v[1], fmaf(u[0], v[0], s[r]));
+                            }
+                        }
+                    }
+                } else {
+                    for (int d = 0; d < a.dim; ++d) {
+                        const float y = load(a.k, k_at + d, a.type);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) s[r] = fmaf(load(a.q, qr[r] * a.q_pitch + hd[r] * a.q_head + d, a.type), y, s[r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {  // scores to weights
+                if (POLY) {
+                    const float x = s[r] * a.scale;
+                    s[r] = a.coef[a.ncoef - 1];
+                    for (int i = a.ncoef - 2; i >= 0; --i) s[r] = fmaf(s[r], x, a.coef[i]);
+                } else {
+                    s[r] = j + lane < lim[r] ? (a.scale < 0.0f ? -s[r] : s[r]) * p.c : -INFINITY;
+                    float nt = s[r];
+                    for (int m = 16; m; m >>= 1) nt = fmaxf(nt, __shfl_xor_sync(~0u, nt, m));
+                    nt = fmaxf(top[r], nt);
+                    const float f = top[r] == -INFINITY ? 0.0f : exp2f(top[r] - nt);
+                    s[r] = nt == -INFINITY ? (s[r] == s[r] ? 0.0f : s[r]) : exp2f(s[r] - nt);
+                    float more = s[r];
+                    for (int m = 16; m; m >>= 1) more += __shfl_xor_sync(~0u, more, m);
+                    sum[r] = sum[r] * f + more;
+                    for (int t = 0; t < T; ++t) o[r][t] *= f;
+                    top[r] = nt;
+                }
+            }
+            for (int i = 0; i < n; i += 8) {  // eight keys' loads at a time
+                uint16_t v[8][T];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int t = 0; t < T; ++t) v[e][t] = v_col[t][min(j + i + e, end - 1) * a.v_pitch];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float weight = __shfl_sync(~0u, s[r], i + e);
+                        if (j + i + e < lim[r]) {
+#pragma unroll
+                            for (int t = 0; t < T; ++t) {
+                                const float x = bf16 ? __uint_as_float(v[e][t] << 16) : __half2float(__ushort_as_half(v[e][t]));
+                                o[r][t] = fmaf(weight, x, o[r][t]);
+                            }
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (!live[r]) continue;
+            const int64_t row = ((int64_t)w.split * a.q_rows + qr[r]) * a.heads + hd[r];
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int d = lane + 32 * t;
+                if (d >= a.dim) continue;
+                if (p.splits > 1) p.part_o[row * a.dim + d] = o[r][t];
+                else store(a.out, qr[r] * a.out_pitch + hd[r] * a.out_head + d, a.type, POLY ? o[r][t] : o[r][t] / sum[r]);
+            }
+            if (p.splits > 1 && lane == 0) p.part_ml[row] = part_of(false, top[r], sum[r]);
+        }
+    }
 }
 
 // 2^x for two values on the multiply-add pipe: the special-function pipe gives 16 exponentials per cycle and SM, half of what
 // the products need at 64 dims, so a quarter of them is computed here (8192 tokens, 12 heads over 4: 164 us without, 156 with
 // a quarter, 166 with half; at 128 dims the products take as long as the exponentials, and it costs 1 %). x = n + f with n the nearest integer (in the low bits of
 // x + 1.5 2^23), |f| <= 1/2; 2^f by the polynomial of least relative error of degree 4 (2.6e-6, a thousandth of the weights'
-// rounding), 2^n added to its exponent. x stays at -126 from below, and the result there is subtracted from all: a key that
-// is masked (x = -inf) or far below weighs exactly 0, or V values near bfloat16's largest would show through 2^-126. NaN gives
-// a value that is not finite in 16 bits.
+// rounding), times 2^n. x stays at -126 from below, and the result there is subtracted from all: a key that is masked (x = -inf)
+// or far below weighs exactly 0, or V values near bfloat16's largest would show through 2^-126. NaN stays NaN.
 __device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
-    float x0, x1, t0, t1, p0, p1;
+    float x0, x1, t0, t1;
     parts(x, x0, x1);
     asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x0) : "f"(x0));  // -126
     asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x1) : "f"(x1));
@@ -136,10 +291,8 @@ __device__ __forceinline__ f32x2 exp2_fma(f32x2 x) {
     p = fma2(p, f, both(0.6931217908859253f));
     p = fma2(p, f, both(0.9999992847442627f));
     parts(t, t0, t1);
-    parts(p, p0, p1);
-    const f32x2 e = two(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
-                        __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
-    return add2(e, both(__uint_as_float(0x807FFFF4u)));  // -0.9999992847442627 2^-126: f = 0, n = -126
+    const f32x2 n = two(__uint_as_float(0x3F800000u + (__float_as_uint(t0) << 23)), __uint_as_float(0x3F800000u + (__float_as_uint(t1) << 23)));
+    return fma2(p, n, both(__uint_as_float(0x807FFFFAu)));  // -0.9999992847442627 2^-126: f = 0, n = -126
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
@@ -187,29 +340,17 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     pdl_wait();
     pdl_release();
 
-    // ---- this block's tile: the sequence, the K/V head, the tokens from t0 (the last ones first), the key blocks
-    const int split = blockIdx.x % p.splits, item = blockIdx.x / p.splits;
-    const int tile = item / p.a.kv_heads, kh = item % p.a.kv_heads;
-    int lo = 0, hi = p.w.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.w.tile0[mid] <= tile) lo = mid;
-        else hi = mid;
-    }
-    const int nq = p.w.nq[lo], nk = p.w.nk[lo], q0 = p.w.q0[lo], k0 = p.w.k0[lo];
-    const int t0 = (p.w.tile0[lo + 1] - 1 - tile) * p.tokens, past = nk - nq;
-    const int t1 = min(nq, t0 + p.tokens);                                           // tokens [t0, t1)
-    const int seen = p.a.causal ? min(nk, max(0, t1 + past)) : nk;                    // keys of the last token
-    const int least = p.a.causal ? min(nk, max(0, t0 + past + 1)) : nk;               // and of the first
-    const int blocks = (seen + KEYS - 1) / KEYS, per = (blocks + p.splits - 1) / p.splits;
-    const int b0 = min(blocks, split * per), n = min(blocks, b0 + per) - b0;
-    const int steps = n > 0 ? (min(seen, (b0 + n) * KEYS) - b0 * KEYS + STEP - 1) / STEP : 0;  // products of 64 keys
+    const Tile w = tile_of(p);
+    const int kh = w.kh, k0 = w.k0, b0 = w.b0, n = w.n;
+    const int least = p.a.causal ? min(w.nk, max(0, w.t0 + w.nk - w.nq + 1)) : w.nk;               // keys of the first token
+    const int steps = n > 0 ? (min(w.seen, (b0 + n) * KEYS) - b0 * KEYS + STEP - 1) / STEP : 0;  // products of 64 keys
 
+    uint32_t again = 0;  // rows of a softmax warp that `redo` computes
     if (warp == 0) {
         if (n > 0) {
             if (elect()) {
                 mbar_expect(q_full, (DP / 64) * 128 * p.group * p.tokens);
-                for (int h = 0; h < DP / 64; ++h) tma_load(base + h * S::HALF, &p.q, 64 * h, kh * p.group, q0 + t0, q_full);
+                for (int h = 0; h < DP / 64; ++h) tma_load(base + h * S::HALF, &p.q, 64 * h, kh * p.group, w.q0 + w.t0, q_full);
             }
             __syncwarp();
             Ring<S::RING> rg;
@@ -297,9 +438,9 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
     } else {
         const int quad = warp % 4, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const int tok = t0 + r / p.group, head = kh * p.group + r % p.group;
-        const bool mine = r < p.group * p.tokens && tok < nq;
-        const int limit = !mine ? 0 : p.a.causal ? min(nk, max(0, tok + past + 1)) : nk;  // keys that this row sees
+        int tok, head, limit;
+        row_of(p, w, r, tok, head, limit);
+        const bool mine = r < p.group * p.tokens && tok < w.nq;
         const bool bf16 = p.a.type == PCB_BF16;
         float top = -INFINITY, sum = 0.0f;
         bool ok = true;
@@ -402,13 +543,13 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
         if (ok && steps > 0) ok = wait_warp(&pv_done[(steps - 1) % 2], (steps - 1) / 2 & 1, dead, &g_attn_timeouts);
         fence_after();
         if (ok) {
-            const int64_t qrow = q0 + tok;
+            const int64_t qrow = w.q0 + tok;
             // sees none of these keys: zeros, whatever the keys that other rows see have left in O (0 x Inf)
             const bool blind = limit <= b0 * KEYS;
             const float scale = POLY ? p.out_scale : p.splits > 1 ? 1.0f : 1.0f / sum;
-            const int64_t prow = ((int64_t)split * p.a.q_rows + qrow) * p.a.heads + head;
+            const int64_t prow = ((int64_t)w.split * p.a.q_rows + qrow) * p.a.heads + head;
             const int64_t orow = qrow * p.a.out_pitch + head * p.a.out_head;
-            bool odd = !blind && !(fabsf(sum) <= 3.4e38f);
+            bool odd = false;
 #pragma unroll 1
             for (int h = 0; h < DP / 32; ++h) {
                 float o[32];
@@ -438,28 +579,16 @@ __global__ void __launch_bounds__(THREADS, 2) attend(const __grid_constant__ Par
                         if (32 * h + i < p.a.dim) store(p.a.out, orow + 32 * h + i, p.a.type, o[i]);
                 }
             }
-            if (mine && p.splits > 1) p.part_ml[prow] = make_float2(blind ? -INFINITY : top, blind ? 0.0f : sum == 0.0f ? -1.0f : sum);
-            for (uint32_t again = __ballot_sync(~0u, mine && odd); again; again &= again - 1) {
-                const int src = __ffs(again) - 1;
-                const int tk = __shfl_sync(~0u, tok, src), hd = __shfl_sync(~0u, head, src), lim = __shfl_sync(~0u, limit, src);
-                const int64_t qr = q0 + tk;
-                float o[4], tp, sm;
-                attend_row(p.a, qr, hd, k0, min(lim, b0 * KEYS), min(lim, (b0 + n) * KEYS), p.c, o, &tp, &sm);
-                const int64_t pr = ((int64_t)split * p.a.q_rows + qr) * p.a.heads + hd;
-                for (int t = 0; t < 4; ++t) {
-                    const int d = lane + 32 * t;
-                    if (d >= p.a.dim) continue;
-                    if (p.splits > 1) p.part_o[pr * p.a.dim + d] = o[t];
-                    else store(p.a.out, qr * p.a.out_pitch + hd * p.a.out_head + d, p.a.type, POLY ? o[t] : o[t] / sm);
-                }
-                if (p.splits > 1 && lane == 0) p.part_ml[pr] = make_float2(tp, sm == 0.0f ? -1.0f : sm);
-            }
+            if (mine && p.splits > 1) p.part_ml[prow] = part_of(blind, top, sum);
+            // a sum of weights that is NaN, or 0, is the row's result (NaN): only keys that it sees take part in it
+            again = __ballot_sync(~0u, mine && odd && (POLY || sum > 0.0f));
         }
     }
     fence_before();
     __syncthreads();
     fence_after();
     if (warp == 1) tmem_free(tmem, S::TMEM);
+    if (again) redo<DP, POLY>(p, again);  // last, where nothing else lives in registers
 }
 
 // The splits of a row joined in order: a warp per (query, head)

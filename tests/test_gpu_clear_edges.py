@@ -99,6 +99,54 @@ def test_attention_blind_rows_beside_values_that_are_not_finite(weights, dim, ba
     R.close(got[:98], (want[0][:98], want[1][:98]))
 
 
+@pytest.mark.parametrize("weights", [None, tuple(A.softmax_poly(256))], ids=["softmax", "poly"])
+@pytest.mark.parametrize("dim,dtype", [(64, BF), (64, HF), (128, BF), (40, HF)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_attention_one_value_that_is_not_finite(weights, dim, dtype, bad):
+    """It reaches its own dim of the queries that see it and nothing else; a query or key that is not finite, its rows whole."""
+    n, at, d, scale = 700, 301, 5, dim**-0.5
+    q, k, v = rnd(1, n, 4, dim, std=0.5, dtype=dtype), rnd(2, n, 2, dim, std=0.5, dtype=dtype), rnd(3, n, 2, dim, dtype=dtype)
+    want = R.attention(q, k, v, [n], [n], scale, True, weights)
+    v[at, 1, d] = bad
+    got = clear.prompt_attention(q, k, v, [n], weights=weights)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[at:, 2:, d] = True
+    assert not torch.isfinite(got[hit]).any()
+    R.close(got[~hit], (want[0][~hit], want[1][~hit]))
+    v[at, 1, d] = 0.0
+    q[at, 1, d] = bad
+    k[at + 50, 1, d] = math.nan
+    want = R.attention(q, torch.where(torch.isnan(k), 0.0, k), v, [n], [n], scale, True, weights)
+    got = clear.prompt_attention(q, k, v, [n], weights=weights)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[at, 1] = hit[at + 50:, 2:] = True
+    assert not torch.isfinite(got[hit]).any()
+    R.close(got[~hit], (want[0][~hit], want[1][~hit]))
+
+
+@pytest.mark.parametrize("weights", [None, tuple(A.softmax_poly(256))], ids=["softmax", "poly"])
+def test_attention_time_with_values_that_are_not_finite(weights):
+    """Rows that see such a value are not computed again key by key, which would take some thousand times the call's time."""
+    n = 4096
+    q, k, v = rnd(1, n, 12, 64, std=0.5), rnd(2, n, 4, 64, std=0.5), rnd(3, n, 4, 64)
+
+    def ms():
+        best = math.inf
+        for _ in range(3):
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            e[0].record()
+            clear.prompt_attention(q, k, v, [n], weights=weights)
+            e[1].record()
+            torch.cuda.synchronize()
+            best = min(best, e[0].elapsed_time(e[1]))
+        return best
+    clean = ms()
+    v[1] = math.nan
+    assert ms() < 100 * clean
+    k[1] = math.nan
+    assert ms() < 100 * clean
+
+
 # ------------------------------------------------------------------------------------------------ vocabulary
 def vocab_case(rows, vocab, dim, dtype, std=2.0, seed=0):
     h, w = rnd(seed + 1, rows, dim, dtype=dtype), rnd(seed + 2, vocab, dim, std=std * dim**-0.5, dtype=dtype)
