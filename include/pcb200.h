@@ -845,12 +845,16 @@ int pcb_ntt_batch(PcbCtx* ctx, uint64_t* x, int32_t nrows, int32_t inverse, cuda
 /* What a client computes in the clear on either side of the encrypted decode: the prompt's pass through the layers that
  * gives the K and V rows of the caches (linear, attention), the vocabulary loss of hidden states, and the gradients that
  * fit the head and the MLP to the polynomials of the encrypted step. Operands are 16-bit floats (PCB_BF16 or PCB_F16, one
- * type per call), products and sums 32-bit. A matrix of r rows and c columns is given by its first element and the pitch
- * of its rows in elements, columns adjacent. Pointers are device memory except where said. Every call is stream-ordered,
- * makes no host copy and no sync (it can be captured in a CUDA graph), uses only the caller's workspace (`ws`, 256-byte
- * aligned, at least the bytes that the matching _ws entry returns; that entry is negative when the arguments are refused)
- * and returns 0, -1 (arguments refused, pcb_last_error has the reason) or a cudaError_t. Results do not depend on the
- * order in which blocks run: no floating-point atomics. */
+ * type per call), products and sums 32-bit (the tensor core's accumulators truncate: some 1.2e-9 of a result per term of its
+ * sum). Results are rounded once, and three intermediate values once before, as 16-bit operands of a second product: the
+ * attention's weights and dz of the linear's gradient under an activation (what is computed from them errs about 1.4 times as
+ * much as one rounding), and dl of the vocabulary's (about 1.05 times). A matrix of r rows and c columns is given by its first
+ * element and the pitch of its rows in elements, columns adjacent; what lies between a row's end and the next row is not
+ * written. Pointers are device memory except where said, multiples of their elements' size. Sizes go up to 2^31 - 1025. Every
+ * call is stream-ordered, makes no host copy and no sync (it can be captured in a CUDA graph), uses only the caller's workspace
+ * (`ws`, 256-byte aligned, at least the bytes that the matching _ws entry returns; that entry is negative when the arguments are
+ * refused) and returns 0, -1 (arguments refused, pcb_last_error has the reason) or a cudaError_t. Results do not depend on
+ * the order in which blocks run: no floating-point atomics. */
 enum { PCB_BF16 = 0, PCB_F16 = 1, PCB_F32 = 2 };
 enum { PCB_ACT_NONE = 0, PCB_ACT_GELU = 1, PCB_ACT_POLY = 2 };
 
@@ -873,7 +877,9 @@ int64_t pcb_clear_linear_ws(const PcbClearLinear* a);
 int pcb_clear_linear(const PcbClearLinear* a, void* ws, size_t ws_bytes, cudaStream_t s);
 
 /* The gradients of y = act(x w + bias) for dy (m x n): with z = x w + bias (formed again, not kept by the forward call)
- * and dz = dy act'(z): dx = dz w^T (m x k), dw = x^T dz (in w's own order), db = the sum of dz's rows. dx, dw and db may
+ * and dz = dy act'(z): dx = dz w^T (m x k), dw = x^T dz (in w's own order), db = the sum of dz's rows in 32 bits. Under an
+ * activation dz is rounded to the call's type, in PCB_F16 times a power of two that brings the largest finite dy, times the
+ * largest slope within the polynomial's bound, to 2^8 (no loss above 2^-22 of it; 2^8 of room past it). dx, dw and db may
  * be null (not wanted); bias is null where the forward call had none, db then still the sum. */
 typedef struct PcbClearLinearGrad {
     const void* dy;
@@ -897,7 +903,9 @@ int pcb_clear_linear_grad(const PcbClearLinearGrad* a, void* ws, size_t ws_bytes
  * j <= i + k_lens[b] - q_lens[b] (causal) or every key of its sequence. q, out: q_rows x heads x dim; k, v: k_rows x
  * kv_heads x dim, query head h reads K/V head h / (heads / kv_heads). *_pitch: elements between tokens, *_head: between
  * heads, the dim elements adjacent (dim <= 128). With s = scale <q, k>: ncoef = 0: out = sum softmax(s) v; ncoef = 1..8:
- * out = sum_j p(s_j) v_j, p(s) = sum_i coef[i] s^i, the encrypted step's weights. A query that sees no key gets zeros. */
+ * out = sum_j p(s_j) v_j, p(s) = sum_i coef[i] s^i, the encrypted step's weights. A query that sees no key gets zeros. Keys and
+ * values that a query does not see do not reach it, whatever they hold; one that it sees and that is not finite makes the dims
+ * that it enters not finite (Inf or NaN). */
 typedef struct PcbClearAttention {
     const void* q;
     const void* k;

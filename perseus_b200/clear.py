@@ -8,7 +8,9 @@ polynomial weights that the encrypted step evaluates). After it, the score of hi
 perseus_b200.prefill runs them together.
 
 Operands are CUDA tensors of torch.bfloat16 or torch.float16 (one type per call), sums are 32-bit, results are rounded
-once. Every call runs on the current stream, without a host copy or sync. Results are plain tensors: nothing is recorded
+once. Three intermediate values are rounded to 16 bits as well, as operands of a second product: prompt_attention's weights
+before they meet v, linear_grad's dy act'(z) under an activation (scaled to float16's range), vocab_loss_grad's slopes; what
+is computed from the first two then errs about 1.4 times as much as by its own rounding. Every call runs on the current stream, without a host copy or sync. Results are plain tensors: nothing is recorded
 for autograd.
 """
 import ctypes as C

@@ -8,12 +8,12 @@
 // range for f16), which after the first steps is rare. Under polynomial weights there is no maximum, no sum and no rescaling.
 // Two blocks share an SM: while one's warps compute weights, the other's products run.
 //
-// What bounds it: at 64 dims a step of a block takes 512 cycles of exponentials (16 per cycle and SM; a quarter of them runs on
-// the multiply-add pipe instead) against 256 of products. 8192 tokens, 12 heads over 4: 155 us, 0.66 PFLOP/s, some 890 cycles
-// a step; a warp's own chain (scores' arrival, maximum, exponentials, weights' way back) is 1500 cycles, two of them overlap.
+// What bounds it: a warp's own chain (scores' arrival, maximum, exponentials, weights' way back), 1500 cycles a step, of which two
+// overlap on an SM. 8192 tokens, 12 heads over 4 of 64: 159 us, 0.65 PFLOP/s, some 890 cycles a step of a block, against 256 of
+// products and 384 on the special-function pipe (512 exponentials' worth of cycles, a quarter of them on the multiply-add pipe);
+// under polynomial weights, without any exponentials, 153 us. 128 dims: 197 us, 1.04 PFLOP/s.
 // More warps per row, three or four blocks of one buffer, and blocks that stay for many tiles measured slower (187, 195, 212,
-// 171 us). 128 dims: 0.74 PFLOP/s. Short sequences: a block costs some 4 us besides its steps (24 prompts of 1 to 1024 tokens:
-// 45 us, 1350 blocks).
+// 171 us). Short sequences: a block costs some 4 us besides its steps (24 prompts of 1 to 1024 tokens: 45 us, 1350 blocks).
 //
 // Few rows against many keys (single tokens) split the keys over several blocks, joined in order by `join_splits`.
 //
@@ -664,8 +664,9 @@ int heads_map(CUtensorMap* map, const Heads& h, int type, int dim, int box_heads
     return encode_map(map, type, h.p, 3, size, stride, box);
 }
 
-// Splits of the keys: as many as fill two blocks per SM, each with at least two key blocks, when the tiles alone do not
-// (one launch's worth of sequences; more sequences have tiles enough)
+// Splits of the keys: as many as fill two blocks per SM, each with at least two key blocks, when the tiles alone do not. One
+// launch's worth of sequences only: more of them are walked whole, launch after launch, though with few K/V heads (129 to 295
+// single tokens of one) their tiles do not fill the SMs either.
 int splits_of(const PcbClearAttention* a) {
     const int tokens = ROWS / (a->heads / a->kv_heads);
     int64_t tiles = 0;

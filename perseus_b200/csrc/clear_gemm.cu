@@ -10,10 +10,10 @@
 //
 // What bounds it: a pair's 64-k block of a 256 x 256 tile takes 512 cycles of products, and the loop keeps to 505 to 520 of
 // them; what falls is the clock (1.5 to 1.6 GHz with all tensor cores busy), so what costs energy costs time: 8192 x 8192 x
-// 8192 721 us (1.52 PFLOP/s, 94 % of the measured library rate) with tiles in bands, 790 reading A again for each column.
-// At k = 768 the epilogue shares the time: 8192 x 768 x 3072 31 us plain, 33.8 under the polynomial, 40 under GELU (two
-// special functions per value), 43 with a residual. Short products (1024 x 1024 x 1024 7.5 us) are set-up, one tile's loads
-// and its epilogue.
+// 8192 730 us (1.51 PFLOP/s, 93 % of the measured library rate) with tiles in bands, 790 reading A again for each column.
+// At k = 768 the epilogue shares the time: 8192 x 768 x 3072 31.4 us plain, 34.5 under the polynomial (36.4 with a bias), 41
+// under GELU (two special functions per value), 44 with a 16-bit residual, 58 with a 32-bit one and result. Short products
+// (1024 x 1024 x 1024 8 us) are set-up, one tile's loads and its epilogue.
 // The accumulators are 32-bit and truncate: the error of a result grows with k, about 1.2e-9 k of it.
 //
 // Waits are bounded (mma::wait_warp): a role that gives up tells the others, the loads and products in flight are waited for
@@ -902,8 +902,8 @@ int gemm(const Gemm& g, cudaStream_t s) {
     p.bf16 = g.type == PCB_BF16;
     p.a_bytes = arows * BK * 2;
     // Where A stays in L2, tiles go down all of its rows, column after column; a larger A is read again for each column, and
-    // bands of 2048 rows, about square over a round, read less of both (8192 x 8192 x 8192: 722 us against 790,
-    // 50000 x 4096 x 768: 225 against 263; 4096 x 768 x 50000, whose A takes 6 MB, 245 down all rows against 252)
+    // bands of 2048 rows, about square over a round, read less of both (8192 x 8192 x 8192: 730 us against 790,
+    // 50000 x 4096 x 768: 225 against 263; 4096 x 768 x 50000, whose A takes 6 MB, 241 down all rows against 252)
     p.band = pl.bn == 256 && tm > 8 && 2.0 * g.m * g.k > 64e6 ? 8 : 0;
     p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.kblocks = (g.k + BK - 1) / BK;
     p.whole = pl.whole, p.tail = (int)(tm * tn) - pl.whole, p.splits = pl.splits, p.kper = pl.kper, p.slices = g.slices;
