@@ -116,12 +116,11 @@ def fit_step(r, targets, tail, cfg, ignore=-100, poly=True):
     count = scored.sum().clamp_min(1.0)
     weight = scored / count
     # float16 ends at 65504 and loses bits below 2^-14: 64 leaves room for gradients of 1000, and for rows by the thousands
-    half = y.dtype is torch.float16
-    scale = count.clamp_max(64.0)
-    dy, dhead = clear.vocab_loss_grad(y, tail.head, targets, lse, weight * scale if half else weight, ignore)
+    scale = count.clamp_max(64.0) if y.dtype is torch.float16 else None
+    dy, dhead = clear.vocab_loss_grad(y, tail.head, targets, lse, weight if scale is None else weight * scale, ignore)
     du, dw_down, db_down = clear.linear_grad(dy, u, w.w_down, bias=w.b_down)
     _, dw_up, db_up = clear.linear_grad(du, n, w.w_up, bias=w.b_up, act=act, needs=(False, True, True))
     grads = {"head": dhead, "w_up": dw_up, "b_up": db_up, "w_down": dw_down, "b_down": db_down}
-    if half:
+    if scale is not None:
         grads = {n: g.float() / scale for n, g in grads.items()}
     return (loss * weight).sum(), grads
